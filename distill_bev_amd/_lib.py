@@ -169,9 +169,20 @@ _SIGNATURES = {
     "dbev_bn_dual_train_forward_mask": [_p, _p, _p, _p, _p, _p, _p, _f, _f, _p, _p, _p, _p, _p, _f, _f, _i, _p, _p, _p, _p, _p, _p, _p,
                                         _ll, _i, _p, _i, _p, _i, _p, _p, _sz, _p],
     "dbev_bn_dual_backward3": [_p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _ll, _i, _p, _sz, _p],
+    "dbev_act8_pack": [_p, _i, _ll, _i, _ll, _i, _p, _p, _p],
+    "dbev_act8_unpack": [_p, _p, _i, _ll, _i, _p, _i, _p],
+    "dbev_act8_activation_forward": [_p, _i, _ll, _i, _ll, _i, _i, _p, _p, _p, _p],
+    "dbev_act8_activation_backward": [_p, _i, _ll, _p, _p, _i, _ll, _i, _i, _p, _p],
+    "dbev_act8_weight_gradient_workspace_bytes": [_ll, _i, _i],
+    "dbev_act8_weight_gradient": [_p, _i, _p, _p, _i, _ll, _i, _i, _p, _p, _p, _sz, _p],
+    "dbev_gn_act_workspace_bytes": [_i, _ll, _i, _i],
+    "dbev_gn_act_forward": [_p, _i, _i, _ll, _i, _i, _p, _p, _f, _i, _p, _p, _p, _i, _p, _p, _p, _sz, _p],
+    "dbev_gn_act_backward": [_p, _i, _p, _i, _p, _p, _i, _ll, _i, _i, _p, _p, _p, _p, _i, _p, _p, _p, _p, _sz, _p],
 }
 _RESTYPES = {"dbev_target_arch": ctypes.c_char_p,
              "dbev_wino_filter_floats": ctypes.c_longlong,
+             "dbev_act8_weight_gradient_workspace_bytes": ctypes.c_size_t,
+             "dbev_gn_act_workspace_bytes": ctypes.c_size_t,
              "dbev_stem7x7s2_workspace_bytes": ctypes.c_longlong,
              "dbev_stem_pool_norm_backward_workspace_bytes": ctypes.c_size_t,
              "dbev_gemm1x1_backward_weight_workspace_bytes": ctypes.c_size_t,
@@ -325,7 +336,7 @@ def kernel_timing_read():
     return out
 
 
-FALLBACK_SITES = {"bn_act": 0, "skinny_conv": 1, "adapt_mse": 2, "pillar_vfe": 3, "head_batch": 4, "depth_head": 5}   # DBEV_FB_*
+FALLBACK_SITES = {"bn_act": 0, "skinny_conv": 1, "adapt_mse": 2, "pillar_vfe": 3, "head_batch": 4, "depth_head": 5, "gn_act": 6, "act8": 7}   # DBEV_FB_*
 _warned_fallbacks = set()
 
 

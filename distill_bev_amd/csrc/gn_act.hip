@@ -1,0 +1,531 @@
+// Group norm + activation, channels-last: y = act((x - mean_g) rstd_g gamma + beta), statistics per (image, group) over S pixels x C / G
+// channels; forward (training or inference, optionally with an 8-bit checkpoint of x, act8.h) and backward (from x or the checkpoint).
+//
+// Forward, two launches, no finalize launch between them:
+//   gn_stats   a workgroup owns a chunk of one image's pixels x a range of channels, a thread one vector column; sums of (x - K_c) and
+//              (x - K_c)^2 with K_c the chunk's first pixel: an offset of the data costs no digits.  Reduced to (mean, M2) per group
+//              and chunk in LDS.
+//   gn_apply   every workgroup merges its image's chunk statistics itself -- a few KB from L2 against its share of x -- in fp64
+//              (M2 = sum of M2_i + n_i (mean_i - mean)^2), then y, and the checkpoint from the same registers.
+// Backward, two launches, xh = (x - mean) rstd, g = dy act'(gamma xh + beta):
+//   gn_bwd_reduce   per chunk: sums of g and g xh per channel (for dbeta, dgamma), weighted with gamma per group (A, B)
+//   gn_bwd_dx       dx = rstd (gamma g - A / D - xh B / D), D = S C / G; its first workgroups add the per-channel rows up instead
+// Bound by HBM: 3 n es forward and 5 n es backward (n es = bytes of x; with a checkpoint the two reads of x in the backward are 1.03
+// bytes a value).  All sums have a fixed order: run-to-run bit-identical, no atomics.
+#include "act8.h"
+
+namespace {
+
+constexpr int GN_U = 4;                                       // rows in flight per thread
+
+struct GnArgs {
+  long long S;                                                // pixels of an image
+  int C, cv, G, cpg, nb;                                      // channels, vector columns, groups, channels a group, blocks of 32 a row
+  int nchunk;
+  long long rows_per;                                         // pixels a chunk
+  A8Tile t;
+};
+
+// (image, pixel chunk, column range) of this workgroup
+struct GnPos { int n, chunk, cc, col, c0, c1, g0, g1, rp; bool on; long long r0, r1; };
+__device__ __forceinline__ GnPos gn_pos(const GnArgs& a, int block, int V) {
+  GnPos p;
+  p.cc = block % a.t.ncol;
+  const int b = block / a.t.ncol;
+  p.chunk = b % a.nchunk;
+  p.n = b / a.nchunk;
+  p.rp = threadIdx.x / a.t.CH;
+  p.col = p.cc * a.t.CH + (threadIdx.x - p.rp * a.t.CH);
+  p.on = p.rp < a.t.RP && p.col < a.cv;
+  p.c0 = p.cc * a.t.CH * V;
+  p.c1 = min(a.C, p.c0 + a.t.CH * V);
+  p.g0 = p.c0 / a.cpg;
+  p.g1 = (p.c1 - 1) / a.cpg + 1;
+  p.r0 = p.chunk * a.rows_per;
+  p.r1 = min(a.S, p.r0 + a.rows_per);
+  return p;
+}
+
+// lanes that share one group's work: the workgroup's threads spread over its groups, at most a wave each
+__device__ __forceinline__ int gn_lanes(int ng) {
+  int l = 64;
+  while (l > 1 && ng * l > static_cast<int>(blockDim.x)) l >>= 1;
+  return l;
+}
+template <typename F>
+__device__ __forceinline__ F gn_lane_sum(F v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// the two per-thread sums of every column -> per channel in sh[0 .. CH V), sh[CH V ..): row phases added in order
+template <int V>
+__device__ __forceinline__ void gn_fold(float* sh, const GnArgs& a, const GnPos& p, const float* s, const float* q) {
+  const int w = a.t.CH * V, lane = threadIdx.x - p.rp * a.t.CH;
+  float* t1 = sh + 2 * w;                                     // [RP][CH V] twice
+  float* t2 = t1 + a.t.RP * w;
+  if (p.rp < a.t.RP) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      t1[p.rp * w + lane * V + i] = s[i];
+      t2[p.rp * w + lane * V + i] = q[i];
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < w; c += blockDim.x) {
+    float a1 = 0.f, a2 = 0.f;
+    for (int r = 0; r < a.t.RP; ++r) {
+      a1 += t1[r * w + c];
+      a2 += t2[r * w + c];
+    }
+    sh[c] = a1;
+    sh[w + c] = a2;
+  }
+  __syncthreads();
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void gn_stats(const T* __restrict__ x, GnArgs a, float2* __restrict__ part) {
+  extern __shared__ float sh[];
+  const GnPos p = gn_pos(a, blockIdx.x, V);
+  const T* xi = x + static_cast<size_t>(p.n) * a.S * a.C + static_cast<size_t>(p.on ? p.col : 0) * V;
+  float k[V], s[V], q[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) k[i] = s[i] = q[i] = 0.f;
+  if (p.on) {
+    A8Vec<T, V>::load(xi + p.r0 * a.C, k);
+    const long long step = static_cast<long long>(a.t.RP) * GN_U;
+    for (long long r = p.r0 + p.rp; r < p.r1; r += step) {
+      float v[GN_U][V];
+#pragma unroll
+      for (int u = 0; u < GN_U; ++u) {
+        const long long ru = r + u * a.t.RP;
+        if (ru < p.r1) A8Vec<T, V>::load(xi + ru * a.C, v[u]);
+        else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[u][i] = k[i];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < GN_U; ++u)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = v[u][i] - k[i];
+          s[i] += d;
+          q[i] = fmaf(d, d, q[i]);
+        }
+    }
+  }
+  gn_fold<V>(sh, a, p, s, q);
+  // per channel: mean and M2 of the chunk's pixels
+  const int w = a.t.CH * V;
+  const float rows = static_cast<float>(p.r1 - p.r0);
+  const T* x0 = x + static_cast<size_t>(p.n) * a.S * a.C + p.r0 * a.C + p.c0;
+  for (int c = threadIdx.x; c < p.c1 - p.c0; c += blockDim.x) {
+    const float d = sh[c] / rows;
+    sh[w + c] = fmaxf(sh[w + c] - sh[c] * d, 0.f) + 0.f * d;  // (a NaN stays one)
+    sh[c] = static_cast<float>(x0[c]) + d;
+  }
+  __syncthreads();
+  const int ng = p.g1 - p.g0, lanes = gn_lanes(ng), sub = threadIdx.x % lanes;
+  for (int gi = threadIdx.x / lanes; gi < ng; gi += blockDim.x / lanes) {
+    const int g = p.g0 + gi, cb = max(p.c0, g * a.cpg) - p.c0, ce = min(p.c1, (g + 1) * a.cpg) - p.c0;
+    float m = 0.f;
+    for (int c = cb + sub; c < ce; c += lanes) m += sh[c];
+    m = gn_lane_sum(m, lanes) / static_cast<float>(ce - cb);
+    float m2 = 0.f;
+    for (int c = cb + sub; c < ce; c += lanes) {
+      const float d = sh[c] - m;
+      m2 += fmaf(rows * d, d, sh[w + c]);
+    }
+    m2 = gn_lane_sum(m2, lanes);
+    if (sub == 0) part[((static_cast<size_t>(p.n) * a.nchunk + p.chunk) * a.t.ncol + p.cc) * a.G + g] = make_float2(m, m2);
+  }
+}
+
+// mean and rstd of the groups this workgroup touches -> sh[2 (g - g0)], merged in fp64 over the image's chunks
+__device__ __forceinline__ void gn_merge_stats(float* sh, const GnArgs& a, const GnPos& p, int V, const float2* __restrict__ part, float eps) {
+  const int ng = p.g1 - p.g0, lanes = gn_lanes(ng), sub = threadIdx.x % lanes;
+  const int w = a.t.CH * V;
+  for (int gi = threadIdx.x / lanes; gi < ng; gi += blockDim.x / lanes) {
+    const int g = p.g0 + gi, cca = g * a.cpg / w, ccb = ((g + 1) * a.cpg - 1) / w + 1;
+    const double D = static_cast<double>(a.S) * a.cpg;
+    double m = 0.0;
+    for (int cc = cca; cc < ccb; ++cc) {
+      const int width = min((cc + 1) * w, (g + 1) * a.cpg) - max(cc * w, g * a.cpg);
+      for (int k = sub; k < a.nchunk; k += lanes) {
+        const double cnt = static_cast<double>(min(a.S, (k + 1) * a.rows_per) - k * a.rows_per) * width;
+        m += cnt * part[((static_cast<size_t>(p.n) * a.nchunk + k) * a.t.ncol + cc) * a.G + g].x;
+      }
+    }
+    m = gn_lane_sum(m, lanes) / D;
+    double m2 = 0.0;
+    for (int cc = cca; cc < ccb; ++cc) {
+      const int width = min((cc + 1) * w, (g + 1) * a.cpg) - max(cc * w, g * a.cpg);
+      for (int k = sub; k < a.nchunk; k += lanes) {
+        const double cnt = static_cast<double>(min(a.S, (k + 1) * a.rows_per) - k * a.rows_per) * width;
+        const float2 e = part[((static_cast<size_t>(p.n) * a.nchunk + k) * a.t.ncol + cc) * a.G + g];
+        m2 += e.y + cnt * (e.x - m) * (e.x - m);
+      }
+    }
+    m2 = gn_lane_sum(m2, lanes) / D;
+    if (sub == 0) {
+      sh[2 * gi] = static_cast<float>(m);
+      sh[2 * gi + 1] = static_cast<float>(1.0 / sqrt(m2 + static_cast<double>(eps)));
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int V, int FMT, int ACT>
+__global__ __launch_bounds__(256) void gn_apply(const T* __restrict__ x, GnArgs a, const float2* __restrict__ part, const float* __restrict__ gamma,
+                                                const float* __restrict__ beta, float eps, T* __restrict__ y, float* __restrict__ mean,
+                                                float* __restrict__ rstd, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  extern __shared__ float sh[];
+  constexpr int LB = 32 / V;
+  const GnPos p = gn_pos(a, blockIdx.x, V);
+  gn_merge_stats(sh, a, p, V, part, eps);
+  if (mean != nullptr && p.chunk == 0)
+    for (int gi = threadIdx.x; gi < p.g1 - p.g0; gi += blockDim.x)
+      if ((p.g0 + gi) * a.cpg >= p.c0) {                      // the column range in which the group begins
+        mean[static_cast<size_t>(p.n) * a.G + p.g0 + gi] = sh[2 * gi];
+        rstd[static_cast<size_t>(p.n) * a.G + p.g0 + gi] = sh[2 * gi + 1];
+      }
+  if (p.rp >= a.t.RP) return;
+  float mu[V], sc[V], bt[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = p.on ? p.col * V + i : 0, gi = p.on ? c / a.cpg - p.g0 : 0;
+    mu[i] = sh[2 * gi];
+    sc[i] = sh[2 * gi + 1] * (gamma != nullptr ? gamma[c] : 1.f);
+    bt[i] = beta != nullptr ? beta[c] : 0.f;
+  }
+  const size_t base = static_cast<size_t>(p.n) * a.S;
+  const long long step = static_cast<long long>(a.t.RP) * GN_U;
+  for (long long r = p.r0 + p.rp; r < p.r1; r += step) {
+    float v[GN_U][V];
+#pragma unroll
+    for (int u = 0; u < GN_U; ++u) {
+      const long long ru = r + u * a.t.RP;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[u][i] = 0.f;
+      if (p.on && ru < p.r1) A8Vec<T, V>::load(x + (base + ru) * a.C + static_cast<size_t>(p.col) * V, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < GN_U; ++u) {
+      const long long ru = r + u * a.t.RP;
+      if (ru >= p.r1) break;                                  // all lanes of a block are on the same pixel
+      const size_t o = (base + ru) * a.C + static_cast<size_t>(p.col) * V;
+      if (FMT != DBEV_ACT8_NONE) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(v[u][i]) & 0x7fffffffu);
+        const unsigned b = a8_scale_byte<FMT>(a8_block_max<V>(m));
+        if (p.on) {
+          *reinterpret_cast<typename A8Bytes<V>::type*>(codes + o) = a8_encode<FMT, V>(v[u], b);
+          if (p.col % LB == 0) scales[(base + ru) * a.nb + p.col / LB] = static_cast<uint8_t>(b);
+        }
+      }
+      if (p.on) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[u][i] = a8_act<ACT>(fmaf(v[u][i] - mu[i], sc[i], bt[i]));
+        A8Vec<T, V>::store(y + o, v[u]);
+      }
+    }
+  }
+}
+
+// one vector of the backward pass's view of x: x itself or its checkpoint
+template <typename T, int V, int FMT>
+struct GnX {
+  typename A8Bytes<V>::type c;
+  unsigned b;
+  float v[V];
+  __device__ __forceinline__ void load(const T* x, const uint8_t* codes, const uint8_t* scales, size_t row, int C, int nb, int col) {
+    if (FMT == DBEV_ACT8_NONE) A8Vec<T, V>::load(x + row * C + static_cast<size_t>(col) * V, v);
+    else {
+      c = *reinterpret_cast<const typename A8Bytes<V>::type*>(codes + row * C + static_cast<size_t>(col) * V);
+      b = scales[row * nb + col / (32 / V)];
+    }
+  }
+  __device__ __forceinline__ void get(float* o) const {
+    if (FMT == DBEV_ACT8_NONE) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = v[i];
+    } else a8_decode<FMT, V>(c, a8_scale(b), o);
+  }
+};
+
+struct GnCoef { const float *gamma, *beta, *mean, *rstd; };
+
+template <typename T, int V, int FMT, int ACT>
+__global__ __launch_bounds__(256) void gn_bwd_reduce(const T* __restrict__ gy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
+                                                     const uint8_t* __restrict__ scales, GnArgs a, GnCoef k, float2* __restrict__ pc,
+                                                     float2* __restrict__ pg) {
+  extern __shared__ float sh[];
+  const GnPos p = gn_pos(a, blockIdx.x, V);
+  float s[V], q[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = q[i] = 0.f;
+  if (p.on) {
+    float mu[V], rs[V], gm[V], bt[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = p.col * V + i;
+      mu[i] = k.mean[static_cast<size_t>(p.n) * a.G + c / a.cpg];
+      rs[i] = k.rstd[static_cast<size_t>(p.n) * a.G + c / a.cpg];
+      gm[i] = k.gamma != nullptr ? k.gamma[c] : 1.f;
+      bt[i] = k.beta != nullptr ? k.beta[c] : 0.f;
+    }
+    const size_t base = static_cast<size_t>(p.n) * a.S;
+    const long long step = static_cast<long long>(a.t.RP) * GN_U;
+    for (long long r = p.r0 + p.rp; r < p.r1; r += step) {
+      float d[GN_U][V];
+      GnX<T, V, FMT> xv[GN_U];
+#pragma unroll
+      for (int u = 0; u < GN_U; ++u) {
+        const long long ru = r + u * a.t.RP;
+        if (ru < p.r1) {
+          A8Vec<T, V>::load(gy + (base + ru) * a.C + static_cast<size_t>(p.col) * V, d[u]);
+          xv[u].load(x, codes, scales, base + ru, a.C, a.nb, p.col);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < GN_U; ++u) {
+        if (r + u * a.t.RP >= p.r1) break;
+        float v[V];
+        xv[u].get(v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float xh = (v[i] - mu[i]) * rs[i];
+          const float g = a8_act_grad<ACT>(d[u][i], fmaf(xh, gm[i], bt[i]));
+          s[i] += g;
+          q[i] = fmaf(g, xh, q[i]);
+        }
+      }
+    }
+  }
+  gn_fold<V>(sh, a, p, s, q);
+  const int w = a.t.CH * V;
+  float2* row = pc + (static_cast<size_t>(p.n) * a.nchunk + p.chunk) * a.C + p.c0;
+  for (int c = threadIdx.x; c < p.c1 - p.c0; c += blockDim.x) row[c] = make_float2(sh[c], sh[w + c]);
+  const int ng = p.g1 - p.g0, lanes = gn_lanes(ng), sub = threadIdx.x % lanes;
+  for (int gi = threadIdx.x / lanes; gi < ng; gi += blockDim.x / lanes) {
+    const int g = p.g0 + gi, cb = max(p.c0, g * a.cpg) - p.c0, ce = min(p.c1, (g + 1) * a.cpg) - p.c0;
+    float A = 0.f, B = 0.f;
+    for (int c = cb + sub; c < ce; c += lanes) {
+      const float gm = k.gamma != nullptr ? k.gamma[p.c0 + c] : 1.f;
+      A = fmaf(gm, sh[c], A);
+      B = fmaf(gm, sh[w + c], B);
+    }
+    A = gn_lane_sum(A, lanes);
+    B = gn_lane_sum(B, lanes);
+    if (sub == 0) pg[((static_cast<size_t>(p.n) * a.nchunk + p.chunk) * a.t.ncol + p.cc) * a.G + g] = make_float2(A, B);
+  }
+}
+
+constexpr int GN_PC = 8;                                      // channels of a workgroup that adds the parameter gradients up (64-byte pieces of a row)
+
+// dgamma, dbeta: the rows of pc added in a fixed order, fp64 (a row is one chunk's fp32 sum)
+__device__ __forceinline__ void gn_param_grads(double* sh, const GnArgs& a, int N, int block, const float2* __restrict__ pc, float* __restrict__ dgamma,
+                                               float* __restrict__ dbeta) {
+  const int c = block * GN_PC + threadIdx.x % GN_PC, ph = threadIdx.x / GN_PC, np = blockDim.x / GN_PC;
+  const long long rows = static_cast<long long>(N) * a.nchunk;
+  double s = 0.0, q = 0.0;
+  if (c < a.C) {
+#pragma unroll 4
+    for (long long r = ph; r < rows; r += np) {
+      const float2 e = pc[r * a.C + c];
+      s += e.x;
+      q += e.y;
+    }
+  }
+  sh[2 * threadIdx.x] = s;
+  sh[2 * threadIdx.x + 1] = q;
+  __syncthreads();
+  if (ph == 0 && c < a.C) {
+    for (int i = 1; i < np; ++i) {
+      s += sh[2 * (threadIdx.x + i * GN_PC)];
+      q += sh[2 * (threadIdx.x + i * GN_PC) + 1];
+    }
+    if (dbeta != nullptr) dbeta[c] = static_cast<float>(s);
+    if (dgamma != nullptr) dgamma[c] = static_cast<float>(q);
+  }
+}
+
+template <typename T, int V, int FMT, int ACT>
+__global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
+                                                 const uint8_t* __restrict__ scales, GnArgs a, GnCoef k, const float2* __restrict__ pc,
+                                                 const float2* __restrict__ pg, int N, int npar, T* __restrict__ dx, float* __restrict__ dgamma,
+                                                 float* __restrict__ dbeta) {
+  extern __shared__ float sh[];
+  if (static_cast<int>(blockIdx.x) < npar) {
+    gn_param_grads(reinterpret_cast<double*>(sh), a, N, blockIdx.x, pc, dgamma, dbeta);
+    return;
+  }
+  const GnPos p = gn_pos(a, static_cast<int>(blockIdx.x) - npar, V);
+  const int ng = p.g1 - p.g0, lanes = gn_lanes(ng), sub = threadIdx.x % lanes, w = a.t.CH * V;
+  const double D = static_cast<double>(a.S) * a.cpg;
+  for (int gi = threadIdx.x / lanes; gi < ng; gi += blockDim.x / lanes) {
+    const int g = p.g0 + gi, cca = g * a.cpg / w, ccb = ((g + 1) * a.cpg - 1) / w + 1;
+    double A = 0.0, B = 0.0;
+    for (int cc = cca; cc < ccb; ++cc)
+      for (int c = sub; c < a.nchunk; c += lanes) {
+        const float2 e = pg[((static_cast<size_t>(p.n) * a.nchunk + c) * a.t.ncol + cc) * a.G + g];
+        A += e.x;
+        B += e.y;
+      }
+    A = gn_lane_sum(A, lanes);
+    B = gn_lane_sum(B, lanes);
+    if (sub == 0) {
+      sh[2 * gi] = static_cast<float>(A / D);
+      sh[2 * gi + 1] = static_cast<float>(B / D);
+    }
+  }
+  __syncthreads();
+  if (!p.on) return;
+  float mu[V], rs[V], gm[V], bt[V], A[V], B[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = p.col * V + i, g = c / a.cpg;
+    mu[i] = k.mean[static_cast<size_t>(p.n) * a.G + g];
+    rs[i] = k.rstd[static_cast<size_t>(p.n) * a.G + g];
+    gm[i] = k.gamma != nullptr ? k.gamma[c] : 1.f;
+    bt[i] = k.beta != nullptr ? k.beta[c] : 0.f;
+    A[i] = sh[2 * (g - p.g0)];
+    B[i] = sh[2 * (g - p.g0) + 1];
+  }
+  const size_t base = static_cast<size_t>(p.n) * a.S;
+  const long long step = static_cast<long long>(a.t.RP) * GN_U;
+  for (long long r = p.r0 + p.rp; r < p.r1; r += step) {
+    float d[GN_U][V];
+    GnX<T, V, FMT> xv[GN_U];
+#pragma unroll
+    for (int u = 0; u < GN_U; ++u) {
+      const long long ru = r + u * a.t.RP;
+      if (ru < p.r1) {
+        A8Vec<T, V>::load(gy + (base + ru) * a.C + static_cast<size_t>(p.col) * V, d[u]);
+        xv[u].load(x, codes, scales, base + ru, a.C, a.nb, p.col);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < GN_U; ++u) {
+      const long long ru = r + u * a.t.RP;
+      if (ru >= p.r1) break;
+      float v[V];
+      xv[u].get(v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float xh = (v[i] - mu[i]) * rs[i];
+        const float g = a8_act_grad<ACT>(d[u][i], fmaf(xh, gm[i], bt[i]));
+        v[i] = rs[i] * (fmaf(gm[i], g, -A[i]) - xh * B[i]);
+      }
+      A8Vec<T, V>::store(dx + (base + ru) * a.C + static_cast<size_t>(p.col) * V, v);
+    }
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------
+// chunks per image: enough workgroups for eight per CU over the whole batch, at least two rounds of loads per thread, at most 128 (every
+// workgroup of the second launch merges its image's chunk rows)
+GnArgs gn_args(int N, long long S, int C, int G, int V) {
+  GnArgs a;
+  a.S = S;
+  a.C = C;
+  a.cv = C / V;
+  a.G = G;
+  a.cpg = C / G;
+  a.nb = (C + 31) / 32;
+  a.t = a8_tile(C, V);
+  long long want = (2048 + static_cast<long long>(N) * a.t.ncol - 1) / (static_cast<long long>(N) * a.t.ncol);
+  const long long least = 2LL * a.t.RP * GN_U;
+  want = want < 1 ? 1 : want > 128 ? 128 : want;
+  const long long most = (S + least - 1) / least;
+  if (want > most) want = most;
+  a.rows_per = (S + want - 1) / want;
+  a.nchunk = static_cast<int>((S + a.rows_per - 1) / a.rows_per);
+  return a;
+}
+
+size_t gn_lds(const GnArgs& a, int V) {
+  const size_t fold = static_cast<size_t>(2) * a.t.CH * V * (1 + a.t.RP) * sizeof(float), merge = static_cast<size_t>(2) * (a.G < a.t.CH * V ? a.G : a.t.CH * V) * sizeof(float);
+  const size_t par = static_cast<size_t>(2) * a.t.threads * sizeof(double);
+  const size_t m = fold > merge ? fold : merge;
+  return m > par ? m : par;
+}
+
+bool gn_ok(int dtype, int N, long long S, int C, int G) {
+  return a8_dtype_ok(dtype) && N >= 0 && S >= 0 && C > 0 && G > 0 && C % G == 0 && C <= 65536 && S <= (1LL << 36) / C &&
+         static_cast<long long>(N) <= (1LL << 22) && (N == 0 || S <= (1LL << 40) / C / N);
+}
+
+// a launch holds fewer than 2^32 threads
+bool gn_grid_ok(int N, const GnArgs& a) { return static_cast<long long>(N) * a.nchunk * a.t.ncol * a.t.threads < (1LL << 32) - (1LL << 26); }
+
+// the plan is made for the narrowest vector width as well: the chunk counts differ, the workspace fits either
+size_t gn_ws(int N, long long S, int C, int G) {
+  size_t m = 0;
+  for (int v : {1, 2, 4, 8}) {
+    if (C % v != 0) continue;
+    const GnArgs a = gn_args(N, S, C, G, v);
+    const size_t b = static_cast<size_t>(N) * a.nchunk * (static_cast<size_t>(a.C) + static_cast<size_t>(a.t.ncol) * a.G) * sizeof(float2);
+    m = b > m ? b : m;
+  }
+  return m;
+}
+
+}  // namespace
+
+extern "C" size_t dbev_gn_act_workspace_bytes(int N, long long S, int C, int G) {
+  if (!gn_ok(DBEV_DT_F32, N, S, C, G) || N == 0 || S == 0) return 0;
+  return gn_ws(N, S, C, G);
+}
+
+extern "C" int dbev_gn_act_forward(const void* x, int dtype, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps,
+                                   int act, void* y, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales, void* workspace,
+                                   size_t workspace_bytes, dbevStream_t stream) {
+  if (!gn_ok(dtype, N, S, C, G) || !a8_act_ok(act) || !(fmt == DBEV_ACT8_NONE || a8_fmt_ok(fmt))) return DBEV_EINVAL;
+  if (N == 0 || S == 0) return 0;
+  if (workspace_bytes < gn_ws(N, S, C, G)) return DBEV_EINVAL;
+  const int vec = a8_pick_vec(a8_elem_size(dtype), C, C, x, y, nullptr);
+  hipStream_t st = dbev_stream(stream);
+  float2* part = static_cast<float2*>(workspace);
+  A8_TYPE_SWITCH(dtype, vec, {
+    const GnArgs a = gn_args(N, S, C, G, V);
+    if ((fmt != DBEV_ACT8_NONE && reinterpret_cast<uintptr_t>(codes) % V != 0) || !gn_grid_ok(N, a)) return DBEV_EINVAL;
+    const dim3 grid(static_cast<unsigned>(N) * a.nchunk * a.t.ncol), block(a.t.threads);
+    hipLaunchKernelGGL((gn_stats<T, V>), grid, block, gn_lds(a, V), st, static_cast<const T*>(x), a, part);
+    DBEV_LAUNCH_CHECK();
+    A8_ACT_SWITCH(act, A8_FMT_SWITCH(fmt, hipLaunchKernelGGL((gn_apply<T, V, FMT, ACT>), grid, block, gn_lds(a, V), st, static_cast<const T*>(x), a, part,
+                                                             gamma, beta, eps, static_cast<T*>(y), mean, rstd, codes, scales)));
+  });
+  DBEV_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" int dbev_gn_act_backward(const void* gy, int dtype, const void* x, int fmt, const uint8_t* codes, const uint8_t* scales, int N, long long S,
+                                    int C, int G, const float* gamma, const float* beta, const float* mean, const float* rstd, int act, void* dx,
+                                    float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, dbevStream_t stream) {
+  if (!gn_ok(dtype, N, S, C, G) || !a8_act_ok(act) || !(fmt == DBEV_ACT8_NONE ? x != nullptr : a8_fmt_ok(fmt))) return DBEV_EINVAL;
+  if (N == 0 || S == 0) return 0;
+  if (workspace_bytes < gn_ws(N, S, C, G)) return DBEV_EINVAL;
+  const int vec = a8_pick_vec(a8_elem_size(dtype), C, C, gy, dx, fmt == DBEV_ACT8_NONE ? x : nullptr);
+  hipStream_t st = dbev_stream(stream);
+  const GnCoef k = {gamma, beta, mean, rstd};
+  A8_TYPE_SWITCH(dtype, vec, {
+    const GnArgs a = gn_args(N, S, C, G, V);
+    if ((fmt != DBEV_ACT8_NONE && reinterpret_cast<uintptr_t>(codes) % V != 0) || !gn_grid_ok(N, a)) return DBEV_EINVAL;
+    float2* pc = static_cast<float2*>(workspace);
+    float2* pg = pc + static_cast<size_t>(N) * a.nchunk * C;
+    const unsigned blocks = static_cast<unsigned>(N) * a.nchunk * a.t.ncol;
+    const int npar = (dgamma != nullptr || dbeta != nullptr) ? (C + GN_PC - 1) / GN_PC : 0;
+    A8_ACT_SWITCH(act, A8_FMT_SWITCH(fmt, {
+      hipLaunchKernelGGL((gn_bwd_reduce<T, V, FMT, ACT>), dim3(blocks), dim3(a.t.threads), gn_lds(a, V), st, static_cast<const T*>(gy),
+                         static_cast<const T*>(x), codes, scales, a, k, pc, pg);
+      hipLaunchKernelGGL((gn_bwd_dx<T, V, FMT, ACT>), dim3(blocks + npar), dim3(a.t.threads), gn_lds(a, V), st, static_cast<const T*>(gy),
+                         static_cast<const T*>(x), codes, scales, a, k, pc, pg, N, npar, static_cast<T*>(dx), dgamma, dbeta);
+    }));
+  });
+  DBEV_LAUNCH_CHECK();
+  return 0;
+}

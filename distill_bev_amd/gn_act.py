@@ -1,0 +1,200 @@
+"""GroupNorm fused with the activation behind it, channels-last, optionally trained from an 8-bit checkpoint (csrc/gn_act.hip).
+
+Host-side mirror of ``norm_cfg=dict(type='GN', num_groups=G)`` layers: nn.GroupNorm -> activation of the ConvModules (mmcv order
+conv -> norm -> act; mmdet3d/models/necks/fpn.py:77-95, lss_fpn.py:30-60).  Unlike the BatchNorm kernels (bn_act.py) these take float32,
+bfloat16 and float16, any channel count, ReLU, SiLU and GELU, and any [N, C, *] shape: two launches forward, two backward, nothing but
+the output written and -- under autograd -- x or its checkpoint kept (act8.py: 1.03 bytes a value, written by the forward's own pass).
+
+    group_norm_act(x, num_groups, weight, bias, eps, act="silu", checkpoint="int8")     # F.group_norm + activation
+    gn_act(x, gn, act, checkpoint)                                                       # the same with a module's parameters
+    GroupNormAct                                                                         # nn.GroupNorm + activation, same state-dict keys
+    fuse_gn_act_modules(model, checkpoint=None)                                          # rewires a built model
+
+`group_norm_act` raises on what the kernels cannot take (a tensor in another layout is copied to channels-last first); the modules leave
+CPU and float64 tensors to the stock operators (device tensors are counted in the fallback ledger)."""
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import act8 as A
+
+_STOCK = {"none": lambda t: t, "relu": F.relu, "silu": F.silu, "gelu": F.gelu}
+
+
+def _maps(x):
+    """x [N, C, *] as a tensor whose memory is dense [N, *, C] (x itself if it is), and its pixels per image"""
+    N, C = x.shape[:2]
+    S = 1
+    for d in x.shape[2:]:
+        S *= d
+    t = x.movedim(1, -1)
+    return (x if t.is_contiguous() else t.contiguous().movedim(-1, 1)), N, C, S
+
+
+def _f32(t):
+    return None if t is None else t.detach().float().contiguous()
+
+
+def _forward(x, G, weight, bias, eps, act, fmt, stats):
+    """x dense channels-last -> y, mean, rstd (None without `stats`), codes, scales (None without `fmt`)"""
+    dev = x.device
+    N, C = x.shape[:2]
+    S = x.numel() // max(1, N * C)
+    y = A.empty_dense(x.shape, 1, x.dtype, dev)
+    mean = torch.empty((N, G), dtype=torch.float32, device=dev) if stats else None
+    rstd = torch.empty((N, G), dtype=torch.float32, device=dev) if stats else None
+    codes, scales = A._buffers(N * S, C, dev) if fmt else (None, None)
+    if x.numel():
+        nbytes = int(L.call("dbev_gn_act_workspace_bytes", N, S, C, G))
+        if nbytes == 0:
+            raise L.DbevHipError(f"group_norm_act: unsupported size {tuple(x.shape)}, {G} groups")
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        L.call("dbev_gn_act_forward", L.ptr(x), A.DTYPES[x.dtype], N, S, C, G, L.ptr(weight), L.ptr(bias), float(eps), A.ACTS[act], L.ptr(y),
+               L.ptr(mean), L.ptr(rstd), A.FORMATS[fmt] if fmt else 0, L.ptr(codes), L.ptr(scales), L.ptr(ws), nbytes, L.stream_ptr(dev),
+               alg_bytes=3 * x.numel() * x.element_size() + (x.numel() if fmt else 0))
+    return y, mean, rstd, codes, scales
+
+
+class _GroupNormAct(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, G, eps, act, fmt):
+        with torch.cuda.device(x.device):
+            xd = _maps(x)[0]
+            w, b = _f32(weight), _f32(bias)
+            y, mean, rstd, codes, scales = _forward(xd, G, w, b, eps, act, fmt, True)
+        ctx.save_for_backward(None if fmt else xd, codes, scales, w, b, mean, rstd)
+        ctx.cfg = (G, act, fmt, tuple(x.shape), None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, codes, scales, w, b, mean, rstd = ctx.saved_tensors
+        G, act, fmt, shape, wt, bt = ctx.cfg
+        dev = gy.device
+        need_w, need_b = w is not None and ctx.needs_input_grad[1], b is not None and ctx.needs_input_grad[2]
+        with torch.cuda.device(dev):
+            gy, N, C, S = _maps(gy)
+            dx = A.empty_dense(shape, 1, gy.dtype, dev)
+            new = torch.empty if gy.numel() else torch.zeros
+            dw = new((C,), dtype=torch.float32, device=dev) if need_w else None
+            db = new((C,), dtype=torch.float32, device=dev) if need_b else None
+            if gy.numel():
+                nbytes = int(L.call("dbev_gn_act_workspace_bytes", N, S, C, G))
+                ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+                n = gy.numel()
+                L.call("dbev_gn_act_backward", L.ptr(gy), A.DTYPES[gy.dtype], L.ptr(x), A.FORMATS[fmt] if fmt else 0, L.ptr(codes), L.ptr(scales),
+                       N, S, C, G, L.ptr(w), L.ptr(b), L.ptr(mean), L.ptr(rstd), A.ACTS[act], L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), nbytes,
+                       L.stream_ptr(dev), alg_bytes=3 * n * gy.element_size() + 2 * (n if fmt else n * gy.element_size()))
+            dw = dw if dw is None or dw.dtype == wt else dw.to(wt)
+            db = db if db is None or db.dtype == bt else db.to(bt)
+        return dx if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", checkpoint=None):
+    """act(F.group_norm(x, num_groups, weight, bias, eps)) for a device tensor x [N, C, *], act one of act8.ACTS; the result is
+    channels-last.  `checkpoint` ("int8" / "e4m3"): under autograd the 8-bit checkpoint of x is kept instead of x, and the gradients are
+    those of the formula with x^ in place of x (mean and rstd stay x's own)."""
+    A._act(act)
+    if checkpoint is not None:
+        A._fmt(checkpoint)
+    dev = L.require_cuda(x, weight, bias)
+    A._dtype(x)
+    G = int(num_groups)
+    if x.dim() < 2:
+        raise ValueError(f"group_norm_act: [N, C, *] expected, got {tuple(x.shape)}")
+    N, C = x.shape[:2]
+    if G < 1 or C == 0 or C % G:
+        raise ValueError(f"group_norm_act: {C} channels in {num_groups} groups")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != (C,) or t.dtype not in A.DTYPES):
+            raise ValueError(f"group_norm_act: {name} {tuple(t.shape)} {t.dtype} for {C} channels")
+    if not eps >= 0:
+        raise ValueError(f"group_norm_act: eps {eps}")
+    if x.numel() and x.numel() // G == 1:                         # F.group_norm's own refusal
+        raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _GroupNormAct.apply(x, weight, bias, G, float(eps), act, checkpoint)
+    with torch.cuda.device(dev):
+        return _forward(_maps(x.detach())[0], G, _f32(weight), _f32(bias), eps, act, None, False)[0]
+
+
+def _ready(x, gn):
+    if not (torch.is_tensor(x) and x.is_cuda and x.numel()):
+        return False
+    why = None
+    if x.dtype not in A.DTYPES or (gn.weight is not None and gn.weight.dtype not in A.DTYPES):
+        why = f"dtype {x.dtype}"
+    elif torch.is_autocast_enabled("cuda"):
+        why = "autocast"
+    if why:
+        L.note_fallback("gn_act", why)
+    return why is None
+
+
+def gn_act(x, gn, act="none", checkpoint=None):
+    """act(gn(x)) with the module `gn`'s parameters: the kernels for device tensors they take, the stock operators otherwise"""
+    A._act(act)
+    if checkpoint is not None:
+        A._fmt(checkpoint)
+    if _ready(x, gn):
+        return group_norm_act(x, gn.num_groups, gn.weight, gn.bias, gn.eps, act, checkpoint)
+    return _STOCK[act](F.group_norm(x, gn.num_groups, gn.weight, gn.bias, gn.eps))
+
+
+class GroupNormAct(nn.GroupNorm):
+    """nn.GroupNorm that also applies the activation behind it (`act`, one of act8.ACTS) and may keep its input as an 8-bit checkpoint
+    (`act8_format`: None, "int8" or "e4m3"); parameters and state-dict keys are nn.GroupNorm's"""
+    act, act8_format = "none", None
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, act="none", checkpoint=None, **kwargs):
+        super().__init__(num_groups, num_channels, eps, affine, **kwargs)
+        A._act(act)
+        if checkpoint is not None:
+            A._fmt(checkpoint)
+        self.act, self.act8_format = act, checkpoint
+
+    def forward(self, x):
+        return gn_act(x, self, self.act, self.act8_format)
+
+    def extra_repr(self):
+        return super().extra_repr() + f", act={self.act}, act8={self.act8_format}"
+
+
+def fuse_gn_act_modules(model, checkpoint=None):
+    """Rewire the nn.GroupNorm modules of nn.Sequential stacks and ConvModules onto the kernels, together with the ReLU / SiLU / GELU right
+    behind them (replaced by nn.Identity; keys unchanged); other GroupNorm modules become GroupNormAct without an activation.
+    `checkpoint`: the format in which they keep their input, or None.  Returns how many norms changed.  Idempotent."""
+    from .registry import ConvModule
+    if checkpoint is not None:
+        A._fmt(checkpoint)
+    n = 0
+
+    def take(norm, act):
+        norm.__class__ = GroupNormAct
+        norm.act, norm.act8_format = act, checkpoint
+
+    for mod in list(model.modules()):
+        if isinstance(mod, nn.Sequential):
+            kids = list(mod._modules.items())
+            for (_, a), (kb, b) in zip(kids, kids[1:]):
+                if type(a) is nn.GroupNorm and A.act_name(b):
+                    take(a, A.act_name(b))
+                    mod._modules[kb] = nn.Identity()
+                    n += 1
+        elif isinstance(mod, ConvModule) and mod.with_norm and type(mod.norm) is nn.GroupNorm:
+            act = A.act_name(mod.activate) if mod.with_activation else None
+            take(mod.norm, act or "none")
+            if act:
+                mod.activate = nn.Identity()
+            n += 1
+    for mod in model.modules():
+        if type(mod) is nn.GroupNorm:
+            take(mod, "none")
+            n += 1
+        elif type(mod) is GroupNormAct:
+            mod.act8_format = checkpoint
+    return n

@@ -67,7 +67,7 @@ const char* dbev_kernel_name(int kernel_id);
  * ---------------------------------------------------------------------------------- */
 enum {
   DBEV_FB_BN_ACT = 0, DBEV_FB_SKINNY_CONV, DBEV_FB_ADAPT_MSE, DBEV_FB_PILLAR_VFE, DBEV_FB_HEAD_BATCH, DBEV_FB_DEPTH_HEAD,
-  DBEV_FB_SITES
+  DBEV_FB_GN_ACT, DBEV_FB_ACT8, DBEV_FB_SITES
 };
 int dbev_fallback_note(int site);
 long long dbev_fallback_count(int site);
@@ -937,6 +937,58 @@ int dbev_gemm1x1_forward(const float* x_nhwc, const float* weight, float* y_nhwc
 size_t dbev_gemm1x1_backward_weight_workspace_bytes(long long M, int Cin, int Cout, int x_row_stride);
 int dbev_gemm1x1_backward_weight(const float* x_nhwc, const float* grad_y_nhwc, float* grad_weight, long long M, int Cin, int Cout,
                                  int x_row_stride, void* workspace, size_t workspace_bytes, dbevStream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * 8-bit activation checkpoints (csrc/act8.hip, csrc/act8_wgrad.hip): an activation needed by the backward pass kept as one byte per
+ * value and one scale byte per 32 neighbouring channels.  The reference's counterpart is activation checkpointing by recomputation
+ * (`with_cp`, mmdet3d/models/bricks/res_block.py:11-230 through torch.utils.checkpoint).
+ *   x [rows, C], row r at x + r * row_stride elements, type `dtype`; codes u8[rows, C], scales u8[rows, ceil(C / 32)], both dense.
+ *   With a = max |x| of a block: DBEV_ACT8_INT8 k = floor(log2 a) - 6, code = clamp(rne(x / 2^k), -127, 127) in two's complement;
+ *   DBEV_ACT8_E4M3 k = floor(log2 a) - 8, one more if a > 448 * 2^k, code = the e4m3 float nearest to x / 2^k (ties to even); k >= -127,
+ *   scale byte k + 127.  A block with an infinity or a NaN has scale byte 255 and restores as NaN.
+ *   dbev_act8_pack                  x -> codes, scales
+ *   dbev_act8_unpack                out[rows, C] (dense, `dtype`) = the values the codes stand for, rounded to `dtype`
+ *   dbev_act8_activation_forward    y[rows, C] (dense) = act(x), and x's checkpoint in the same pass (fmt DBEV_ACT8_NONE: y only, codes and
+ *                                   scales unused)
+ *   dbev_act8_activation_backward   dx[rows, C] (dense) = gy * act'(x^), gy with gy_row_stride
+ * ---------------------------------------------------------------------------------- */
+enum { DBEV_DT_F32 = 0, DBEV_DT_BF16, DBEV_DT_F16 };
+enum { DBEV_ACT8_NONE = 0, DBEV_ACT8_INT8, DBEV_ACT8_E4M3 };
+enum { DBEV_ACT_NONE = 0, DBEV_ACT_RELU, DBEV_ACT_SILU, DBEV_ACT_GELU /* the erf form */ };
+int dbev_act8_pack(const void* x, int dtype, long long rows, int C, long long row_stride, int fmt, uint8_t* codes, uint8_t* scales,
+                   dbevStream_t stream);
+int dbev_act8_unpack(const uint8_t* codes, const uint8_t* scales, int fmt, long long rows, int C, void* out, int dtype, dbevStream_t stream);
+int dbev_act8_activation_forward(const void* x, int dtype, long long rows, int C, long long row_stride, int act, int fmt, void* y,
+                                 uint8_t* codes, uint8_t* scales, dbevStream_t stream);
+int dbev_act8_activation_backward(const void* gy, int dtype, long long gy_row_stride, const uint8_t* codes, const uint8_t* scales, int fmt,
+                                  long long rows, int C, int act, void* dx, dbevStream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Weight and bias gradient of a linear layer / channels-last 1x1 convolution whose saved input is an 8-bit checkpoint
+ * (csrc/act8_wgrad.hip): gw[Co, Ci] = gy^T x^, gb[Co] = column sums of gy (gb may be NULL); gy [M, Co] dense of type `dtype`, codes /
+ * scales as above for [M, Ci], gw and gb of type `dtype`.  fp32 accuracy for fp32 gy (exact bf16 pieces, fp32 sums, fixed order).
+ * M may be 0 (zeros).  Workspace: dbev_act8_weight_gradient_workspace_bytes (0: unsupported sizes).
+ * ---------------------------------------------------------------------------------- */
+size_t dbev_act8_weight_gradient_workspace_bytes(long long M, int Ci, int Co);
+int dbev_act8_weight_gradient(const void* gy, int dtype, const uint8_t* codes, const uint8_t* scales, int fmt, long long M, int Ci, int Co,
+                              void* gw, void* gb, void* workspace, size_t workspace_bytes, dbevStream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Group norm + activation, channels-last (csrc/gn_act.hip).  Replaces nn.GroupNorm -> activation of norm_cfg=dict(type='GN') layers
+ * (mmcv ConvModule as built by mmdet3d/models/necks/fpn.py:77-95, lss_fpn.py:30-60).
+ *   x [N, S, C] dense (S pixels, channels last), G groups of C / G channels; y = act((x - mean) * rstd * gamma + beta) with the biased
+ *   variance, rstd = 1 / sqrt(var + eps); gamma / beta f32[C] or NULL (1 / 0).
+ *   forward: mean, rstd f32[N, G] (both NULL at inference); fmt / codes / scales as above: x's checkpoint, written by the same pass.
+ *   backward: x is read from codes / scales when fmt != DBEV_ACT8_NONE (then x may be NULL); dgamma, dbeta f32[C] (either may be NULL).
+ *   Fixed summation order.  Workspace: dbev_gn_act_workspace_bytes (0: unsupported sizes).
+ * ---------------------------------------------------------------------------------- */
+size_t dbev_gn_act_workspace_bytes(int N, long long S, int C, int G);
+int dbev_gn_act_forward(const void* x, int dtype, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps,
+                        int act, void* y, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales, void* workspace,
+                        size_t workspace_bytes, dbevStream_t stream);
+int dbev_gn_act_backward(const void* gy, int dtype, const void* x, int fmt, const uint8_t* codes, const uint8_t* scales, int N, long long S,
+                         int C, int G, const float* gamma, const float* beta, const float* mean, const float* rstd, int act, void* dx,
+                         float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, dbevStream_t stream);
 
 #ifdef __cplusplus
 }

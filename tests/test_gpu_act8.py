@@ -1,0 +1,423 @@
+"""8-bit activation checkpoints on the GPU (csrc/act8.hip, csrc/act8_wgrad.hip, distill_bev_amd/act8.py) against oracle/act8.py (64 bits).
+
+Codes, scale bytes and restored values are compared for equality: scales are powers of two, the code is the only rounding.  Tolerances of
+computed values, u = 2^-24 (half a step of fp32), and half a step of the output type on top (`_half`):
+  silu      exp2's argument is rounded (|z| u), exp2, 1 +, reciprocal and product a few u each: |dy| <= (1.5 |z| + 8) u |y|
+  silu'     f = s (1 + z (1 - s)); a relative error e = (1.5 |z| + 8) u of s moves f by s e (1 + |z|)
+  gelu      Q = 1 - Phi(|z|) to (z^2 + 16) u relative (fit 3.2e-8, fp32 Horner 5 u, argument z^2 / 2 rounded twice); Phi = 1 - Q or Q
+  gelu'     f = Phi + z phi, phi to (z^2 + 6) u
+  (sigmoid, Q and phi below 2^-126 are flushed to zero by the hardware's exp2 and reciprocal: |z| 2^-126 of the result, (1 + |z|) 2^-126 of
+  the derivative)
+  weight gradient   products exact, fp32 sums of n terms in chains and a tree: independent roundings grow like sqrt(n):
+                    |dg| <= (8 + 4 sqrt(3 M)) u sum |gy| |x^|"""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from oracle import act8 as O
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _half(ref, dtype):
+    """half a step of `dtype` at |ref| (and below its normal range)"""
+    f = torch.finfo(dtype)
+    return (f.eps / 2) * ref.abs().clamp(min=f.tiny)
+
+
+def _data(rows, C, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, C, generator=g) * torch.exp(1.5 * torch.randn(rows, 1, generator=g))
+    return x.to(dtype)
+
+
+def _within(got, ref, lim, what=""):
+    """|got - ref| <= lim everywhere; says where not"""
+    d = (got.detach().cpu().double() - ref).abs()
+    bad = ~(d <= lim)
+    if bool(bad.any()):
+        i = int((d / lim).nan_to_num(posinf=1e30, nan=1e30).argmax())
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()}, worst at {i}: {float(got.reshape(-1)[i])} against {float(ref.reshape(-1)[i])}, "
+                             f"off by {float(d.reshape(-1)[i]):.3e}, limit {float(lim.reshape(-1)[i]):.3e}")
+
+
+SHAPES = [(1, 1), (1, 32), (3, 31), (5, 33), (7, 64), (4, 200), (129, 80), (64, 256), (50, 59), (9, 1030), (2, 4097), (600, 10)]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,C", SHAPES)
+def test_pack_and_unpack_equal_the_definition(rows, C, dtype, fmt):
+    from distill_bev_amd import act8 as A
+    x = _data(rows, C, dtype, rows * 7 + C)
+    ck = A.pack(x.to(DEV), fmt, -1)
+    codes, scales = O.quantise(x, fmt)
+    assert torch.equal(ck.scales.cpu(), scales) and torch.equal(ck.codes.cpu(), codes)
+    ref = O.values(codes, scales, fmt)
+    out = A.unpack(ck)
+    assert out.dtype == dtype and out.shape == x.shape and torch.equal(out.cpu(), ref.to(dtype))
+    assert torch.equal(A.unpack(ck, torch.float32).cpu().double(), ref)
+    for other in DTYPES:
+        assert torch.equal(A.unpack(ck, other).cpu(), ref.float().to(other))
+    assert ck.nbytes == rows * C + rows * -(-C // 32)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_special_values(fmt):
+    from distill_bev_amd import act8 as A
+    fmax = torch.finfo(torch.float32).max
+    x = torch.zeros(16, 64)
+    x[1] = -0.0
+    x[2, :32] = torch.linspace(-127.5, 127.5, 32)                      # ties and the clamp
+    x[2, 32:] = torch.arange(32) + 0.5
+    x[3, 5] = float("inf")
+    x[4, 40] = float("-inf")
+    x[5, 63] = float("nan")
+    x[6] = fmax * torch.linspace(-1, 1, 64)
+    x[7] = 1e-45 * torch.arange(64)                                     # subnormals
+    x[8] = 2.0 ** -126 * torch.linspace(-1, 1, 64)
+    x[9] = 1.75 * torch.linspace(-1, 1, 64)                             # 448 / 256: the largest that does not move the exponent
+    x[10] = torch.nextafter(torch.tensor(1.75), torch.tensor(2.0)) * torch.linspace(-1, 1, 64)
+    x[11] = 2.0 ** torch.arange(-32, 32)
+    x[12, 0], x[12, 1:] = 1e4, 1e-3
+    x[13] = 2.0 ** -120 * torch.linspace(-1, 1, 64)
+    x[14] = (1 + 2.0 ** -4) * 2.0 ** torch.arange(-40, 24)              # ties of e4m3
+    x[15] = torch.randn(64, generator=torch.Generator().manual_seed(1))
+    ck = A.pack(x.to(DEV), fmt)
+    codes, scales = O.quantise(x, fmt)
+    assert torch.equal(ck.scales.cpu(), scales) and torch.equal(ck.codes.cpu().int() * (scales.repeat_interleave(32, 1) != 255),
+                                                                codes.int() * (scales.repeat_interleave(32, 1) != 255))
+    # (the value is rounded to fp32: the e4m3 neighbour of fp32's largest number is 2^128, an infinity there)
+    out, ref = A.unpack(ck).cpu().double(), O.values(codes, scales, fmt).float().double()
+    assert torch.equal(torch.isnan(out), torch.isnan(ref)) and torch.equal(out.nan_to_num(), ref.nan_to_num())
+    assert bool(torch.isnan(out[3, :32]).all()) and bool((out[3, 32:] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layouts_strides_and_alignment(dtype, fmt):
+    from distill_bev_amd import act8 as A
+    big = _data(60, 300, dtype, 3).to(DEV)
+    views = {"columns": big[:, 3:131], "even columns": big[:, 2:98], "odd width": big[:, 1:60], "every second row": big[::2, :64],
+             "transposed": big.t(), "expanded": big[:1].expand(7, 300), "three dimensions": big.view(6, 10, 300)[:, 1:9, 16:80],
+             "one row": big[5:6, 7:77], "offset storage": big.view(-1)[5:5 + 64 * 9].view(9, 64)}
+    for name, v in views.items():
+        ck = A.pack(v, fmt, -1)
+        ref = O.restored(v.reshape(-1, v.shape[-1]), fmt).view(v.shape)
+        assert torch.equal(A.unpack(ck, torch.float32).cpu().double(), ref), name
+    m = _data(2 * 5 * 7, 40, dtype, 4).to(DEV).view(2, 5, 7, 40).permute(0, 3, 1, 2)         # channels-last map
+    ck = A.pack(m, fmt)
+    out = A.unpack(ck)
+    assert ck.dim == 1 and out.shape == m.shape and out.is_contiguous(memory_format=torch.channels_last)
+    assert torch.equal(out.cpu().double(), O.restored(m.permute(0, 2, 3, 1).reshape(-1, 40), fmt).to(dtype).double().view(2, 5, 7, 40).permute(0, 3, 1, 2))
+    assert A.pack(m.contiguous(), fmt).dim == 3
+    for shape in ((0, 32), (4, 0), (2, 0, 5)):
+        e = A.unpack(A.pack(torch.empty(shape, dtype=dtype, device=DEV), fmt, -1))
+        assert e.shape == shape
+
+
+def _act_bounds(z, act):
+    a = z.abs()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        e = (1.5 * a + 8) * U
+        return e * (z * s).abs(), s * e * (1 + a)
+    if act == "gelu":
+        q = 0.5 * torch.special.erfc(a / math.sqrt(2))
+        phi = torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+        dq = q * (z * z + 16) * U + (z > 0) * 2 * U
+        return a * dq + 2 * U * O.act(z, act)[0].abs(), dq + a * phi * (z * z + 6) * U + 2 * U
+    return torch.zeros_like(z), torch.zeros_like(z)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,C", [(1, 1), (5, 33), (40, 64), (17, 200), (300, 59)])
+def test_activation_forward_and_backward(rows, C, dtype, act, fmt):
+    from distill_bev_amd import act8 as A
+    x = _data(rows, C, dtype, C)
+    gy = _data(rows, C, dtype, C + 1)
+    leaf = x.to(DEV).requires_grad_(True)
+    y = A.activation(leaf, act, fmt, -1)
+    dx, = torch.autograd.grad(y, (leaf,), gy.to(DEV))
+    assert y.dtype == dtype and dx.dtype == dtype and y.shape == x.shape
+    z = x.double()
+    zr = O.restored(x, fmt)
+    ref, dref = O.act(z, act)[0], gy.double() * O.act(zr, act)[1]
+    by, bd = _act_bounds(z, act)[0], gy.double().abs() * (_act_bounds(zr, act)[1] + 2 * U * O.act(zr, act)[1].abs())
+    flush, gflush = z.abs() * 2.0 ** -126, gy.double().abs() * (1 + zr.abs()) * 2.0 ** -126
+    _within(y, ref, 3 * by + flush + _half(ref, dtype), f"{act} forward")
+    _within(dx, dref, 3 * bd + gflush + _half(dref, dtype), f"{act} backward")
+    with torch.no_grad():
+        assert torch.equal(A.activation(leaf, act, fmt, -1), y)          # without a gradient: the same values
+
+
+def test_activation_tails_and_non_finite_values():
+    from distill_bev_amd import act8 as A
+    x = torch.cat([torch.linspace(-40, 40, 4001), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 3e38, -3e38, float("inf"), float("nan")])]).view(1, -1)
+    for act in ("silu", "gelu", "relu"):
+        y = A.activation(x.to(DEV), act)
+        ref = O.act(x.double(), act)[0]
+        fin = torch.isfinite(ref)
+        _within(y.cpu()[fin], ref[fin], (_act_bounds(x.double(), act)[0] * 3 + x.double().abs() * 2.0 ** -126 + _half(ref, torch.float32))[fin], act)
+        # at +infinity the formulas' own limit (the library's CPU gelu gives a NaN there, so it is no reference)
+        assert torch.equal(torch.isnan(y.cpu()), torch.isnan(ref)) and torch.equal(torch.isinf(y.cpu()), torch.isinf(ref.float()))
+
+
+def test_activation_layouts_and_gradient_forms():
+    from distill_bev_amd import act8 as A
+    base = _data(2 * 6 * 5, 70, torch.float32, 5).to(DEV)
+    m = base[:, :40].reshape(2, 6, 5, 40).permute(0, 3, 1, 2).requires_grad_(True)     # channels-last map
+    y = A.activation(m, "silu", "int8")
+    assert y.is_contiguous(memory_format=torch.channels_last)
+    g, = torch.autograd.grad(y.sum(), (m,))                              # an expanded gradient
+    zr = O.restored(m.detach().permute(0, 2, 3, 1).reshape(-1, 40), "int8")
+    assert torch.allclose(g.cpu().permute(0, 2, 3, 1).reshape(-1, 40).double(), O.act(zr, "silu")[1], atol=2e-6, rtol=0)
+    leaf = base.clone().requires_grad_(True)
+    y = A.activation(leaf[:, 3:50], "gelu", "e4m3")                      # a strided input inside a graph
+    g, = torch.autograd.grad(y, (leaf,), base[:, 10:57])                 # a strided gradient
+    zr = O.restored(base[:, 3:50], "e4m3")
+    ref = torch.zeros(60, 70, dtype=torch.float64)
+    ref[:, 3:50] = base[:, 10:57].cpu().double() * O.act(zr, "gelu")[1]
+    assert torch.allclose(g.cpu().double(), ref, atol=1e-5, rtol=1e-6)
+    e = torch.empty((0, 32), device=DEV, requires_grad=True)
+    A.activation(e, "gelu").sum().backward()
+    assert e.grad.shape == (0, 32)
+    leaf = base.clone().requires_grad_(True)
+    y = A.activation(leaf, "gelu", "int8")
+    with torch.no_grad():
+        leaf.mul_(2.0)                                                   # the checkpoint is kept, not the tensor: nothing to detect
+    y.sum().backward()
+    assert torch.allclose(leaf.grad.cpu().double(), O.act(O.restored(base, "int8"), "gelu")[1], atol=2e-6, rtol=0)
+
+
+WG = [(1, 1, 1), (1, 64, 64), (5, 3, 5), (31, 64, 63), (32, 65, 64), (33, 129, 127), (127, 128, 128), (129, 256, 10), (1000, 300, 200), (700, 512, 130),
+      (4100, 96, 256), (2050, 257, 66), (900, 10, 256)]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,Ci,Co", WG)
+def test_weight_gradient(M, Ci, Co, dtype, fmt):
+    from distill_bev_amd import act8 as A
+    x, gy = _data(M, Ci, dtype, M + Ci), _data(M, Co, dtype, M + Co + 1)
+    ck = A.pack(x.to(DEV), fmt, -1)
+    gw, gb = A.weight_gradient(ck, gy.to(DEV), bias=True)
+    xr, g = O.restored(x, fmt), gy.double()
+    ref, refb = g.t() @ xr, g.sum(0)
+    c = (8 + 4 * math.sqrt(3 * M)) * U
+    bw, bb = c * (g.abs().t() @ xr.abs()), c * g.abs().sum(0)
+    assert gw.dtype == dtype and gw.shape == (Co, Ci) and gb.shape == (Co,)
+    _within(gw, ref, bw * (1 + c) + _half(ref, dtype) * (1 + c), "weight gradient")
+    _within(gb, refb, bb * (1 + c) + _half(refb, dtype), "bias gradient")
+    assert torch.equal(A.weight_gradient(ck, gy.to(DEV)), gw)            # fixed order, with and without the bias
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,Ci,Co", [(64, 96, 33), (517, 130, 65), (2000, 64, 200)])
+def test_weight_gradient_of_whole_numbers_is_exact(M, Ci, Co, dtype):
+    """whole numbers up to 127 are their own checkpoint when a block holds a 64..127; sums below 2^24 (2^8 for bf16, 2^11 for fp16 outputs
+    are rounded once): every index and every share has to be right"""
+    from distill_bev_amd import act8 as A
+    g = torch.Generator().manual_seed(M)
+    x = torch.randint(-9, 10, (M, Ci), generator=g).float()
+    x[:, ::32] = 100
+    gy = torch.randint(-8, 9, (M, Co), generator=g).float()
+    gw, gb = A.weight_gradient(A.pack(x.to(DEV, dtype), "int8", -1), gy.to(DEV, dtype), bias=True)
+    assert torch.equal(gw.cpu(), (gy.double().t() @ x.double()).to(dtype)) and torch.equal(gb.cpu(), gy.double().sum(0).to(dtype))
+
+
+def test_weight_gradient_keeps_every_bit_of_an_fp32_gradient():
+    from distill_bev_amd import act8 as A
+    M, C = 128, 64
+    x = torch.zeros(M, C)
+    x[torch.arange(C) * 2, torch.arange(C)] = 1.0                         # one row per channel
+    gy = _data(M, 40, torch.float32, 9)
+    gw = A.weight_gradient(A.pack(x.to(DEV), "int8", -1), gy.to(DEV))
+    assert torch.equal(gw.cpu(), gy[::2].t())
+    gy16 = gy.half()
+    assert torch.equal(A.weight_gradient(A.pack(x.to(DEV).half(), "e4m3", -1), gy16.to(DEV)).cpu(), gy16[::2].t())
+
+
+def test_weight_gradient_non_finite_empty_and_layouts():
+    from distill_bev_amd import act8 as A
+    M, Ci, Co = 200, 70, 40
+    x, gy = _data(M, Ci, torch.float32, 1).abs() + 0.5, _data(M, Co, torch.float32, 2)
+    x[7, 40] = float("nan")                                               # channels 32..63 of the checkpoint's row 7
+    gy[11, 3], gy[12, 5], gy[13, 6], gy[14, 8] = float("inf"), float("-inf"), float("nan"), 3.4e38
+    gw, gb = A.weight_gradient(A.pack(x.to(DEV), "int8", -1), gy.to(DEV), bias=True)
+    gw, gb = gw.cpu(), gb.cpu()
+    assert bool(torch.isnan(gw[:, 32:64]).all())
+    rest = [c for c in range(Ci) if not 32 <= c < 64]
+    assert bool((gw[3][rest] == float("inf")).all()) and bool((gw[5][rest] == float("-inf")).all()) and bool(torch.isnan(gw[6][rest]).all())
+    ok = [r for r in range(Co) if r not in (3, 5, 6, 8)]
+    assert bool(torch.isfinite(gw[ok][:, rest]).all())
+    assert gb[3] == float("inf") and gb[5] == float("-inf") and bool(torch.isnan(gb[6])) and bool(torch.isfinite(gb[8]))
+    gw, gb = A.weight_gradient(A.pack(torch.empty((0, 48), device=DEV), "int8", -1), torch.empty((0, 20), device=DEV), bias=True)
+    assert torch.equal(gw, torch.zeros_like(gw)) and torch.equal(gb, torch.zeros_like(gb))
+    x, gy = _data(60, 48, torch.float32, 3).to(DEV), _data(60, 90, torch.float32, 4).to(DEV)
+    a = A.weight_gradient(A.pack(x, "int8", -1), gy[:, 11:50])            # a strided gradient
+    assert torch.equal(a, A.weight_gradient(A.pack(x, "int8", -1), gy[:, 11:50].contiguous()))
+    m = x.view(3, 4, 5, 48).permute(0, 3, 1, 2)
+    gm = gy[:, 11:50].reshape(3, 4, 5, 39).permute(0, 3, 1, 2)
+    assert torch.equal(A.weight_gradient(A.pack(m, "int8", 1), gm), a)    # the same rows as a map
+    with pytest.raises(ValueError):
+        A.weight_gradient(A.pack(x, "int8", -1), gy[:59])
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("shape,Co", [((7, 33), 20), ((3, 50, 64), 128), ((4096, 64), 128), ((60000, 128), 128)])
+def test_linear_layer(shape, Co, fmt):
+    """forward and data gradient are the layer's ordinary products; weight and bias gradient those of the checkpoint.  (The last size takes
+    the bf16x6 products.)"""
+    from distill_bev_amd import act8 as A
+    torch.manual_seed(0)
+    x = torch.randn(*shape)
+    mod = nn.Linear(shape[-1], Co)
+    xl = x.to(DEV).requires_grad_(True)
+    w, b = mod.weight.detach().to(DEV).requires_grad_(True), mod.bias.detach().to(DEV).requires_grad_(True)
+    gy = torch.randn(*shape[:-1], Co)
+    y = A.linear(xl, w, b, fmt)
+    gx, gw, gb = torch.autograd.grad(y, (xl, w, b), gy.to(DEV))
+    x2, g2 = x.reshape(-1, shape[-1]).double(), gy.reshape(-1, Co).double()
+    wd = mod.weight.detach().double()
+    rel = lambda a, r: float((a.detach().cpu().double() - r).norm() / r.norm())    # noqa: E731
+    assert rel(y.reshape(-1, Co), x2 @ wd.t() + mod.bias.detach().double()) < 2e-6
+    assert rel(gx.reshape(-1, shape[-1]), g2 @ wd) < 2e-6
+    assert rel(gw, g2.t() @ O.restored(x2, fmt)) < 2e-6 and rel(gb, g2.sum(0)) < 2e-6
+    frozen = A.linear(xl, w.detach(), b, fmt)                             # only the bias and the input want gradients
+    gx2, gb2 = torch.autograd.grad(frozen, (xl, b), gy.to(DEV))
+    assert torch.equal(frozen, y) and torch.equal(gx2, gx) and rel(gb2, g2.sum(0)) < 2e-6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_conv1x1_layer(dtype):
+    from distill_bev_amd import act8 as A
+    torch.manual_seed(1)
+    x = torch.randn(3, 40, 9, 7).to(dtype)
+    w, b = (torch.randn(24, 40, 1, 1) * 0.2).to(dtype), torch.randn(24).to(dtype)
+    gy = torch.randn(3, 24, 9, 7).to(dtype)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    y = A.conv1x1(*leaves, "int8")
+    gx, gw, gb = torch.autograd.grad(y, leaves, gy.to(DEV))
+    rows = lambda t: t.double().permute(0, 2, 3, 1).reshape(-1, t.shape[1])     # noqa: E731
+    tol = 3 * torch.finfo(dtype).eps + 2e-6
+    rel = lambda a, r: float((a.detach().cpu().double() - r).norm() / r.norm())    # noqa: E731
+    assert y.is_contiguous(memory_format=torch.channels_last)
+    assert rel(rows(y.detach().cpu()), rows(x) @ w.double().view(24, 40).t() + b.double()) < tol
+    assert rel(rows(gx.cpu()), rows(gy) @ w.double().view(24, 40)) < tol and gx.shape == x.shape
+    assert gw.shape == w.shape and rel(gw.view(24, 40), rows(gy).t() @ O.restored(rows(x).to(dtype), "int8")) < tol
+    assert rel(gb, rows(gy).sum(0)) < tol
+    with pytest.raises(ValueError):
+        A.conv1x1(leaves[0], torch.randn(4, 40, 3, 3, device=DEV, dtype=dtype))
+    from distill_bev_amd import _lib as L
+    with pytest.raises(L.DbevHipError):
+        A.conv1x1(leaves[0], leaves[1].double())
+
+
+def test_feed_forward_block_as_a_model_uses_it():
+    """use_act8 on a Linear -> GELU -> Linear block with a skip connection: forward equals the stock modules', gradients equal the oracle's
+    (which takes the same checkpoints), memory kept between forward and backward falls"""
+    from distill_bev_amd import act8 as A
+
+    class Block(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.net = nn.Sequential(nn.Linear(64, 192), nn.GELU(), nn.Linear(192, 64))
+
+        def forward(self, x):
+            return x + self.net(x)
+
+    torch.manual_seed(3)
+    stock, mod = Block(), Block()
+    mod.load_state_dict(stock.state_dict())
+    stock, mod = stock.to(DEV), mod.to(DEV)
+    assert A.use_act8(mod, "int8") == 3 and list(mod.state_dict()) == list(stock.state_dict())
+    x = torch.randn(2, 500, 64)
+    xa, gy = x.to(DEV).requires_grad_(True), torch.randn(2, 500, 64)
+    y = mod(xa)
+    assert torch.allclose(y, stock(x.to(DEV)), atol=2e-5)
+    y.backward(gy.to(DEV))
+    xd = x.double().reshape(-1, 64).requires_grad_(True)
+    p = [t.detach().cpu().double().requires_grad_(True) for t in stock.parameters()]
+    h = O.LinearFn.apply(xd, p[0], p[1], "int8")
+    out = xd + O.LinearFn.apply(O.ActFn.apply(h, "gelu", "int8"), p[2], p[3], "int8")
+    out.backward(gy.double().reshape(-1, 64))
+    # A hidden value within its fp32 error e of a code border may take the neighbouring code: a share 2 e / step of the values, each off by
+    # one step, moves a gradient by sqrt(2 e / step) * step = sqrt(2 e step) of its norm.  In units of the spread e <= 1e-6 (64 to 192
+    # products and the activation) and step <= 1 / 32 (a largest value of 2 to 4 spreads / 64): 2.5e-4.
+    rel = lambda a, r: float((a.detach().cpu().double().reshape(r.shape) - r).norm() / r.norm())      # noqa: E731
+    assert rel(xa.grad, xd.grad) < 2.5e-4
+    for q, r in zip(mod.parameters(), p):
+        assert rel(q.grad, r.grad) < 2.5e-4
+
+    def kept(m):
+        held = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: held.append((t.untyped_storage().data_ptr(), t.untyped_storage().nbytes())) or t, lambda t: t):
+            m(x.to(DEV).requires_grad_(True))
+        own = {q.untyped_storage().data_ptr() for q in m.parameters()}
+        return sum({a: b for a, b in held if a not in own}.values())
+
+    assert kept(mod) < 0.3 * kept(stock)
+    mod.eval()
+    with torch.no_grad():
+        assert torch.allclose(mod(x.to(DEV)), stock(x.to(DEV)), atol=2e-5)
+
+
+def test_ineligible_device_tensors_take_the_stock_modules_and_are_counted():
+    from distill_bev_amd import _lib as L
+    from distill_bev_amd import act8 as A
+    import warnings
+    m = nn.Sequential(nn.Linear(8, 4), nn.SiLU()).to(DEV).double()
+    A.use_act8(m)
+    L.fallback_reset()
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        m(torch.randn(3, 8, device=DEV, dtype=torch.float64)).sum().backward()
+    assert L.fallback_counts()["act8"] == 2
+    L.fallback_reset()
+
+
+def test_other_streams_and_graph_replays():
+    """on a stream of its own, and captured: forward, backward and weight gradient replayed on new inputs with eager work between"""
+    from distill_bev_amd import act8 as A
+    torch.manual_seed(4)
+    xs = [torch.randn(300, 96, device=DEV) for _ in range(4)]
+    gs = [torch.randn(300, 96, device=DEV) for _ in range(4)]
+
+    def step(x, g):
+        leaf = x.detach().requires_grad_(True)
+        y = A.activation(leaf, "gelu", "int8")
+        dx, = torch.autograd.grad(y, (leaf,), g)
+        gw, gb = A.weight_gradient(A.pack(x, "e4m3", -1), g, bias=True)
+        return y.detach(), dx, gw, gb
+
+    eager = [step(x, g) for x, g in zip(xs, gs)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = step(xs[1], gs[1])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(out, eager[1]))
+    sx, sg = xs[0].clone(), gs[0].clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(sx, sg)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(sx, sg)
+    for i in (1, 2, 3, 0, 2):
+        sx.copy_(xs[i])
+        sg.copy_(gs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager[i]))
+        again = step(xs[3 - i], gs[3 - i])
+        assert all(torch.equal(a, b) for a, b in zip(again, eager[3 - i]))

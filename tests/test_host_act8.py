@@ -1,0 +1,159 @@
+"""CPU: 8-bit checkpoints and the group norm's host side -- the oracle against itself and against differences, argument checks, refusals of
+the C entry points, module rewiring, and the stock path of CPU tensors."""
+import ctypes
+
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from oracle import act8 as O
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_quantiser_error_bounds_and_both_statements_of_it_agree(fmt):
+    torch.manual_seed(0)
+    x = torch.randn(40, 70).double() * torch.exp(3 * torch.randn(40, 1).double())
+    x[3] = 0
+    x[4, 5] = float("inf")
+    x[5, 40] = float("nan")
+    x[6] *= 1e-42                                                       # below the smallest scale
+    v = O.values(*O.quantise(x, fmt), fmt)
+    w = O.restored(x, fmt)
+    assert torch.equal(v.nan_to_num(nan=-7.0), w.nan_to_num(nan=-7.0))
+    assert bool(torch.isnan(v[4, :32]).all()) and not bool(torch.isnan(v[4, 32:]).any()) and bool(torch.isnan(v[5, 32:64]).all())
+    ok = torch.isfinite(v)
+    a = F.pad(x, (0, 26)).view(40, 3, 32).abs().amax(2).repeat_interleave(32, 1)[:, :70]
+    err = (v - x).abs()
+    if fmt == "int8":
+        bound = a / 64
+    else:
+        bound = torch.maximum(x.abs() / 16, a / 2 ** 14)
+    assert bool((err <= bound.clamp(min=2.0 ** -127))[ok].all())
+    assert torch.equal(O.restored(v.nan_to_num(), fmt), v.nan_to_num())  # a fixed point
+
+
+def test_values_are_bf16_numbers():
+    x = torch.randn(64, 96) * torch.exp(4 * torch.randn(64, 1))
+    for fmt in ("int8", "e4m3"):
+        v = O.restored(x, fmt)
+        assert torch.equal(v, v.to(torch.bfloat16).double())
+
+
+@pytest.mark.parametrize("name", ["none", "relu", "silu", "gelu"])
+def test_oracle_gradients_against_differences(name):
+    torch.manual_seed(1)
+    N, S, C, G, h = 2, 5, 12, 3, 1e-6
+    x, w, b = torch.randn(N, S, C).double(), torch.randn(C).double(), torch.randn(C).double()
+    gy = torch.randn(N, S, C).double()
+    _, dx, dg, db, _ = O.group_norm(x, G, w, b, 1e-5, name, None, gy)
+    loss = lambda x, w, b: float((O.group_norm(x, G, w, b, 1e-5, name) * gy).sum())     # noqa: E731
+    for t, grad, at in ((x, dx, 0), (w, dg, 1), (b, db, 2)):
+        d = torch.randn_like(t)
+        args = [x, w, b]
+        args[at] = t + h * d
+        up = loss(*args)
+        args[at] = t - h * d
+        assert abs((up - loss(*args)) / (2 * h) - float((grad * d).sum())) < 1e-6 * (1 + float((grad * d).abs().sum()))
+    y, g = O.act(x, name)
+    assert torch.allclose((O.act(x + h, name)[0] - O.act(x - h, name)[0]) / (2 * h), g, atol=1e-8, rtol=0)
+
+
+def test_argument_checks_and_no_cpu_fallback_of_the_functions():
+    from distill_bev_amd import _lib as L
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    x = torch.randn(4, 32)
+    for bad in ("int4", None, 8):
+        with pytest.raises(ValueError):
+            A.pack(x, bad)
+    with pytest.raises(ValueError):
+        A.activation(x, "tanh")
+    with pytest.raises(ValueError):
+        A.activation(x, "gelu", None)
+    with pytest.raises(L.DbevHipError):
+        A.pack(x.double())
+    for call in (lambda: A.pack(x), lambda: A.activation(x), lambda: A.linear(x, torch.randn(8, 32)),
+                 lambda: A.conv1x1(torch.randn(1, 8, 2, 2), torch.randn(4, 8, 1, 1)), lambda: GN.group_norm_act(x, 4)):
+        with pytest.raises(L.DbevHipError):
+            call()
+    with pytest.raises(ValueError):
+        GN.gn_act(x, nn.GroupNorm(4, 32), "tanh")
+    with pytest.raises(ValueError):
+        GN.GroupNormAct(4, 32, checkpoint="int7")
+
+
+def test_rows_of_takes_views_where_it_can_and_dense_dim_follows_memory():
+    from distill_bev_amd import act8 as A
+    big = torch.randn(6, 5, 40)
+    v, rows, C, stride = A.rows_of(big[..., 3:19], 2)
+    assert (rows, C, stride) == (30, 16, 40) and v.data_ptr() == big[..., 3:].data_ptr()
+    v, rows, C, stride = A.rows_of(big[:, ::2], 2)                       # unevenly spaced rows: a copy
+    assert (rows, C, stride) == (18, 40, 40) and v.is_contiguous()
+    v, rows, C, stride = A.rows_of(torch.randn(1, 8).expand(4, 8), 1)    # rows on top of each other: a copy
+    assert stride == 8 and v.is_contiguous()
+    v, rows, C, stride = A.rows_of(torch.randn(8, 6).t(), 1)
+    assert (rows, C, stride) == (6, 8, 8)
+    assert A.rows_of(torch.randn(0, 8), 1)[1] == 0 and A.rows_of(torch.randn(3, 0), 1)[1:3] == (0, 0)
+    m = torch.randn(2, 6, 3, 5).contiguous(memory_format=torch.channels_last)
+    assert A.dense_dim(m) == 1 and A.dense_dim(m.contiguous()) == 3 and A.dense_dim(torch.randn(2, 7, 1, 1)) == 1
+    v, rows, C, stride = A.rows_of(m, 1)
+    assert (rows, C, stride) == (30, 6, 6) and v.data_ptr() == m.data_ptr()
+    e = A.empty_dense((2, 6, 3, 5), 1, torch.float32, "cpu")
+    assert e.is_contiguous(memory_format=torch.channels_last) and e.shape == (2, 6, 3, 5)
+    e = A.empty_dense((2, 6, 3), 1, torch.float32, "cpu")
+    assert e.movedim(1, -1).is_contiguous()
+
+
+def test_c_entry_points_refuse_without_touching_the_device():
+    from distill_bev_amd import _lib as L
+    h = L.lib()
+    one = ctypes.c_void_p(16)                                            # never dereferenced: every call below is refused on the host
+    bad = 10001
+    assert h.dbev_act8_pack(one, 3, 4, 32, 32, 1, one, one, None) == bad         # type
+    assert h.dbev_act8_pack(one, 0, 4, 32, 32, 0, one, one, None) == bad         # format
+    assert h.dbev_act8_pack(one, 0, 4, 32, 31, 1, one, one, None) == bad         # rows on top of each other
+    assert h.dbev_act8_pack(one, 0, -1, 32, 32, 1, one, one, None) == bad
+    assert h.dbev_act8_pack(one, 0, 4, 0, 32, 1, one, one, None) == bad
+    assert h.dbev_act8_pack(one, 0, 1 << 36, 32, 32, 1, one, one, None) == bad   # too large
+    assert h.dbev_act8_pack(one, 0, 4, 32, 32, 1, ctypes.c_void_p(17), one, None) == bad   # misaligned codes
+    assert h.dbev_act8_pack(one, 0, 0, 32, 32, 1, one, one, None) == 0           # nothing to do
+    assert h.dbev_act8_unpack(one, one, 0, 4, 32, one, 0, None) == bad
+    assert h.dbev_act8_activation_forward(one, 0, 4, 32, 32, 4, 1, one, one, one, None) == bad
+    assert h.dbev_act8_activation_backward(one, 0, 32, one, one, 0, 4, 32, 1, one, None) == bad
+    assert h.dbev_act8_weight_gradient_workspace_bytes(-1, 8, 8) == 0 and h.dbev_act8_weight_gradient_workspace_bytes(10, 0, 8) == 0
+    assert h.dbev_act8_weight_gradient_workspace_bytes(1 << 40, 8, 8) == 0
+    n = h.dbev_act8_weight_gradient_workspace_bytes(100, 64, 64)
+    assert n > 0 and h.dbev_act8_weight_gradient(one, 0, one, one, 1, 100, 64, 64, one, None, one, n // 2, None) == bad
+    assert h.dbev_act8_weight_gradient(one, 0, one, one, 0, 100, 64, 64, one, None, one, n, None) == bad
+    assert h.dbev_gn_act_workspace_bytes(2, 10, 12, 5) == 0              # groups do not divide
+    n = h.dbev_gn_act_workspace_bytes(2, 10, 12, 4)
+    f = ctypes.c_float(1e-5)
+    assert n > 0 and h.dbev_gn_act_forward(one, 0, 2, 10, 12, 4, None, None, f, 0, one, one, one, 0, None, None, one, n - 1, None) == bad
+    assert h.dbev_gn_act_forward(one, 0, 2, 10, 12, 4, None, None, f, 9, one, one, one, 0, None, None, one, n, None) == bad
+    assert h.dbev_gn_act_backward(one, 0, None, 0, None, None, 2, 10, 12, 4, None, None, one, one, 0, one, one, one, one, n, None) == bad   # no x
+    assert h.dbev_gn_act_forward(one, 0, 0, 10, 12, 4, None, None, f, 0, one, one, one, 0, None, None, one, 0, None) == 0
+
+
+def test_modules_run_the_stock_operators_on_cpu_tensors():
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    from distill_bev_amd.registry import ConvModule
+    torch.manual_seed(2)
+    net = nn.Sequential(nn.Conv2d(6, 16, 1), nn.GroupNorm(4, 16), nn.SiLU(), ConvModule(16, 8, 3, padding=1, norm_cfg=dict(type="GN", num_groups=2)),
+                        nn.GroupNorm(2, 8), nn.Conv2d(8, 4, 1, bias=False), nn.ReLU())
+    keys = list(net.state_dict())
+    x = torch.randn(2, 6, 5, 4)
+    ref = net(x)
+    assert GN.fuse_gn_act_modules(net, "int8") == 3 and GN.fuse_gn_act_modules(net, "int8") == 0
+    assert [m.act for m in net.modules() if isinstance(m, GN.GroupNormAct)] == ["silu", "relu", "none"]
+    assert A.use_act8(net, "e4m3") == 3 and A.use_act8(net, "e4m3") == 0          # two 1x1 convolutions, the ReLU behind one of them
+    assert type(net[6]) is A.Act8Activation and list(net.state_dict()) == keys
+    assert torch.allclose(net(x), ref, atol=1e-6)
+    net(x).sum().backward()
+    ffn = nn.Sequential(nn.Sequential(nn.Linear(8, 16), nn.ReLU(inplace=True), nn.Dropout(0.0)), nn.Linear(16, 8), nn.GELU())
+    t = torch.randn(3, 8)
+    ref = ffn(t)
+    assert A.use_act8(ffn) == 4 and torch.allclose(ffn(t), ref, atol=1e-6)
+    mha = nn.MultiheadAttention(8, 2)
+    assert A.use_act8(mha) == 0

@@ -6,6 +6,7 @@ the HIP stream is torch's *current* stream so the kernels order correctly with t
 surrounding PyTorch-ROCm ops (the reference launched on the default stream,
 bev_pool_cuda.cu:88 -- noted in SURVEY 8b).
 """
+import contextlib
 import ctypes
 import os
 
@@ -498,6 +499,19 @@ def exported_symbols():
 
 def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on(dev):
+    """context in which `dev` is the current device; free where it already is"""
+    return _HERE_ALREADY if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def raw_stream(dev):
+    """torch's current stream of `dev` as an integer handle (stream_ptr without building a Stream object)"""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def check(rc, what):

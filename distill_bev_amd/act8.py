@@ -95,24 +95,31 @@ def rows_of(x, dim):
 
 
 class Checkpoint8:
-    """What `pack` keeps of a tensor: codes uint8 [rows, C], scales uint8 [rows, ceil(C / 32)], the format, and the tensor's shape, channel
-    dimension and type."""
-    __slots__ = ("codes", "scales", "fmt", "shape", "dim", "dtype")
+    """What `pack` keeps of a tensor: one uint8 buffer -- the codes [rows, C], then the scale bytes [rows, ceil(C / 32)] --, the format, and
+    the tensor's shape, channel dimension and type."""
+    __slots__ = ("buf", "rows", "C", "fmt", "shape", "dim", "dtype")
 
-    def __init__(self, codes, scales, fmt, shape, dim, dtype):
-        self.codes, self.scales, self.fmt, self.shape, self.dim, self.dtype = codes, scales, fmt, tuple(shape), dim, dtype
+    def __init__(self, buf, rows, C, fmt, shape, dim, dtype):
+        self.buf, self.rows, self.C, self.fmt, self.shape, self.dim, self.dtype = buf, rows, C, fmt, tuple(shape), dim, dtype
+
+    @property
+    def codes(self):
+        return self.buf[:self.rows * self.C].view(self.rows, self.C)
+
+    @property
+    def scales(self):
+        return self.buf[self.rows * self.C:].view(self.rows, -(-self.C // BLOCK))
 
     @property
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return self.buf.numel()
 
     def __repr__(self):
         return f"Checkpoint8({self.fmt}, shape={self.shape}, {self.dtype}, {self.nbytes} bytes)"
 
 
-def _buffers(rows, C, dev):
-    return (torch.empty((rows, C), dtype=torch.uint8, device=dev),
-            torch.empty((rows, -(-C // BLOCK)), dtype=torch.uint8, device=dev))
+def _buffer(rows, C, dev):
+    return torch.empty((rows * (C + -(-C // BLOCK)),), dtype=torch.uint8, device=dev)
 
 
 def _dim(x, channel_dim):
@@ -131,12 +138,13 @@ def pack(x, fmt="int8", channel_dim=None):
     f, dt = _fmt(fmt), _dtype(x)
     dev = L.require_cuda(x)
     dim = _dim(x, channel_dim)
-    with torch.cuda.device(dev):
+    with L.on(dev):
         v, rows, C, stride = rows_of(x.detach(), dim)
-        codes, scales = _buffers(rows, C, dev)
+        buf = _buffer(rows, C, dev)
         if rows:
-            L.call("dbev_act8_pack", L.ptr(v), dt, rows, C, stride, f, L.ptr(codes), L.ptr(scales), L.stream_ptr(dev))
-    return Checkpoint8(codes, scales, fmt, x.shape, dim, x.dtype)
+            p = buf.data_ptr()
+            L.call("dbev_act8_pack", v.data_ptr(), dt, rows, C, stride, f, p, p + rows * C, L.raw_stream(dev))
+    return Checkpoint8(buf, rows, C, fmt, x.shape, dim, x.dtype)
 
 
 def unpack(ck, dtype=None):
@@ -144,43 +152,53 @@ def unpack(ck, dtype=None):
     dtype = ck.dtype if dtype is None else dtype
     if dtype not in DTYPES:
         raise L.DbevHipError(f"unpack: float32, bfloat16 or float16 expected, got {dtype}")
-    dev = L.require_cuda(ck.codes, ck.scales)
-    with torch.cuda.device(dev):
+    dev = L.require_cuda(ck.buf)
+    with L.on(dev):
         out = empty_dense(ck.shape, ck.dim, dtype, dev)
-        if ck.codes.numel():
-            L.call("dbev_act8_unpack", L.ptr(ck.codes), L.ptr(ck.scales), FORMATS[ck.fmt], ck.codes.shape[0], ck.codes.shape[1], L.ptr(out),
-                   DTYPES[dtype], L.stream_ptr(dev))
+        if ck.buf.numel():
+            p = ck.buf.data_ptr()
+            L.call("dbev_act8_unpack", p, p + ck.rows * ck.C, FORMATS[ck.fmt], ck.rows, ck.C, out.data_ptr(), DTYPES[dtype], L.raw_stream(dev))
     return out
+
+
+def _act_forward(x, act, fmt, dim):
+    """-> act(x), the checkpoint's buffer (None without `fmt`), rows, C"""
+    dev = x.device
+    with L.on(dev):
+        v, rows, C, stride = rows_of(x, dim)
+        y = empty_dense(x.shape, dim, x.dtype, dev)
+        buf = p = q = None
+        if fmt is not None:
+            buf = _buffer(rows, C, dev)
+            p = buf.data_ptr()
+            q = p + rows * C
+        if rows:
+            L.call("dbev_act8_activation_forward", v.data_ptr(), DTYPES[x.dtype], rows, C, stride, ACTS[act], FORMATS[fmt] if fmt else 0,
+                   y.data_ptr(), p, q, L.raw_stream(dev))
+    return y, buf, rows, C
 
 
 class _Activation8(Function):
     @staticmethod
     def forward(ctx, x, act, fmt, dim):
-        dev = x.device
-        with torch.cuda.device(dev):
-            v, rows, C, stride = rows_of(x, dim)
-            y = empty_dense(x.shape, dim, x.dtype, dev)
-            keep = fmt is not None and ctx.needs_input_grad[0]
-            codes, scales = _buffers(rows, C, dev) if keep else (None, None)
-            if rows:
-                L.call("dbev_act8_activation_forward", L.ptr(v), DTYPES[x.dtype], rows, C, stride, ACTS[act], FORMATS[fmt] if keep else 0,
-                       L.ptr(y), L.ptr(codes), L.ptr(scales), L.stream_ptr(dev))
-        ctx.save_for_backward(codes, scales)
+        y, buf, rows, C = _act_forward(x, act, fmt, dim)
+        ctx.save_for_backward(buf)
         ctx.cfg = (act, fmt, dim, rows, C)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        codes, scales = ctx.saved_tensors
+        buf, = ctx.saved_tensors
         act, fmt, dim, rows, C = ctx.cfg
         dev = gy.device
-        with torch.cuda.device(dev):
+        with L.on(dev):
             g, _, _, stride = rows_of(gy, dim)
             dx = empty_dense(gy.shape, dim, gy.dtype, dev)
             if rows:
-                L.call("dbev_act8_activation_backward", L.ptr(g), DTYPES[gy.dtype], stride, L.ptr(codes), L.ptr(scales), FORMATS[fmt], rows, C,
-                       ACTS[act], L.ptr(dx), L.stream_ptr(dev))
+                p = buf.data_ptr()
+                L.call("dbev_act8_activation_backward", g.data_ptr(), DTYPES[gy.dtype], stride, p, p + rows * C, FORMATS[fmt], rows, C,
+                       ACTS[act], dx.data_ptr(), L.raw_stream(dev))
         return dx, None, None, None
 
 
@@ -189,23 +207,16 @@ def activation(x, act="gelu", checkpoint="int8", channel_dim=None):
     _act(act), _fmt(checkpoint), _dtype(x)
     L.require_cuda(x)
     dim = _dim(x, channel_dim)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         return _Activation8.apply(x, act, checkpoint, dim)
-    dev = x.device
-    with torch.cuda.device(dev):
-        v, rows, C, stride = rows_of(x.detach(), dim)
-        y = empty_dense(x.shape, dim, x.dtype, dev)
-        if rows:
-            L.call("dbev_act8_activation_forward", L.ptr(v), DTYPES[x.dtype], rows, C, stride, ACTS[act], 0, L.ptr(y), None, None, L.stream_ptr(dev))
-    return y
+    return _act_forward(x.detach(), act, None, dim)[0]
 
 
-def _weight_gradient(codes, scales, fmt, gy2, bias):
-    """gy2 [M, Co] dense -> (gw [Co, Ci], gb [Co] or None) in gy2's type"""
+def _weight_gradient(buf, fmt, Ci, gy2, bias):
+    """checkpoint buffer of [M, Ci], gy2 [M, Co] dense -> (gw [Co, Ci], gb [Co] or None) in gy2's type"""
     dev = gy2.device
     M, Co = gy2.shape
-    Ci = codes.shape[1]
-    with torch.cuda.device(dev):
+    with L.on(dev):
         gw = torch.empty((Co, Ci), dtype=gy2.dtype, device=dev)
         gb = torch.empty((Co,), dtype=gy2.dtype, device=dev) if bias else None
         if Co and Ci:
@@ -213,8 +224,11 @@ def _weight_gradient(codes, scales, fmt, gy2, bias):
             if nbytes == 0:
                 raise L.DbevHipError(f"weight_gradient: unsupported sizes {M} x {Ci} -> {Co}")
             ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-            L.call("dbev_act8_weight_gradient", L.ptr(gy2), DTYPES[gy2.dtype], L.ptr(codes), L.ptr(scales), FORMATS[fmt], M, Ci, Co, L.ptr(gw),
-                   L.ptr(gb), L.ptr(ws), nbytes, L.stream_ptr(dev))
+            p = buf.data_ptr()
+            L.call("dbev_act8_weight_gradient", gy2.data_ptr(), DTYPES[gy2.dtype], p, p + M * Ci, FORMATS[fmt], M, Ci, Co, gw.data_ptr(),
+                   gb.data_ptr() if bias else None, ws.data_ptr(), nbytes, L.raw_stream(dev))
+        elif bias and Co:
+            gb = gy2.sum(0)
     return gw, gb
 
 
@@ -222,15 +236,17 @@ def weight_gradient(ck, gy, bias=False):
     """gy^T x^ [Co, Ci] (and with `bias` the sums of gy over its rows, [Co]) in gy's type, for the checkpoint of a layer's input and the
     gradient of its output: gy has the checkpoint's shape but for the channel dimension.  fp32 sums, fp32 accuracy for fp32 gy."""
     _dtype(gy, "gy")
-    dev = L.require_cuda(ck.codes, ck.scales, gy)
-    dim = ck.dim
-    want = list(ck.shape)
+    dev = L.require_cuda(ck.buf, gy)
+    dim, want = ck.dim, ck.shape
     if gy.dim() != len(want) or any(gy.shape[d] != want[d] for d in range(len(want)) if d != dim):
         raise ValueError(f"weight_gradient: gy {tuple(gy.shape)} does not match a checkpoint of {ck.shape} with channels in dimension {dim}")
-    with torch.cuda.device(dev):
-        Co = gy.shape[dim]
-        gy2 = gy.detach().movedim(dim, -1).reshape(-1, Co).contiguous() if gy.numel() else gy.new_empty((ck.codes.shape[0], Co))
-        gw, gb = _weight_gradient(ck.codes, ck.scales, ck.fmt, gy2, bias)
+    with L.on(dev):
+        g, rows, Co, stride = rows_of(gy.detach(), dim)
+        if rows == 0:
+            g = gy.new_empty((0, Co))
+        elif stride != Co:
+            g = g.contiguous()
+        gw, gb = _weight_gradient(ck.buf, ck.fmt, ck.C, g, bias)
     return (gw, gb) if bias else gw
 
 
@@ -266,7 +282,7 @@ class _Linear8(Function):
         else:
             y = F.linear(x2, weight, bias)
         ck = pack(x2, fmt, -1) if ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(weight, None if ck is None else ck.codes, None if ck is None else ck.scales)
+        ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt = fmt
         return y
 
@@ -274,9 +290,9 @@ class _Linear8(Function):
     @once_differentiable
     def backward(ctx, gy):
         from . import gemm_bf6 as G
-        weight, codes, scales = ctx.saved_tensors
+        weight, buf = ctx.saved_tensors
         gx = gw = gb = None
-        with torch.cuda.device(gy.device):
+        with L.on(gy.device):
             gy = gy.contiguous()
             if ctx.needs_input_grad[0]:
                 if (G._ON and G._LIN and gy.dtype == torch.float32 and weight.is_contiguous() and gy.numel() < 2 ** 31
@@ -285,7 +301,7 @@ class _Linear8(Function):
                 else:
                     gx = gy @ weight
             if ctx.needs_input_grad[1]:
-                gw, gb = _weight_gradient(codes, scales, ctx.fmt, gy, ctx.needs_input_grad[2])
+                gw, gb = _weight_gradient(buf, ctx.fmt, int(weight.shape[1]), gy, ctx.needs_input_grad[2])
             elif ctx.needs_input_grad[2]:
                 gb = _bias_grad(gy)
         return gx, gw, gb, None
@@ -297,7 +313,7 @@ def linear(x, weight, bias=None, checkpoint="int8"):
     _check_layer(x, weight, bias, "linear")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
-    with torch.cuda.device(x.device):
+    with L.on(x.device):
         x2 = x.reshape(-1, weight.shape[1])
         x2 = x2 if x2.is_contiguous() else x2.contiguous()
         return _Linear8.apply(x2, weight, bias, checkpoint).view(*x.shape[:-1], weight.shape[0])
@@ -320,7 +336,7 @@ class _Conv1x1_8(Function):
         else:
             y = F.conv2d(x, weight, bias)
         ck = pack(x, fmt, 1) if ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(weight, None if ck is None else ck.codes, None if ck is None else ck.scales)
+        ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt, ctx.x_shape = fmt, tuple(x.shape)
         return y
 
@@ -328,9 +344,9 @@ class _Conv1x1_8(Function):
     @once_differentiable
     def backward(ctx, gy):
         from . import gemm_bf6 as G
-        weight, codes, scales = ctx.saved_tensors
+        weight, buf = ctx.saved_tensors
         gx = gw = gb = None
-        with torch.cuda.device(gy.device):
+        with L.on(gy.device):
             gy = gy.contiguous(memory_format=torch.channels_last)
             gy2 = gy.permute(0, 2, 3, 1).reshape(-1, gy.shape[1])
             if ctx.needs_input_grad[0]:
@@ -339,7 +355,7 @@ class _Conv1x1_8(Function):
                     x_like = gy.new_empty(1).expand(ctx.x_shape)          # (only its shape is read)
                     gx = torch.ops.aten.convolution_backward(gy, x_like, weight, None, [1, 1], [0, 0], [1, 1], False, [0, 0], 1, [True, False, False])[0]
             if ctx.needs_input_grad[1]:
-                gw, gb = _weight_gradient(codes, scales, ctx.fmt, gy2, ctx.needs_input_grad[2])
+                gw, gb = _weight_gradient(buf, ctx.fmt, int(weight.shape[1]), gy2, ctx.needs_input_grad[2])
                 gw = gw.view(weight.shape)                                # [Co, Ci] in memory: dense in both memory formats of a 1x1 filter
             elif ctx.needs_input_grad[2]:
                 gb = _bias_grad(gy2)
@@ -353,7 +369,7 @@ def conv1x1(x, weight, bias=None, checkpoint="int8"):
     _check_layer(x, weight, bias, "conv1x1")
     if weight.dim() != 4 or tuple(weight.shape[2:]) != (1, 1) or x.dim() != 4 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"conv1x1: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
-    with torch.cuda.device(x.device):
+    with L.on(x.device):
         return _Conv1x1_8.apply(x.contiguous(memory_format=torch.channels_last), weight, bias, checkpoint)
 
 

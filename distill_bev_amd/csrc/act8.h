@@ -15,15 +15,23 @@
 typedef __bf16 a8_bf16;
 typedef _Float16 a8_f16;
 
-// V values of T as one naturally aligned access (V * sizeof(T) = 2..16 bytes) <-> V floats; float -> T rounds to nearest even
+// V values of T as one naturally aligned access (V * sizeof(T) = 2..16 bytes); `Raw` keeps them as loaded (16-bit types: half the registers
+// of their float values while other loads are in flight).  float -> T rounds to nearest even
 template <typename T, int V>
 struct A8Vec {
   typedef T vec __attribute__((ext_vector_type(V)));
   typedef float fvec __attribute__((ext_vector_type(V)));
-  static __device__ __forceinline__ void load(const T* p, float* v) {
-    const vec t = *reinterpret_cast<const vec*>(p);
+  typedef vec Raw;
+  static __device__ __forceinline__ Raw load(const T* p) { return *reinterpret_cast<const vec*>(p); }
+  static __device__ __forceinline__ void get(const Raw& t, float* v) {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = static_cast<float>(t[i]);
+  }
+  static __device__ __forceinline__ Raw zero() {
+    Raw t;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = static_cast<T>(0.f);
+    return t;
   }
   static __device__ __forceinline__ void store(T* p, const float* v) {
     fvec f;
@@ -34,7 +42,10 @@ struct A8Vec {
 };
 template <typename T>
 struct A8Vec<T, 1> {
-  static __device__ __forceinline__ void load(const T* p, float* v) { v[0] = static_cast<float>(*p); }
+  typedef T Raw;
+  static __device__ __forceinline__ Raw load(const T* p) { return *p; }
+  static __device__ __forceinline__ void get(const Raw& t, float* v) { v[0] = static_cast<float>(t); }
+  static __device__ __forceinline__ Raw zero() { return static_cast<T>(0.f); }
   static __device__ __forceinline__ void store(T* p, const float* v) { *p = static_cast<T>(v[0]); }
 };
 

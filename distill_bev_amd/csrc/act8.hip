@@ -32,33 +32,33 @@ __global__ __launch_bounds__(256) void a8_forward(const T* __restrict__ x, long 
                                                   uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   constexpr int LB = 32 / V;
   const A8Pos p = a8_pos(t, cv);
-  float v[A8_U][V];
+  typename A8Vec<T, V>::Raw raw[A8_U];
 #pragma unroll
   for (int u = 0; u < A8_U; ++u) {
     const long long r = p.row0 + u * p.step;
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[u][i] = 0.f;
-    if (p.on && r < rows) A8Vec<T, V>::load(x + r * xs + static_cast<long long>(p.col) * V, v[u]);
+    raw[u] = p.on && r < rows ? A8Vec<T, V>::load(x + r * xs + static_cast<long long>(p.col) * V) : A8Vec<T, V>::zero();
   }
 #pragma unroll
   for (int u = 0; u < A8_U; ++u) {
     const long long r = p.row0 + u * p.step;
     if (r >= rows) break;                                      // all lanes of a block are on the same row
     const long long o = (r * cv + p.col) * V;
+    float v[V];
+    A8Vec<T, V>::get(raw[u], v);
     if (FMT != DBEV_ACT8_NONE) {
       unsigned m = 0;
 #pragma unroll
-      for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(v[u][i]) & 0x7fffffffu);
+      for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
       const unsigned b = a8_scale_byte<FMT>(a8_block_max<V>(m));
       if (p.on) {
-        *reinterpret_cast<typename A8Bytes<V>::type*>(codes + o) = a8_encode<FMT, V>(v[u], b);
+        *reinterpret_cast<typename A8Bytes<V>::type*>(codes + o) = a8_encode<FMT, V>(v, b);
         if (p.col % LB == 0) scales[r * nb + p.col / LB] = static_cast<uint8_t>(b);
       }
     }
     if (WITH_Y && p.on) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[u][i] = a8_act<ACT>(v[u][i]);
-      A8Vec<T, V>::store(y + o, v[u]);
+      for (int i = 0; i < V; ++i) v[i] = a8_act<ACT>(v[i]);
+      A8Vec<T, V>::store(y + o, v);
     }
   }
 }
@@ -72,14 +72,14 @@ __global__ __launch_bounds__(256) void a8_backward(const T* __restrict__ gy, lon
   if (!p.on) return;
   typename A8Bytes<V>::type c[A8_U];
   unsigned b[A8_U];
-  float g[A8_U][V];
+  typename A8Vec<T, V>::Raw graw[A8_U];
 #pragma unroll
   for (int u = 0; u < A8_U; ++u) {
     const long long r = p.row0 + u * p.step;
     if (r < rows) {
       c[u] = *reinterpret_cast<const typename A8Bytes<V>::type*>(codes + (r * cv + p.col) * V);
       b[u] = scales[r * nb + p.col / LB];
-      if (WITH_GY) A8Vec<T, V>::load(gy + r * gs + static_cast<long long>(p.col) * V, g[u]);
+      if (WITH_GY) graw[u] = A8Vec<T, V>::load(gy + r * gs + static_cast<long long>(p.col) * V);
     }
   }
 #pragma unroll
@@ -89,8 +89,10 @@ __global__ __launch_bounds__(256) void a8_backward(const T* __restrict__ gy, lon
     float v[V];
     a8_decode<FMT, V>(c[u], a8_scale(b[u]), v);
     if (WITH_GY) {
+      float g[V];
+      A8Vec<T, V>::get(graw[u], g);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = a8_act_grad<ACT>(g[u][i], v[i]);
+      for (int i = 0; i < V; ++i) v[i] = a8_act_grad<ACT>(g[i], v[i]);
     }
     A8Vec<T, V>::store(out + (r * cv + p.col) * V, v);
   }

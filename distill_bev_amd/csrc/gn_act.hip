@@ -17,17 +17,26 @@
 namespace {
 
 constexpr int GN_U = 4;                                       // rows in flight per thread
+constexpr int GN_BLOCKS = 4096;                               // workgroups of a launch that the chunking aims at
 
 struct GnArgs {
   long long S;                                                // pixels of an image
   int C, cv, G, cpg, nb;                                      // channels, vector columns, groups, channels a group, blocks of 32 a row
+  // an image's pixels in tiles of RP * GN_U; chunk k takes the tiles k, k + nchunk, ...: the workgroups of an image sweep its memory side by
+  // side, as one front (3 % faster than with a region of its own for each)
   int nchunk;
-  long long rows_per;                                         // pixels a chunk
+  int tiles_each, extra, last;                                // tiles of a chunk, chunks with one more, the chunk that holds the image's last tile
+  int lack;                                                   // pixels missing from that tile
   A8Tile t;
 };
+__host__ __device__ __forceinline__ long long gn_tile(const GnArgs& a) { return static_cast<long long>(a.t.RP) * GN_U; }
+// pixels of a chunk
+__device__ __forceinline__ int gn_rows(const GnArgs& a, int chunk) {
+  return (a.tiles_each + (chunk < a.extra ? 1 : 0)) * (a.t.RP * GN_U) - (chunk == a.last ? a.lack : 0);
+}
 
 // (image, pixel chunk, column range) of this workgroup
-struct GnPos { int n, chunk, cc, col, c0, c1, g0, g1, rp; bool on; long long r0, r1; };
+struct GnPos { int n, chunk, cc, col, c0, c1, g0, g1, rp; bool on; long long r0, step; };
 __device__ __forceinline__ GnPos gn_pos(const GnArgs& a, int block, int V) {
   GnPos p;
   p.cc = block % a.t.ncol;
@@ -41,8 +50,8 @@ __device__ __forceinline__ GnPos gn_pos(const GnArgs& a, int block, int V) {
   p.c1 = min(a.C, p.c0 + a.t.CH * V);
   p.g0 = p.c0 / a.cpg;
   p.g1 = (p.c1 - 1) / a.cpg + 1;
-  p.r0 = p.chunk * a.rows_per;
-  p.r1 = min(a.S, p.r0 + a.rows_per);
+  p.r0 = p.chunk * gn_tile(a);
+  p.step = a.nchunk * gn_tile(a);
   return p;
 }
 
@@ -93,33 +102,29 @@ __global__ __launch_bounds__(256) void gn_stats(const T* __restrict__ x, GnArgs 
 #pragma unroll
   for (int i = 0; i < V; ++i) k[i] = s[i] = q[i] = 0.f;
   if (p.on) {
-    A8Vec<T, V>::load(xi + p.r0 * a.C, k);
-    const long long step = static_cast<long long>(a.t.RP) * GN_U;
-    for (long long r = p.r0 + p.rp; r < p.r1; r += step) {
-      float v[GN_U][V];
+    A8Vec<T, V>::get(A8Vec<T, V>::load(xi + p.r0 * a.C), k);
+    for (long long r = p.r0 + p.rp; r < a.S; r += p.step) {
+      typename A8Vec<T, V>::Raw raw[GN_U];
+#pragma unroll
+      for (int u = 0; u < GN_U; ++u) raw[u] = A8Vec<T, V>::load(xi + min(r + u * a.t.RP, a.S - 1) * a.C);
 #pragma unroll
       for (int u = 0; u < GN_U; ++u) {
-        const long long ru = r + u * a.t.RP;
-        if (ru < p.r1) A8Vec<T, V>::load(xi + ru * a.C, v[u]);
-        else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[u][i] = k[i];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < GN_U; ++u)
+        if (r + u * a.t.RP >= a.S) break;
+        float v[V];
+        A8Vec<T, V>::get(raw[u], v);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = v[u][i] - k[i];
+          const float d = v[i] - k[i];
           s[i] += d;
           q[i] = fmaf(d, d, q[i]);
         }
+      }
     }
   }
   gn_fold<V>(sh, a, p, s, q);
   // per channel: mean and M2 of the chunk's pixels
   const int w = a.t.CH * V;
-  const float rows = static_cast<float>(p.r1 - p.r0);
+  const float rows = static_cast<float>(gn_rows(a, p.chunk));
   const T* x0 = x + static_cast<size_t>(p.n) * a.S * a.C + p.r0 * a.C + p.c0;
   for (int c = threadIdx.x; c < p.c1 - p.c0; c += blockDim.x) {
     const float d = sh[c] / rows;
@@ -143,38 +148,59 @@ __global__ __launch_bounds__(256) void gn_stats(const T* __restrict__ x, GnArgs 
   }
 }
 
-// mean and rstd of the groups this workgroup touches -> sh[2 (g - g0)], merged in fp64 over the image's chunks
-__device__ __forceinline__ void gn_merge_stats(float* sh, const GnArgs& a, const GnPos& p, int V, const float2* __restrict__ part, float eps) {
-  const int ng = p.g1 - p.g0, lanes = gn_lanes(ng), sub = threadIdx.x % lanes;
-  const int w = a.t.CH * V;
-  for (int gi = threadIdx.x / lanes; gi < ng; gi += blockDim.x / lanes) {
-    const int g = p.g0 + gi, cca = g * a.cpg / w, ccb = ((g + 1) * a.cpg - 1) / w + 1;
-    const double D = static_cast<double>(a.S) * a.cpg;
-    double m = 0.0;
-    for (int cc = cca; cc < ccb; ++cc) {
-      const int width = min((cc + 1) * w, (g + 1) * a.cpg) - max(cc * w, g * a.cpg);
-      for (int k = sub; k < a.nchunk; k += lanes) {
-        const double cnt = static_cast<double>(min(a.S, (k + 1) * a.rows_per) - k * a.rows_per) * width;
-        m += cnt * part[((static_cast<size_t>(p.n) * a.nchunk + k) * a.t.ncol + cc) * a.G + g].x;
+// The image's chunk rows of every group that this workgroup touches, added in fp64 into sh[2 gi], sh[2 gi + 1] behind the scratch: neighbouring
+// threads take neighbouring groups of a row (coalesced), the chunks are spread over the rest of the workgroup, eight loads in flight.
+// STATS: entries (mean, M2) -> (mean, rstd), from sum n m and sum (M2 + n m^2): the cancellation costs (mean / spread)^2 of 2^-53;
+// else (A, B) -> (A / D, B / D)
+template <bool STATS>
+__device__ __forceinline__ float* gn_gather(float* sh, const GnArgs& a, const GnPos& p, int V, const float2* __restrict__ part, float eps) {
+  double* scratch = reinterpret_cast<double*>(sh);
+  float* out = sh + 4 * blockDim.x;
+  const int ng = p.g1 - p.g0, w = a.t.CH * V;
+  const int wide = min(ng, static_cast<int>(blockDim.x)), ph = threadIdx.x / wide, np = blockDim.x / wide;
+  const float2* image = part + static_cast<size_t>(p.n) * a.nchunk * a.t.ncol * a.G;
+  const double D = static_cast<double>(a.S) * a.cpg;
+  for (int first = 0; first < ng; first += wide) {
+    const int gi = first + threadIdx.x - ph * wide, g = p.g0 + gi;
+    double s0 = 0.0, s1 = 0.0;
+    if (ph < np && gi < ng) {
+      const int cca = a.t.ncol > 1 ? g * a.cpg / w : 0, ccb = a.t.ncol > 1 ? ((g + 1) * a.cpg - 1) / w + 1 : 1;
+      for (int cc = cca; cc < ccb; ++cc) {
+        const int width = a.t.ncol > 1 ? min((cc + 1) * w, (g + 1) * a.cpg) - max(cc * w, g * a.cpg) : a.cpg;
+#pragma unroll 8
+        for (int k = ph; k < a.nchunk; k += np) {
+          const float2 e = image[(static_cast<size_t>(k) * a.t.ncol + cc) * a.G + g];
+          if (STATS) {
+            const double cnt = static_cast<double>(gn_rows(a, k)) * width, m = e.x;
+            s0 += cnt * m;
+            s1 += e.y + cnt * m * m;
+          } else {
+            s0 += e.x;
+            s1 += e.y;
+          }
+        }
       }
     }
-    m = gn_lane_sum(m, lanes) / D;
-    double m2 = 0.0;
-    for (int cc = cca; cc < ccb; ++cc) {
-      const int width = min((cc + 1) * w, (g + 1) * a.cpg) - max(cc * w, g * a.cpg);
-      for (int k = sub; k < a.nchunk; k += lanes) {
-        const double cnt = static_cast<double>(min(a.S, (k + 1) * a.rows_per) - k * a.rows_per) * width;
-        const float2 e = part[((static_cast<size_t>(p.n) * a.nchunk + k) * a.t.ncol + cc) * a.G + g];
-        m2 += e.y + cnt * (e.x - m) * (e.x - m);
+    scratch[threadIdx.x] = s0;
+    scratch[blockDim.x + threadIdx.x] = s1;
+    __syncthreads();
+    if (ph == 0 && gi < ng) {
+      for (int i = 1; i < np; ++i) {
+        s0 += scratch[threadIdx.x + i * wide];
+        s1 += scratch[blockDim.x + threadIdx.x + i * wide];
       }
+      s0 /= D;
+      s1 /= D;
+      if (STATS) {
+        const double var = s1 - s0 * s0;
+        s1 = 1.0 / sqrt((var < 0.0 ? 0.0 : var) + static_cast<double>(eps));
+      }
+      out[2 * gi] = static_cast<float>(s0);
+      out[2 * gi + 1] = static_cast<float>(s1);
     }
-    m2 = gn_lane_sum(m2, lanes) / D;
-    if (sub == 0) {
-      sh[2 * gi] = static_cast<float>(m);
-      sh[2 * gi + 1] = static_cast<float>(1.0 / sqrt(m2 + static_cast<double>(eps)));
-    }
+    __syncthreads();
   }
-  __syncthreads();
+  return out;
 }
 
 template <typename T, int V, int FMT, int ACT>
@@ -184,52 +210,51 @@ __global__ __launch_bounds__(256) void gn_apply(const T* __restrict__ x, GnArgs 
   extern __shared__ float sh[];
   constexpr int LB = 32 / V;
   const GnPos p = gn_pos(a, blockIdx.x, V);
-  gn_merge_stats(sh, a, p, V, part, eps);
+  const float* st = gn_gather<true>(sh, a, p, V, part, eps);
   if (mean != nullptr && p.chunk == 0)
     for (int gi = threadIdx.x; gi < p.g1 - p.g0; gi += blockDim.x)
       if ((p.g0 + gi) * a.cpg >= p.c0) {                      // the column range in which the group begins
-        mean[static_cast<size_t>(p.n) * a.G + p.g0 + gi] = sh[2 * gi];
-        rstd[static_cast<size_t>(p.n) * a.G + p.g0 + gi] = sh[2 * gi + 1];
+        mean[static_cast<size_t>(p.n) * a.G + p.g0 + gi] = st[2 * gi];
+        rstd[static_cast<size_t>(p.n) * a.G + p.g0 + gi] = st[2 * gi + 1];
       }
   if (p.rp >= a.t.RP) return;
   float mu[V], sc[V], bt[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = p.on ? p.col * V + i : 0, gi = p.on ? c / a.cpg - p.g0 : 0;
-    mu[i] = sh[2 * gi];
-    sc[i] = sh[2 * gi + 1] * (gamma != nullptr ? gamma[c] : 1.f);
+    mu[i] = st[2 * gi];
+    sc[i] = st[2 * gi + 1] * (gamma != nullptr ? gamma[c] : 1.f);
     bt[i] = beta != nullptr ? beta[c] : 0.f;
   }
   const size_t base = static_cast<size_t>(p.n) * a.S;
-  const long long step = static_cast<long long>(a.t.RP) * GN_U;
-  for (long long r = p.r0 + p.rp; r < p.r1; r += step) {
-    float v[GN_U][V];
+  for (long long r = p.r0 + p.rp; r < a.S; r += p.step) {
+    typename A8Vec<T, V>::Raw raw[GN_U];
 #pragma unroll
     for (int u = 0; u < GN_U; ++u) {
       const long long ru = r + u * a.t.RP;
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[u][i] = 0.f;
-      if (p.on && ru < p.r1) A8Vec<T, V>::load(x + (base + ru) * a.C + static_cast<size_t>(p.col) * V, v[u]);
+      raw[u] = p.on && ru < a.S ? A8Vec<T, V>::load(x + (base + ru) * a.C + static_cast<size_t>(p.col) * V) : A8Vec<T, V>::zero();
     }
 #pragma unroll
     for (int u = 0; u < GN_U; ++u) {
       const long long ru = r + u * a.t.RP;
-      if (ru >= p.r1) break;                                  // all lanes of a block are on the same pixel
+      if (ru >= a.S) break;                                  // all lanes of a block are on the same pixel
+      float v[V];
+      A8Vec<T, V>::get(raw[u], v);
       const size_t o = (base + ru) * a.C + static_cast<size_t>(p.col) * V;
       if (FMT != DBEV_ACT8_NONE) {
         unsigned m = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(v[u][i]) & 0x7fffffffu);
+        for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
         const unsigned b = a8_scale_byte<FMT>(a8_block_max<V>(m));
         if (p.on) {
-          *reinterpret_cast<typename A8Bytes<V>::type*>(codes + o) = a8_encode<FMT, V>(v[u], b);
+          *reinterpret_cast<typename A8Bytes<V>::type*>(codes + o) = a8_encode<FMT, V>(v, b);
           if (p.col % LB == 0) scales[(base + ru) * a.nb + p.col / LB] = static_cast<uint8_t>(b);
         }
       }
       if (p.on) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[u][i] = a8_act<ACT>(fmaf(v[u][i] - mu[i], sc[i], bt[i]));
-        A8Vec<T, V>::store(y + o, v[u]);
+        for (int i = 0; i < V; ++i) v[i] = a8_act<ACT>(fmaf(v[i] - mu[i], sc[i], bt[i]));
+        A8Vec<T, V>::store(y + o, v);
       }
     }
   }
@@ -240,19 +265,17 @@ template <typename T, int V, int FMT>
 struct GnX {
   typename A8Bytes<V>::type c;
   unsigned b;
-  float v[V];
+  typename A8Vec<T, V>::Raw v;
   __device__ __forceinline__ void load(const T* x, const uint8_t* codes, const uint8_t* scales, size_t row, int C, int nb, int col) {
-    if (FMT == DBEV_ACT8_NONE) A8Vec<T, V>::load(x + row * C + static_cast<size_t>(col) * V, v);
+    if (FMT == DBEV_ACT8_NONE) v = A8Vec<T, V>::load(x + row * C + static_cast<size_t>(col) * V);
     else {
       c = *reinterpret_cast<const typename A8Bytes<V>::type*>(codes + row * C + static_cast<size_t>(col) * V);
       b = scales[row * nb + col / (32 / V)];
     }
   }
   __device__ __forceinline__ void get(float* o) const {
-    if (FMT == DBEV_ACT8_NONE) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = v[i];
-    } else a8_decode<FMT, V>(c, a8_scale(b), o);
+    if (FMT == DBEV_ACT8_NONE) A8Vec<T, V>::get(v, o);
+    else a8_decode<FMT, V>(c, a8_scale(b), o);
   }
 };
 
@@ -278,27 +301,27 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce(const T* __restrict__ gy, c
       bt[i] = k.beta != nullptr ? k.beta[c] : 0.f;
     }
     const size_t base = static_cast<size_t>(p.n) * a.S;
-    const long long step = static_cast<long long>(a.t.RP) * GN_U;
-    for (long long r = p.r0 + p.rp; r < p.r1; r += step) {
-      float d[GN_U][V];
+    for (long long r = p.r0 + p.rp; r < a.S; r += p.step) {
+      typename A8Vec<T, V>::Raw draw[GN_U];
       GnX<T, V, FMT> xv[GN_U];
 #pragma unroll
       for (int u = 0; u < GN_U; ++u) {
         const long long ru = r + u * a.t.RP;
-        if (ru < p.r1) {
-          A8Vec<T, V>::load(gy + (base + ru) * a.C + static_cast<size_t>(p.col) * V, d[u]);
+        if (ru < a.S) {
+          draw[u] = A8Vec<T, V>::load(gy + (base + ru) * a.C + static_cast<size_t>(p.col) * V);
           xv[u].load(x, codes, scales, base + ru, a.C, a.nb, p.col);
         }
       }
 #pragma unroll
       for (int u = 0; u < GN_U; ++u) {
-        if (r + u * a.t.RP >= p.r1) break;
-        float v[V];
+        if (r + u * a.t.RP >= a.S) break;
+        float v[V], d[V];
         xv[u].get(v);
+        A8Vec<T, V>::get(draw[u], d);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float xh = (v[i] - mu[i]) * rs[i];
-          const float g = a8_act_grad<ACT>(d[u][i], fmaf(xh, gm[i], bt[i]));
+          const float g = a8_act_grad<ACT>(d[i], fmaf(xh, gm[i], bt[i]));
           s[i] += g;
           q[i] = fmaf(g, xh, q[i]);
         }
@@ -326,14 +349,13 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce(const T* __restrict__ gy, c
 
 constexpr int GN_PC = 8;                                      // channels of a workgroup that adds the parameter gradients up (64-byte pieces of a row)
 
-// dgamma, dbeta: the rows of pc added in a fixed order, fp64 (a row is one chunk's fp32 sum)
-__device__ __forceinline__ void gn_param_grads(double* sh, const GnArgs& a, int N, int block, const float2* __restrict__ pc, float* __restrict__ dgamma,
-                                               float* __restrict__ dbeta) {
+// dgamma, dbeta: the rows of pc (one chunk's fp32 sums each) added in a fixed order in fp64
+__device__ __forceinline__ void gn_param_grads(double* sh, const GnArgs& a, long long rows, int block, const float2* __restrict__ pc,
+                                               float* __restrict__ dgamma, float* __restrict__ dbeta) {
   const int c = block * GN_PC + threadIdx.x % GN_PC, ph = threadIdx.x / GN_PC, np = blockDim.x / GN_PC;
-  const long long rows = static_cast<long long>(N) * a.nchunk;
   double s = 0.0, q = 0.0;
   if (c < a.C) {
-#pragma unroll 4
+#pragma unroll 8
     for (long long r = ph; r < rows; r += np) {
       const float2 e = pc[r * a.C + c];
       s += e.x;
@@ -356,33 +378,14 @@ __device__ __forceinline__ void gn_param_grads(double* sh, const GnArgs& a, int 
 template <typename T, int V, int FMT, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
                                                  const uint8_t* __restrict__ scales, GnArgs a, GnCoef k, const float2* __restrict__ pc,
-                                                 const float2* __restrict__ pg, int N, int npar, T* __restrict__ dx, float* __restrict__ dgamma,
-                                                 float* __restrict__ dbeta) {
+                                                 const float2* __restrict__ pg, int N, int npar, T* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta) {
   extern __shared__ float sh[];
   if (static_cast<int>(blockIdx.x) < npar) {
-    gn_param_grads(reinterpret_cast<double*>(sh), a, N, blockIdx.x, pc, dgamma, dbeta);
+    gn_param_grads(reinterpret_cast<double*>(sh), a, static_cast<long long>(N) * a.nchunk, blockIdx.x, pc, dgamma, dbeta);
     return;
   }
   const GnPos p = gn_pos(a, static_cast<int>(blockIdx.x) - npar, V);
-  const int ng = p.g1 - p.g0, lanes = gn_lanes(ng), sub = threadIdx.x % lanes, w = a.t.CH * V;
-  const double D = static_cast<double>(a.S) * a.cpg;
-  for (int gi = threadIdx.x / lanes; gi < ng; gi += blockDim.x / lanes) {
-    const int g = p.g0 + gi, cca = g * a.cpg / w, ccb = ((g + 1) * a.cpg - 1) / w + 1;
-    double A = 0.0, B = 0.0;
-    for (int cc = cca; cc < ccb; ++cc)
-      for (int c = sub; c < a.nchunk; c += lanes) {
-        const float2 e = pg[((static_cast<size_t>(p.n) * a.nchunk + c) * a.t.ncol + cc) * a.G + g];
-        A += e.x;
-        B += e.y;
-      }
-    A = gn_lane_sum(A, lanes);
-    B = gn_lane_sum(B, lanes);
-    if (sub == 0) {
-      sh[2 * gi] = static_cast<float>(A / D);
-      sh[2 * gi + 1] = static_cast<float>(B / D);
-    }
-  }
-  __syncthreads();
+  const float* ab = gn_gather<false>(sh, a, p, V, pg, 0.f);
   if (!p.on) return;
   float mu[V], rs[V], gm[V], bt[V], A[V], B[V];
 #pragma unroll
@@ -392,32 +395,32 @@ __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const
     rs[i] = k.rstd[static_cast<size_t>(p.n) * a.G + g];
     gm[i] = k.gamma != nullptr ? k.gamma[c] : 1.f;
     bt[i] = k.beta != nullptr ? k.beta[c] : 0.f;
-    A[i] = sh[2 * (g - p.g0)];
-    B[i] = sh[2 * (g - p.g0) + 1];
+    A[i] = ab[2 * (g - p.g0)];
+    B[i] = ab[2 * (g - p.g0) + 1];
   }
   const size_t base = static_cast<size_t>(p.n) * a.S;
-  const long long step = static_cast<long long>(a.t.RP) * GN_U;
-  for (long long r = p.r0 + p.rp; r < p.r1; r += step) {
-    float d[GN_U][V];
+  for (long long r = p.r0 + p.rp; r < a.S; r += p.step) {
+    typename A8Vec<T, V>::Raw draw[GN_U];
     GnX<T, V, FMT> xv[GN_U];
 #pragma unroll
     for (int u = 0; u < GN_U; ++u) {
       const long long ru = r + u * a.t.RP;
-      if (ru < p.r1) {
-        A8Vec<T, V>::load(gy + (base + ru) * a.C + static_cast<size_t>(p.col) * V, d[u]);
+      if (ru < a.S) {
+        draw[u] = A8Vec<T, V>::load(gy + (base + ru) * a.C + static_cast<size_t>(p.col) * V);
         xv[u].load(x, codes, scales, base + ru, a.C, a.nb, p.col);
       }
     }
 #pragma unroll
     for (int u = 0; u < GN_U; ++u) {
       const long long ru = r + u * a.t.RP;
-      if (ru >= p.r1) break;
-      float v[V];
+      if (ru >= a.S) break;
+      float v[V], d[V];
       xv[u].get(v);
+      A8Vec<T, V>::get(draw[u], d);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float xh = (v[i] - mu[i]) * rs[i];
-        const float g = a8_act_grad<ACT>(d[u][i], fmaf(xh, gm[i], bt[i]));
+        const float g = a8_act_grad<ACT>(d[i], fmaf(xh, gm[i], bt[i]));
         v[i] = rs[i] * (fmaf(gm[i], g, -A[i]) - xh * B[i]);
       }
       A8Vec<T, V>::store(dx + (base + ru) * a.C + static_cast<size_t>(p.col) * V, v);
@@ -426,8 +429,10 @@ __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
-// chunks per image: enough workgroups for eight per CU over the whole batch, at least two rounds of loads per thread, at most 128 (every
-// workgroup of the second launch merges its image's chunk rows)
+// chunks per image: enough workgroups for sixteen per CU over the whole batch (twice what fits: 813 -> 776 us at 48 x 256 x 64 x 176 fp32 against
+// eight), at least two tiles each, at most 128 (every workgroup of the second launch merges its image's chunk rows).  Taking the batch in
+// slices that fit the 256 MB memory-side cache, so that the second launch would find its data there, was slower at every slice size
+// (96 MB: 894 us against 823): a launch's ramp and its merge cost more than the cache gives.
 GnArgs gn_args(int N, long long S, int C, int G, int V) {
   GnArgs a;
   a.S = S;
@@ -437,38 +442,40 @@ GnArgs gn_args(int N, long long S, int C, int G, int V) {
   a.cpg = C / G;
   a.nb = (C + 31) / 32;
   a.t = a8_tile(C, V);
-  long long want = (2048 + static_cast<long long>(N) * a.t.ncol - 1) / (static_cast<long long>(N) * a.t.ncol);
-  const long long least = 2LL * a.t.RP * GN_U;
+  const long long side = static_cast<long long>(N) * a.t.ncol, most = (S + 2 * gn_tile(a) - 1) / (2 * gn_tile(a));
+  long long want = (GN_BLOCKS + side - 1) / side;
   want = want < 1 ? 1 : want > 128 ? 128 : want;
-  const long long most = (S + least - 1) / least;
-  if (want > most) want = most;
-  a.rows_per = (S + want - 1) / want;
-  a.nchunk = static_cast<int>((S + a.rows_per - 1) / a.rows_per);
+  a.nchunk = static_cast<int>(want > most ? most : want);
+  const long long tiles = (S + gn_tile(a) - 1) / gn_tile(a);
+  a.tiles_each = static_cast<int>(tiles / a.nchunk);
+  a.extra = static_cast<int>(tiles % a.nchunk);
+  a.last = static_cast<int>((tiles - 1) % a.nchunk);
+  a.lack = static_cast<int>(tiles * gn_tile(a) - S);
   return a;
 }
 
 size_t gn_lds(const GnArgs& a, int V) {
-  const size_t fold = static_cast<size_t>(2) * a.t.CH * V * (1 + a.t.RP) * sizeof(float), merge = static_cast<size_t>(2) * (a.G < a.t.CH * V ? a.G : a.t.CH * V) * sizeof(float);
-  const size_t par = static_cast<size_t>(2) * a.t.threads * sizeof(double);
-  const size_t m = fold > merge ? fold : merge;
-  return m > par ? m : par;
+  const size_t fold = static_cast<size_t>(2) * a.t.CH * V * (1 + a.t.RP) * sizeof(float);
+  const size_t gather = static_cast<size_t>(2) * a.t.threads * sizeof(double) + static_cast<size_t>(2) * (a.G < a.t.CH * V ? a.G : a.t.CH * V) * sizeof(float);
+  return fold > gather ? fold : gather;
 }
 
 bool gn_ok(int dtype, int N, long long S, int C, int G) {
-  return a8_dtype_ok(dtype) && N >= 0 && S >= 0 && C > 0 && G > 0 && C % G == 0 && C <= 65536 && S <= (1LL << 36) / C &&
+  return a8_dtype_ok(dtype) && N >= 0 && S >= 0 && C > 0 && G > 0 && C % G == 0 && C <= 65536 && S <= (1LL << 36) / C && S <= (1LL << 30) &&
          static_cast<long long>(N) <= (1LL << 22) && (N == 0 || S <= (1LL << 40) / C / N);
 }
 
 // a launch holds fewer than 2^32 threads
 bool gn_grid_ok(int N, const GnArgs& a) { return static_cast<long long>(N) * a.nchunk * a.t.ncol * a.t.threads < (1LL << 32) - (1LL << 26); }
 
-// the plan is made for the narrowest vector width as well: the chunk counts differ, the workspace fits either
-size_t gn_ws(int N, long long S, int C, int G) {
+// chunk rows for whatever vector width a call ends up with: N * nchunk <= GN_BLOCKS / ncol + N
+size_t gn_ws(int N, int C, int G) {
   size_t m = 0;
   for (int v : {1, 2, 4, 8}) {
     if (C % v != 0) continue;
-    const GnArgs a = gn_args(N, S, C, G, v);
-    const size_t b = static_cast<size_t>(N) * a.nchunk * (static_cast<size_t>(a.C) + static_cast<size_t>(a.t.ncol) * a.G) * sizeof(float2);
+    const A8Tile t = a8_tile(C, v);
+    const size_t rows = static_cast<size_t>(GN_BLOCKS / t.ncol) + static_cast<size_t>(N) + 1;
+    const size_t b = rows * (static_cast<size_t>(C) + static_cast<size_t>(t.ncol) * G) * sizeof(float2);
     m = b > m ? b : m;
   }
   return m;
@@ -478,7 +485,7 @@ size_t gn_ws(int N, long long S, int C, int G) {
 
 extern "C" size_t dbev_gn_act_workspace_bytes(int N, long long S, int C, int G) {
   if (!gn_ok(DBEV_DT_F32, N, S, C, G) || N == 0 || S == 0) return 0;
-  return gn_ws(N, S, C, G);
+  return gn_ws(N, C, G);
 }
 
 extern "C" int dbev_gn_act_forward(const void* x, int dtype, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps,
@@ -486,7 +493,7 @@ extern "C" int dbev_gn_act_forward(const void* x, int dtype, int N, long long S,
                                    size_t workspace_bytes, dbevStream_t stream) {
   if (!gn_ok(dtype, N, S, C, G) || !a8_act_ok(act) || !(fmt == DBEV_ACT8_NONE || a8_fmt_ok(fmt))) return DBEV_EINVAL;
   if (N == 0 || S == 0) return 0;
-  if (workspace_bytes < gn_ws(N, S, C, G)) return DBEV_EINVAL;
+  if (workspace_bytes < gn_ws(N, C, G)) return DBEV_EINVAL;
   const int vec = a8_pick_vec(a8_elem_size(dtype), C, C, x, y, nullptr);
   hipStream_t st = dbev_stream(stream);
   float2* part = static_cast<float2*>(workspace);
@@ -508,7 +515,7 @@ extern "C" int dbev_gn_act_backward(const void* gy, int dtype, const void* x, in
                                     float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, dbevStream_t stream) {
   if (!gn_ok(dtype, N, S, C, G) || !a8_act_ok(act) || !(fmt == DBEV_ACT8_NONE ? x != nullptr : a8_fmt_ok(fmt))) return DBEV_EINVAL;
   if (N == 0 || S == 0) return 0;
-  if (workspace_bytes < gn_ws(N, S, C, G)) return DBEV_EINVAL;
+  if (workspace_bytes < gn_ws(N, C, G)) return DBEV_EINVAL;
   const int vec = a8_pick_vec(a8_elem_size(dtype), C, C, gy, dx, fmt == DBEV_ACT8_NONE ? x : nullptr);
   hipStream_t st = dbev_stream(stream);
   const GnCoef k = {gamma, beta, mean, rstd};

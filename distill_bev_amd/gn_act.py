@@ -35,62 +35,70 @@ def _maps(x):
 
 
 def _f32(t):
-    return None if t is None else t.detach().float().contiguous()
+    return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
 
 
-def _forward(x, G, weight, bias, eps, act, fmt, stats):
-    """x dense channels-last -> y, mean, rstd (None without `stats`), codes, scales (None without `fmt`)"""
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _forward(x, N, C, S, G, weight, bias, eps, act, fmt, stats):
+    """x dense channels-last -> y, f32 [2, N, G] of mean and rstd (None without `stats`), the checkpoint's buffer (None without `fmt`)"""
     dev = x.device
-    N, C = x.shape[:2]
-    S = x.numel() // max(1, N * C)
     y = A.empty_dense(x.shape, 1, x.dtype, dev)
-    mean = torch.empty((N, G), dtype=torch.float32, device=dev) if stats else None
-    rstd = torch.empty((N, G), dtype=torch.float32, device=dev) if stats else None
-    codes, scales = A._buffers(N * S, C, dev) if fmt else (None, None)
-    if x.numel():
+    st = torch.empty((2, N, G), dtype=torch.float32, device=dev) if stats else None
+    buf = A._buffer(N * S, C, dev) if fmt else None
+    n = N * S * C
+    if n:
         nbytes = int(L.call("dbev_gn_act_workspace_bytes", N, S, C, G))
         if nbytes == 0:
             raise L.DbevHipError(f"group_norm_act: unsupported size {tuple(x.shape)}, {G} groups")
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        L.call("dbev_gn_act_forward", L.ptr(x), A.DTYPES[x.dtype], N, S, C, G, L.ptr(weight), L.ptr(bias), float(eps), A.ACTS[act], L.ptr(y),
-               L.ptr(mean), L.ptr(rstd), A.FORMATS[fmt] if fmt else 0, L.ptr(codes), L.ptr(scales), L.ptr(ws), nbytes, L.stream_ptr(dev),
-               alg_bytes=3 * x.numel() * x.element_size() + (x.numel() if fmt else 0))
-    return y, mean, rstd, codes, scales
+        mean = _ptr(st)
+        codes = _ptr(buf)
+        L.call("dbev_gn_act_forward", x.data_ptr(), A.DTYPES[x.dtype], N, S, C, G, _ptr(weight), _ptr(bias), eps, A.ACTS[act], y.data_ptr(),
+               mean, mean + 4 * N * G if stats else None, A.FORMATS[fmt] if fmt else 0, codes, codes + n if fmt else None, ws.data_ptr(), nbytes,
+               L.raw_stream(dev), alg_bytes=2 * n * x.element_size() + (n if fmt else 0))
+    return y, st, buf
 
 
 class _GroupNormAct(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, G, eps, act, fmt):
-        with torch.cuda.device(x.device):
-            xd = _maps(x)[0]
+        with L.on(x.device):
+            xd, N, C, S = _maps(x)
             w, b = _f32(weight), _f32(bias)
-            y, mean, rstd, codes, scales = _forward(xd, G, w, b, eps, act, fmt, True)
-        ctx.save_for_backward(None if fmt else xd, codes, scales, w, b, mean, rstd)
-        ctx.cfg = (G, act, fmt, tuple(x.shape), None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+            y, st, buf = _forward(xd, N, C, S, G, w, b, eps, act, fmt, True)
+        ctx.save_for_backward(buf if fmt else xd, w, b, st)
+        ctx.cfg = (G, act, fmt, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        x, codes, scales, w, b, mean, rstd = ctx.saved_tensors
-        G, act, fmt, shape, wt, bt = ctx.cfg
+        kept, w, b, st = ctx.saved_tensors
+        G, act, fmt, wt, bt = ctx.cfg
         dev = gy.device
-        need_w, need_b = w is not None and ctx.needs_input_grad[1], b is not None and ctx.needs_input_grad[2]
-        with torch.cuda.device(dev):
+        _, need_w, need_b = ctx.needs_input_grad[:3]
+        with L.on(dev):
+            dx = A.empty_dense(gy.shape, 1, gy.dtype, dev)
             gy, N, C, S = _maps(gy)
-            dx = A.empty_dense(shape, 1, gy.dtype, dev)
-            new = torch.empty if gy.numel() else torch.zeros
-            dw = new((C,), dtype=torch.float32, device=dev) if need_w else None
-            db = new((C,), dtype=torch.float32, device=dev) if need_b else None
-            if gy.numel():
+            n = N * S * C
+            new = torch.empty if n else torch.zeros
+            dwb = new((2, C), dtype=torch.float32, device=dev) if need_w or need_b else None
+            if n:
                 nbytes = int(L.call("dbev_gn_act_workspace_bytes", N, S, C, G))
                 ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-                n = gy.numel()
-                L.call("dbev_gn_act_backward", L.ptr(gy), A.DTYPES[gy.dtype], L.ptr(x), A.FORMATS[fmt] if fmt else 0, L.ptr(codes), L.ptr(scales),
-                       N, S, C, G, L.ptr(w), L.ptr(b), L.ptr(mean), L.ptr(rstd), A.ACTS[act], L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), nbytes,
-                       L.stream_ptr(dev), alg_bytes=3 * n * gy.element_size() + 2 * (n if fmt else n * gy.element_size()))
-            dw = dw if dw is None or dw.dtype == wt else dw.to(wt)
-            db = db if db is None or db.dtype == bt else db.to(bt)
+                mean, k, dw = st.data_ptr(), kept.data_ptr(), _ptr(dwb)
+                L.call("dbev_gn_act_backward", gy.data_ptr(), A.DTYPES[gy.dtype], None if fmt else k, A.FORMATS[fmt] if fmt else 0,
+                       k if fmt else None, k + n if fmt else None, N, S, C, G, _ptr(w), _ptr(b), mean, mean + 4 * N * G, A.ACTS[act],
+                       dx.data_ptr(), dw if need_w else None, dw + 4 * C if need_b else None, ws.data_ptr(), nbytes, L.raw_stream(dev),
+                       alg_bytes=2 * n * gy.element_size() + (n if fmt else n * gy.element_size()))
+            dw = db = None
+            if need_w:
+                dw = dwb[0] if wt == torch.float32 else dwb[0].to(wt)
+            if need_b:
+                db = dwb[1] if bt == torch.float32 else dwb[1].to(bt)
         return dx if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None
 
 
@@ -116,10 +124,11 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
         raise ValueError(f"group_norm_act: eps {eps}")
     if x.numel() and x.numel() // G == 1:                         # F.group_norm's own refusal
         raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _GroupNormAct.apply(x, weight, bias, G, float(eps), act, checkpoint)
-    with torch.cuda.device(dev):
-        return _forward(_maps(x.detach())[0], G, _f32(weight), _f32(bias), eps, act, None, False)[0]
+    with L.on(dev):
+        xd, N, C, S = _maps(x.detach())
+        return _forward(xd, N, C, S, G, _f32(weight), _f32(bias), float(eps), act, None, False)[0]
 
 
 def _ready(x, gn):

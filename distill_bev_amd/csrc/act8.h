@@ -138,37 +138,49 @@ __device__ __forceinline__ void a8_decode(typename A8Bytes<V>::type c, float s, 
 // exp2 and the reciprocal are the hardware's (1 ulp); relative error of silu ~ (1 + |z|) 2^-23.
 __device__ __forceinline__ float a8_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z)); }
 
-// Q = 1 - Phi(|z|) = exp(-z^2 / 2) * t R(t), t = 1 / (1 + 0.45 |z| / sqrt 2): R is a degree-9 least-maximum fit of erfcx / (2 t) made for
-// this file (relative error 3.2e-8 over |z| <= 14, 3e-7 with fp32 evaluation); e = exp(-z^2 / 2) serves the density of the derivative too.
-__device__ __forceinline__ float a8_normal_tail(float z, float* e) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3181980515339464f, fabsf(z), 1.f));
+// 1 - Phi(|z|) = exp(-z^2 / 2) * t R(t), t = 1 / (1 + p |z|): R is a least-maximum fit of erfcx / (2 t) over |z| <= 14 made for this file.
+// Degree 8: relative error 1.3e-7 (4.2e-7 with fp32 evaluation); degree 5, for results that are rounded to 16 bits: 1.8e-5, a twenty-fifth
+// of fp16's half step.  Returns t, R(t); e = exp(-z^2 / 2) serves the density of the derivative too.
+template <bool LOW>
+__device__ __forceinline__ void a8_normal_tail(float z, float* e, float* t, float* r) {
+  *t = __builtin_amdgcn_rcpf(fmaf(LOW ? 0.32526911934581204f : 0.2828427124746192f, fabsf(z), 1.f));
   *e = __builtin_amdgcn_exp2f(z * z * -0.7213475204444817f);
-  float r = -0.02069561555981636f;
-  r = fmaf(r, t, 0.09534421563148499f);
-  r = fmaf(r, t, -0.15029174089431763f);
-  r = fmaf(r, t, 0.07120098918676376f);
-  r = fmaf(r, t, -0.01117928046733141f);
-  r = fmaf(r, t, 0.05997532978653908f);
-  r = fmaf(r, t, 0.08762603998184204f);
-  r = fmaf(r, t, 0.11413582414388657f);
-  r = fmaf(r, t, 0.12694157660007477f);
-  r = fmaf(r, t, 0.12694266438484192f);
-  return *e * (t * r);
+  float p;
+  if (LOW) {
+    p = fmaf(-0.06317635625600815f, *t, 0.12090154737234116f);
+    p = fmaf(p, *t, 0.06272470206022263f);
+    p = fmaf(p, *t, 0.12026229500770569f);
+    p = fmaf(p, *t, 0.12951712310314178f);
+    p = fmaf(p, *t, 0.12976586818695068f);
+  } else {
+    p = fmaf(0.02512962929904461f, *t, -0.09144552052021027f);
+    p = fmaf(p, *t, 0.08453510701656342f);
+    p = fmaf(p, *t, -0.0027980783488601446f);
+    p = fmaf(p, *t, 0.07071340829133987f);
+    p = fmaf(p, *t, 0.08427148312330246f);
+    p = fmaf(p, *t, 0.1039213016629219f);
+    p = fmaf(p, *t, 0.11283480376005173f);
+    p = fmaf(p, *t, 0.11283793300390244f);
+  }
+  *r = p;
 }
 
-template <int ACT>
+// T: the type that the result is rounded to
+template <int ACT, typename T>
 __device__ __forceinline__ float a8_act(float z) {
   if (ACT == DBEV_ACT_RELU) return z < 0.f ? 0.f : z;              // a NaN passes
   if (ACT == DBEV_ACT_SILU) return z * a8_sigmoid(z);
   if (ACT == DBEV_ACT_GELU) {
-    float e;
-    const float q = a8_normal_tail(z, &e);
+    float e, t, r;
+    a8_normal_tail<sizeof(T) == 2>(z, &e, &t, &r);
+    const float q = e * (t * r);
     return z * (z > 0.f ? 1.f - q : q);
   }
   return z;
 }
 
-// g * act'(z); ReLU's derivative at 0 is 0
+// g * act'(z); ReLU's derivative at 0 is 0.  GELU: Phi(z) + z phi(z) = h for z <= 0 and 1 - h for z > 0, h = 1 - Phi(|z|) - |z| phi(z).
+// (Always the finer fit: the parameter gradients are fp32 sums of these.)
 template <int ACT>
 __device__ __forceinline__ float a8_act_grad(float g, float z) {
   if (ACT == DBEV_ACT_RELU) return z > 0.f ? g : (z == z ? 0.f : z);
@@ -177,9 +189,10 @@ __device__ __forceinline__ float a8_act_grad(float g, float z) {
     return g * (s * fmaf(z, 1.f - s, 1.f));
   }
   if (ACT == DBEV_ACT_GELU) {
-    float e;
-    const float q = a8_normal_tail(z, &e);
-    return g * fmaf(z * 0.3989422804014327f, e, z > 0.f ? 1.f - q : q);
+    float e, t, r;
+    a8_normal_tail<false>(z, &e, &t, &r);
+    const float h = e * fmaf(t, r, -0.3989422804014327f * fabsf(z));
+    return g * (z > 0.f ? 1.f - h : h);
   }
   return g;
 }

@@ -12,86 +12,10 @@
 //   gn_bwd_dx       dx = rstd (gamma g - A / D - xh B / D), D = S C / G; its first workgroups add the per-channel rows up instead
 // Bound by HBM: 3 n es forward and 5 n es backward (n es = bytes of x; with a checkpoint the two reads of x in the backward are 1.03
 // bytes a value).  All sums have a fixed order: run-to-run bit-identical, no atomics.
-#include "act8.h"
+#include "gn_act.h"
+#include "gn_one.h"
 
 namespace {
-
-constexpr int GN_U = 4;                                       // rows in flight per thread
-constexpr int GN_BLOCKS = 4096;                               // workgroups of a launch that the chunking aims at
-
-struct GnArgs {
-  long long S;                                                // pixels of an image
-  int C, cv, G, cpg, nb;                                      // channels, vector columns, groups, channels a group, blocks of 32 a row
-  // an image's pixels in tiles of RP * GN_U; chunk k takes the tiles k, k + nchunk, ...: the workgroups of an image sweep its memory side by
-  // side, as one front (3 % faster than with a region of its own for each)
-  int nchunk;
-  int tiles_each, extra, last;                                // tiles of a chunk, chunks with one more, the chunk that holds the image's last tile
-  int lack;                                                   // pixels missing from that tile
-  A8Tile t;
-};
-__host__ __device__ __forceinline__ long long gn_tile(const GnArgs& a) { return static_cast<long long>(a.t.RP) * GN_U; }
-// pixels of a chunk
-__device__ __forceinline__ int gn_rows(const GnArgs& a, int chunk) {
-  return (a.tiles_each + (chunk < a.extra ? 1 : 0)) * (a.t.RP * GN_U) - (chunk == a.last ? a.lack : 0);
-}
-
-// (image, pixel chunk, column range) of this workgroup
-struct GnPos { int n, chunk, cc, col, c0, c1, g0, g1, rp; bool on; long long r0, step; };
-__device__ __forceinline__ GnPos gn_pos(const GnArgs& a, int block, int V) {
-  GnPos p;
-  p.cc = block % a.t.ncol;
-  const int b = block / a.t.ncol;
-  p.chunk = b % a.nchunk;
-  p.n = b / a.nchunk;
-  p.rp = threadIdx.x / a.t.CH;
-  p.col = p.cc * a.t.CH + (threadIdx.x - p.rp * a.t.CH);
-  p.on = p.rp < a.t.RP && p.col < a.cv;
-  p.c0 = p.cc * a.t.CH * V;
-  p.c1 = min(a.C, p.c0 + a.t.CH * V);
-  p.g0 = p.c0 / a.cpg;
-  p.g1 = (p.c1 - 1) / a.cpg + 1;
-  p.r0 = p.chunk * gn_tile(a);
-  p.step = a.nchunk * gn_tile(a);
-  return p;
-}
-
-// lanes that share one group's work: the workgroup's threads spread over its groups, at most a wave each
-__device__ __forceinline__ int gn_lanes(int ng) {
-  int l = 64;
-  while (l > 1 && ng * l > static_cast<int>(blockDim.x)) l >>= 1;
-  return l;
-}
-template <typename F>
-__device__ __forceinline__ F gn_lane_sum(F v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-// the two per-thread sums of every column -> per channel in sh[0 .. CH V), sh[CH V ..): row phases added in order
-template <int V>
-__device__ __forceinline__ void gn_fold(float* sh, const GnArgs& a, const GnPos& p, const float* s, const float* q) {
-  const int w = a.t.CH * V, lane = threadIdx.x - p.rp * a.t.CH;
-  float* t1 = sh + 2 * w;                                     // [RP][CH V] twice
-  float* t2 = t1 + a.t.RP * w;
-  if (p.rp < a.t.RP) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      t1[p.rp * w + lane * V + i] = s[i];
-      t2[p.rp * w + lane * V + i] = q[i];
-    }
-  }
-  __syncthreads();
-  for (int c = threadIdx.x; c < w; c += blockDim.x) {
-    float a1 = 0.f, a2 = 0.f;
-    for (int r = 0; r < a.t.RP; ++r) {
-      a1 += t1[r * w + c];
-      a2 += t2[r * w + c];
-    }
-    sh[c] = a1;
-    sh[w + c] = a2;
-  }
-  __syncthreads();
-}
 
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gn_stats(const T* __restrict__ x, GnArgs a, float2* __restrict__ part) {
@@ -218,13 +142,12 @@ __global__ __launch_bounds__(256) void gn_apply(const T* __restrict__ x, GnArgs 
         rstd[static_cast<size_t>(p.n) * a.G + p.g0 + gi] = st[2 * gi + 1];
       }
   if (p.rp >= a.t.RP) return;
-  float mu[V], sc[V], bt[V];
+  float sc[V], bt[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = p.on ? p.col * V + i : 0, gi = p.on ? c / a.cpg - p.g0 : 0;
-    mu[i] = st[2 * gi];
     sc[i] = st[2 * gi + 1] * (gamma != nullptr ? gamma[c] : 1.f);
-    bt[i] = beta != nullptr ? beta[c] : 0.f;
+    bt[i] = fmaf(-st[2 * gi], sc[i], beta != nullptr ? beta[c] : 0.f);
   }
   const size_t base = static_cast<size_t>(p.n) * a.S;
   for (long long r = p.r0 + p.rp; r < a.S; r += p.step) {
@@ -253,33 +176,12 @@ __global__ __launch_bounds__(256) void gn_apply(const T* __restrict__ x, GnArgs 
       }
       if (p.on) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = a8_act<ACT>(fmaf(v[i] - mu[i], sc[i], bt[i]));
+        for (int i = 0; i < V; ++i) v[i] = a8_act<ACT, T>(fmaf(v[i], sc[i], bt[i]));
         A8Vec<T, V>::store(y + o, v);
       }
     }
   }
 }
-
-// one vector of the backward pass's view of x: x itself or its checkpoint
-template <typename T, int V, int FMT>
-struct GnX {
-  typename A8Bytes<V>::type c;
-  unsigned b;
-  typename A8Vec<T, V>::Raw v;
-  __device__ __forceinline__ void load(const T* x, const uint8_t* codes, const uint8_t* scales, size_t row, int C, int nb, int col) {
-    if (FMT == DBEV_ACT8_NONE) v = A8Vec<T, V>::load(x + row * C + static_cast<size_t>(col) * V);
-    else {
-      c = *reinterpret_cast<const typename A8Bytes<V>::type*>(codes + row * C + static_cast<size_t>(col) * V);
-      b = scales[row * nb + col / (32 / V)];
-    }
-  }
-  __device__ __forceinline__ void get(float* o) const {
-    if (FMT == DBEV_ACT8_NONE) A8Vec<T, V>::get(v, o);
-    else a8_decode<FMT, V>(c, a8_scale(b), o);
-  }
-};
-
-struct GnCoef { const float *gamma, *beta, *mean, *rstd; };
 
 template <typename T, int V, int FMT, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_reduce(const T* __restrict__ gy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
@@ -291,13 +193,13 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce(const T* __restrict__ gy, c
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = q[i] = 0.f;
   if (p.on) {
-    float mu[V], rs[V], gm[V], bt[V];
+    float mu[V], rs[V], sc[V], bt[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = p.col * V + i;
       mu[i] = k.mean[static_cast<size_t>(p.n) * a.G + c / a.cpg];
       rs[i] = k.rstd[static_cast<size_t>(p.n) * a.G + c / a.cpg];
-      gm[i] = k.gamma != nullptr ? k.gamma[c] : 1.f;
+      sc[i] = rs[i] * (k.gamma != nullptr ? k.gamma[c] : 1.f);
       bt[i] = k.beta != nullptr ? k.beta[c] : 0.f;
     }
     const size_t base = static_cast<size_t>(p.n) * a.S;
@@ -320,13 +222,15 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce(const T* __restrict__ gy, c
         A8Vec<T, V>::get(draw[u], d);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float xh = (v[i] - mu[i]) * rs[i];
-          const float g = a8_act_grad<ACT>(d[i], fmaf(xh, gm[i], bt[i]));
+          const float dev = v[i] - mu[i];
+          const float g = a8_act_grad<ACT>(d[i], fmaf(dev, sc[i], bt[i]));
           s[i] += g;
-          q[i] = fmaf(g, xh, q[i]);
+          q[i] = fmaf(g, dev, q[i]);
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[i] *= rs[i];
   }
   gn_fold<V>(sh, a, p, s, q);
   const int w = a.t.CH * V;
@@ -387,16 +291,16 @@ __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const
   const GnPos p = gn_pos(a, static_cast<int>(blockIdx.x) - npar, V);
   const float* ab = gn_gather<false>(sh, a, p, V, pg, 0.f);
   if (!p.on) return;
-  float mu[V], rs[V], gm[V], bt[V], A[V], B[V];
+  float mu[V], sc[V], bt[V], A[V], B[V];                     // dx = sc g - (rstd A) - (x - mean) (rstd^2 B), sc = rstd gamma
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = p.col * V + i, g = c / a.cpg;
+    const float rs = k.rstd[static_cast<size_t>(p.n) * a.G + g];
     mu[i] = k.mean[static_cast<size_t>(p.n) * a.G + g];
-    rs[i] = k.rstd[static_cast<size_t>(p.n) * a.G + g];
-    gm[i] = k.gamma != nullptr ? k.gamma[c] : 1.f;
+    sc[i] = rs * (k.gamma != nullptr ? k.gamma[c] : 1.f);
     bt[i] = k.beta != nullptr ? k.beta[c] : 0.f;
-    A[i] = ab[2 * (g - p.g0)];
-    B[i] = ab[2 * (g - p.g0) + 1];
+    A[i] = rs * ab[2 * (g - p.g0)];
+    B[i] = rs * rs * ab[2 * (g - p.g0) + 1];
   }
   const size_t base = static_cast<size_t>(p.n) * a.S;
   for (long long r = p.r0 + p.rp; r < a.S; r += p.step) {
@@ -419,9 +323,9 @@ __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const
       A8Vec<T, V>::get(draw[u], d);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float xh = (v[i] - mu[i]) * rs[i];
-        const float g = a8_act_grad<ACT>(d[i], fmaf(xh, gm[i], bt[i]));
-        v[i] = rs[i] * (fmaf(gm[i], g, -A[i]) - xh * B[i]);
+        const float dev = v[i] - mu[i];
+        const float g = a8_act_grad<ACT>(d[i], fmaf(dev, sc[i], bt[i]));
+        v[i] = fmaf(sc[i], g, -fmaf(dev, B[i], A[i]));
       }
       A8Vec<T, V>::store(dx + (base + ru) * a.C + static_cast<size_t>(p.col) * V, v);
     }
@@ -469,8 +373,8 @@ bool gn_ok(int dtype, int N, long long S, int C, int G) {
 bool gn_grid_ok(int N, const GnArgs& a) { return static_cast<long long>(N) * a.nchunk * a.t.ncol * a.t.threads < (1LL << 32) - (1LL << 26); }
 
 // chunk rows for whatever vector width a call ends up with: N * nchunk <= GN_BLOCKS / ncol + N
-size_t gn_ws(int N, int C, int G) {
-  size_t m = 0;
+size_t gn_ws(int N, long long S, int C, int G) {
+  size_t m = gn_one_bytes(N, S, C, G);
   for (int v : {1, 2, 4, 8}) {
     if (C % v != 0) continue;
     const A8Tile t = a8_tile(C, v);
@@ -485,7 +389,7 @@ size_t gn_ws(int N, int C, int G) {
 
 extern "C" size_t dbev_gn_act_workspace_bytes(int N, long long S, int C, int G) {
   if (!gn_ok(DBEV_DT_F32, N, S, C, G) || N == 0 || S == 0) return 0;
-  return gn_ws(N, C, G);
+  return gn_ws(N, S, C, G);
 }
 
 extern "C" int dbev_gn_act_forward(const void* x, int dtype, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps,
@@ -493,9 +397,14 @@ extern "C" int dbev_gn_act_forward(const void* x, int dtype, int N, long long S,
                                    size_t workspace_bytes, dbevStream_t stream) {
   if (!gn_ok(dtype, N, S, C, G) || !a8_act_ok(act) || !(fmt == DBEV_ACT8_NONE || a8_fmt_ok(fmt))) return DBEV_EINVAL;
   if (N == 0 || S == 0) return 0;
-  if (workspace_bytes < gn_ws(N, C, G)) return DBEV_EINVAL;
+  if (workspace_bytes < gn_ws(N, S, C, G)) return DBEV_EINVAL;
   const int vec = a8_pick_vec(a8_elem_size(dtype), C, C, x, y, nullptr);
   hipStream_t st = dbev_stream(stream);
+  if ((fmt == DBEV_ACT8_NONE || reinterpret_cast<uintptr_t>(codes) % 8 == 0) &&
+      gn_one_forward(x, dtype, vec, N, S, C, G, gamma, beta, eps, act, y, mean, rstd, fmt, codes, scales, workspace, st)) {
+    DBEV_LAUNCH_CHECK();
+    return 0;
+  }
   float2* part = static_cast<float2*>(workspace);
   A8_TYPE_SWITCH(dtype, vec, {
     const GnArgs a = gn_args(N, S, C, G, V);
@@ -515,9 +424,14 @@ extern "C" int dbev_gn_act_backward(const void* gy, int dtype, const void* x, in
                                     float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, dbevStream_t stream) {
   if (!gn_ok(dtype, N, S, C, G) || !a8_act_ok(act) || !(fmt == DBEV_ACT8_NONE ? x != nullptr : a8_fmt_ok(fmt))) return DBEV_EINVAL;
   if (N == 0 || S == 0) return 0;
-  if (workspace_bytes < gn_ws(N, C, G)) return DBEV_EINVAL;
+  if (workspace_bytes < gn_ws(N, S, C, G)) return DBEV_EINVAL;
   const int vec = a8_pick_vec(a8_elem_size(dtype), C, C, gy, dx, fmt == DBEV_ACT8_NONE ? x : nullptr);
   hipStream_t st = dbev_stream(stream);
+  if ((fmt == DBEV_ACT8_NONE || reinterpret_cast<uintptr_t>(codes) % 8 == 0) &&
+      gn_one_backward(gy, dtype, vec, x, fmt, codes, scales, N, S, C, G, gamma, beta, mean, rstd, act, dx, dgamma, dbeta, workspace, st)) {
+    DBEV_LAUNCH_CHECK();
+    return 0;
+  }
   const GnCoef k = {gamma, beta, mean, rstd};
   A8_TYPE_SWITCH(dtype, vec, {
     const GnArgs a = gn_args(N, S, C, G, V);

@@ -983,6 +983,10 @@ int dbev_act8_weight_gradient(const void* gy, int dtype, const uint8_t* codes, c
  *   Fixed summation order.  Workspace: dbev_gn_act_workspace_bytes (0: unsupported sizes).
  * ---------------------------------------------------------------------------------- */
 size_t dbev_gn_act_workspace_bytes(int N, long long S, int C, int G);
+/* Large batches are done in one pass over the data, where workgroups wait -- a bounded number of looks -- for their image's sums and a further
+ * launch finishes what did not get them in time.  Sets that number (process-wide; < 0: leaves it) and returns the one before; 0 sends every
+ * tile that is not the last of its image the long way (for tests).  The results are the same bits. */
+int dbev_gn_act_poll_limit(int polls);
 int dbev_gn_act_forward(const void* x, int dtype, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps,
                         int act, void* y, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales, void* workspace,
                         size_t workspace_bytes, dbevStream_t stream);

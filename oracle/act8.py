@@ -48,7 +48,7 @@ def values(codes, scales, fmt):
 
 def restored(x, fmt):
     """x [rows, C] -> x^ f64 (x itself without a format); vectorised, agrees with `values(*quantise(x, fmt))` (tests/test_host_act8.py)"""
-    x = x.detach().cpu().double()
+    x = x.detach().double()
     if fmt is None:
         return x
     rows, C = x.shape
@@ -108,8 +108,8 @@ class LinearFn(torch.autograd.Function):
 def group_norm(x, G, weight, bias, eps, name, fmt=None, gy=None):
     """x [N, S, C] f64 -> y, or with gy (y, dx, dgamma, dbeta, z) by the formulas (z: the activation's argument in the backward)"""
     N, S, C = x.shape
-    w = torch.ones(C, dtype=torch.float64) if weight is None else weight
-    b = torch.zeros(C, dtype=torch.float64) if bias is None else bias
+    w = x.new_ones(C) if weight is None else weight
+    b = x.new_zeros(C) if bias is None else bias
     t = x.view(N, S, G, C // G)
     mean = t.mean((1, 3), keepdim=True)
     rstd = 1 / torch.sqrt(((t - mean) ** 2).mean((1, 3), keepdim=True) + eps)

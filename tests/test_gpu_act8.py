@@ -108,13 +108,13 @@ def test_layouts_strides_and_alignment(dtype, fmt):
              "one row": big[5:6, 7:77], "offset storage": big.view(-1)[5:5 + 64 * 9].view(9, 64)}
     for name, v in views.items():
         ck = A.pack(v, fmt, -1)
-        ref = O.restored(v.reshape(-1, v.shape[-1]), fmt).view(v.shape)
+        ref = O.restored(v.cpu().reshape(-1, v.shape[-1]), fmt).view(v.shape)
         assert torch.equal(A.unpack(ck, torch.float32).cpu().double(), ref), name
     m = _data(2 * 5 * 7, 40, dtype, 4).to(DEV).view(2, 5, 7, 40).permute(0, 3, 1, 2)         # channels-last map
     ck = A.pack(m, fmt)
     out = A.unpack(ck)
     assert ck.dim == 1 and out.shape == m.shape and out.is_contiguous(memory_format=torch.channels_last)
-    assert torch.equal(out.cpu().double(), O.restored(m.permute(0, 2, 3, 1).reshape(-1, 40), fmt).to(dtype).double().view(2, 5, 7, 40).permute(0, 3, 1, 2))
+    assert torch.equal(out.cpu().double(), O.restored(m.cpu().permute(0, 2, 3, 1).reshape(-1, 40), fmt).to(dtype).double().view(2, 5, 7, 40).permute(0, 3, 1, 2))
     assert A.pack(m.contiguous(), fmt).dim == 3
     for shape in ((0, 32), (4, 0), (2, 0, 5)):
         e = A.unpack(A.pack(torch.empty(shape, dtype=dtype, device=DEV), fmt, -1))
@@ -177,12 +177,12 @@ def test_activation_layouts_and_gradient_forms():
     y = A.activation(m, "silu", "int8")
     assert y.is_contiguous(memory_format=torch.channels_last)
     g, = torch.autograd.grad(y.sum(), (m,))                              # an expanded gradient
-    zr = O.restored(m.detach().permute(0, 2, 3, 1).reshape(-1, 40), "int8")
+    zr = O.restored(m.detach().cpu().permute(0, 2, 3, 1).reshape(-1, 40), "int8")
     assert torch.allclose(g.cpu().permute(0, 2, 3, 1).reshape(-1, 40).double(), O.act(zr, "silu")[1], atol=2e-6, rtol=0)
     leaf = base.clone().requires_grad_(True)
     y = A.activation(leaf[:, 3:50], "gelu", "e4m3")                      # a strided input inside a graph
     g, = torch.autograd.grad(y, (leaf,), base[:, 10:57])                 # a strided gradient
-    zr = O.restored(base[:, 3:50], "e4m3")
+    zr = O.restored(base[:, 3:50].cpu(), "e4m3")
     ref = torch.zeros(60, 70, dtype=torch.float64)
     ref[:, 3:50] = base[:, 10:57].cpu().double() * O.act(zr, "gelu")[1]
     assert torch.allclose(g.cpu().double(), ref, atol=1e-5, rtol=1e-6)
@@ -194,7 +194,7 @@ def test_activation_layouts_and_gradient_forms():
     with torch.no_grad():
         leaf.mul_(2.0)                                                   # the checkpoint is kept, not the tensor: nothing to detect
     y.sum().backward()
-    assert torch.allclose(leaf.grad.cpu().double(), O.act(O.restored(base, "int8"), "gelu")[1], atol=2e-6, rtol=0)
+    assert torch.allclose(leaf.grad.cpu().double(), O.act(O.restored(base.cpu(), "int8"), "gelu")[1], atol=2e-6, rtol=0)
 
 
 WG = [(1, 1, 1), (1, 64, 64), (5, 3, 5), (31, 64, 63), (32, 65, 64), (33, 129, 127), (127, 128, 128), (129, 256, 10), (1000, 300, 200), (700, 512, 130),

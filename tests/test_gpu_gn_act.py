@@ -299,3 +299,94 @@ def test_conv_module_with_group_norm_and_the_ledger():
         GN.gn_act(x.double().repeat(1, 2, 1, 1), nn.GroupNorm(4, 16).to(DEV).double())
     assert L.fallback_counts()["gn_act"] == 1
     L.fallback_reset()
+
+
+# ---- batches that go through the one-pass kernels (csrc/gn_one.hip): 2048 register tiles or more, an image of 2 to 512 of them ----------
+ONE = [(260, 4200, 42, 64, 8), (24, 11440, 104, 256, 32), (66, 11000, 100, 80, 16), (31, 2111, 1, 1024, 512), (17, 20999, 1, 192, 3)]
+
+
+def _run(x, w, b, gy, G, act, fmt):
+    from distill_bev_amd import gn_act as GN
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    y = GN.group_norm_act(leaves[0], G, leaves[1], leaves[2], 1e-5, act, fmt)
+    return (y.detach(), *torch.autograd.grad(y, leaves, gy))
+
+
+def _big(N, S, H, C, G, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV)                 # noqa: E731
+    x = (r(N, S, C) * torch.exp(0.5 * r(C)) + r(C)).to(dtype)
+    m = lambda t: t.view(N, H, S // H, C).permute(0, 3, 1, 2)              # noqa: E731
+    return m(x), 1 + 0.3 * r(C), 0.3 * r(C), m(r(N, S, C).to(dtype))
+
+
+@pytest.mark.parametrize("dtype,fmt,act", [(torch.float32, None, "silu"), (torch.float32, "int8", "gelu"), (torch.float32, "e4m3", "none"),
+                                           (torch.bfloat16, None, "gelu"), (torch.bfloat16, "int8", "silu"), (torch.float16, "e4m3", "gelu")])
+@pytest.mark.parametrize("N,S,H,C,G", ONE)
+def test_large_batches(N, S, H, C, G, dtype, fmt, act):
+    """against the oracle evaluated in 64 bits on the device; chains of sums are longer than in the small cases by the channels of a group and
+    the tiles, both under sqrt: the same 4e-6, five times it for the worst of 10^7 elements"""
+    x, w, b, gy = _big(N, S, H, C, G, dtype, S)
+    y, dx, dw, db = _run(x, w, b, gy, G, act, fmt)
+    rows = lambda t: t.movedim(1, -1).reshape(N, S, C).double()            # noqa: E731
+    ry, rdx, rdw, rdb, _ = O.group_norm(rows(x), G, w.double(), b.double(), 1e-5, act, fmt, rows(gy))
+    half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    for got, ref in ((rows(y), ry), (rows(dx), rdx)):
+        d = (got - ref).abs()
+        rms = ref.square().mean().sqrt()
+        assert float(d.norm() / ref.norm()) < 8e-6 + half
+        assert bool((d <= (2e-4 + half) * torch.maximum(ref.abs(), rms)).all())
+    scale = float(rows(gy).abs().sum((0, 1)).max())
+    assert float((dw.double() - rdw).abs().max()) < 4e-6 * scale and float((db.double() - rdb).abs().max()) < 4e-6 * scale
+
+
+@pytest.mark.parametrize("dtype,fmt", [(torch.float32, None), (torch.float32, "int8"), (torch.bfloat16, "e4m3")])
+def test_tiles_that_give_up_waiting_are_finished_with_the_same_bits(dtype, fmt):
+    """a wait of no looks at all: whatever is not there at once goes the long way"""
+    from distill_bev_amd import _lib as L
+    x, w, b, gy = _big(24, 11440, 104, 256, 32, dtype, 1)
+    ref = _run(x, w, b, gy, 32, "silu", fmt)
+    old = L.call("dbev_gn_act_poll_limit", 0)
+    try:
+        for _ in range(3):
+            assert all(torch.equal(p, q) for p, q in zip(_run(x, w, b, gy, 32, "silu", fmt), ref))
+        L.call("dbev_gn_act_poll_limit", 3)
+        assert all(torch.equal(p, q) for p, q in zip(_run(x, w, b, gy, 32, "silu", fmt), ref))
+    finally:
+        assert L.call("dbev_gn_act_poll_limit", old) == 3
+    assert L.call("dbev_gn_act_poll_limit", -1) == old
+    assert all(torch.equal(p, q) for p, q in zip(_run(x, w, b, gy, 32, "silu", fmt), ref))
+
+
+def test_large_batches_side_by_side_and_captured():
+    """several at once on streams of their own, beside other work, and replayed from a graph: the bits of the call alone"""
+    data = [_big(24, 11440, 104, 256, 32, torch.float32, 30 + i) for i in range(3)]
+    alone = [_run(*d, 32, "silu", "int8") for d in data]
+    streams = [torch.cuda.Stream() for _ in data]
+    for _ in range(2):
+        outs = []
+        for s, d in zip(streams, data):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                outs.append(_run(*d, 32, "silu", "int8"))
+        busy = torch.randn(4096, 4096, device=DEV)
+        busy @ busy
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        for a, o in zip(alone, outs):
+            assert all(torch.equal(p, q) for p, q in zip(a, o))
+    sx, w, b, sg = [t.clone(memory_format=torch.preserve_format) for t in data[0]]
+    streams[0].wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(streams[0]):
+        _run(sx, w, b, sg, 32, "silu", "int8")
+    torch.cuda.current_stream().wait_stream(streams[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _run(sx, w, b, sg, 32, "silu", "int8")
+    for i in (1, 2, 0, 1):
+        for t, src in zip((sx, w, b, sg), data[i]):
+            t.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, alone[i]))
+        assert all(torch.equal(p, q) for p, q in zip(_run(*data[2 - i], 32, "silu", "int8"), alone[2 - i]))

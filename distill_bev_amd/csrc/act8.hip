@@ -12,7 +12,10 @@
 
 namespace {
 
-constexpr int A8_U = 4;                                        // rows per thread: 64 bytes in flight per lane before the first use
+#ifndef A8_UU
+#define A8_UU 4
+#endif
+constexpr int A8_U = A8_UU;                                        // rows per thread: 64 bytes in flight per lane before the first use
 
 struct A8Pos { int col; bool on; long long row0, step; };
 

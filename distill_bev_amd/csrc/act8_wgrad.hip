@@ -6,10 +6,21 @@
 //
 // The reduction runs over m, the slow index of both operands, while a matrix instruction wants 8 consecutive m of one channel per lane:
 // a thread fetches 8 rows of a few channels (coalesced along the channels), so that a channel's 8 values sit in its registers and go to
-// LDS as one 16-byte unit [m / 8][channel]; the unit index is channel ^ ((channel >> 4) & 3), which spreads both the strided writes and
-// the reads over all banks.  Workgroup = 4 waves, tile TA output x TB input channels, chunks of 32 rows, two LDS buffers, one barrier per
-// chunk; raw values are fetched through buffer descriptors of the share's rows (a row or channel past the end reads as zero).  The rows
-// are cut into shares, partial sums [share][Co][Ci] are added in a fixed order by a8_wsum: bit-reproducible, no atomics.
+// LDS as one 16-byte unit [m / 8][channel]; the unit index is channel ^ ((channel >> 3) & 3), which spreads both the strided writes and
+// the reads over all banks.  Raw values come through buffer descriptors of the share's rows: a row or channel past the end reads as zero.
+//
+// Workgroup = 4 waves, tile TA output x TB input channels, chunks of 32 rows, two LDS buffers, one barrier a chunk.  The largest tile, 128 x 256,
+// has the register file to itself (one wave a SIMD): one tile of partial sums a CU.  A wave has two chunks of raw values in flight and splits
+// the next chunk UNDER the current one's matrix instructions: a chunk is one basic block -- infinities, the last chunk and the bias sums are
+// handled without branches -- cut into fenced steps of a few matrix instructions with some seven VALU behind each.  The rows are cut into
+// shares, partial sums [share][Co][Ci] are added in a fixed order by a8_wsum: bit-reproducible, no atomics.
+//
+// Measured, fp32 gy (bf16 gy), both launches, int8: 40000 rows, 256 -> 512: 49 us (35); 33792, 1024 -> 256: 68 us (45); 540672, 64 -> 256: 137 us
+// (76, 4.3 TB/s); the fp32 library product alone takes 470 us on the first.  What bounds the first: its 92 MB come at 4.7 TB/s while the chunks
+// run (0.95 us each; their matrix instructions are 0.64 us of that at 2.4 GHz, busy 40 % of the launch), then 32 MB of partial sums go out
+// and come back: 43 + 6.5 us.  Two workgroups a CU (64 MB of partial sums): 43 + 12 us; tiles of 128 x 128: 61 us; two teams of waves on
+// one tile, or the whole chunk ordered as one block: 44 us; four bytes a row of a lane's codes written with a swizzle by 16 channels: 330
+// cycles of LDS conflicts a chunk, by 8: none.
 #include "act8.h"
 
 namespace {
@@ -18,6 +29,7 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
+#define A8W_SGB(mask_, n_) __builtin_amdgcn_sched_group_barrier((mask_), (n_), 0)
 constexpr int A8W_KC = 32;                                    // rows a chunk: two reduction steps of 16
 constexpr unsigned A8W_OOB = 0x80000000u;                     // offset of a channel past the end: beyond every descriptor (shares stay below 2 GiB)
 
@@ -38,16 +50,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t a8w_rsrc(const void* p, long l
 // upper halves of two dwords: (hi(b) << 16) | hi(a)
 __device__ __forceinline__ unsigned a8w_hi2(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// (a, b) -> NP dwords of two bf16 each, their sums are a and b exactly: truncation leaves the remainder exact.  INF: the remainder of an
-// infinity, inf - inf, is taken as 0, so that the products see inf and not a NaN.
-template <int NP, bool INF>
+// (a, b) -> NP dwords of two bf16 each, their sums are a and b exactly: truncation leaves the remainder exact.  The remainder of an infinity,
+// inf - inf, is taken as 0, so that the products see inf and not a NaN.
+template <int NP>
 __device__ __forceinline__ void a8w_split(float a, float b, unsigned* p) {
   p[0] = a8w_hi2(__float_as_uint(a), __float_as_uint(b));
 #pragma unroll
   for (int i = 1; i < NP; ++i) {
     const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-    a = INF && __builtin_isinf(a) ? 0.f : ra;
-    b = INF && __builtin_isinf(b) ? 0.f : rb;
+    a = i == 1 && __builtin_isinf(a) ? 0.f : ra;
+    b = i == 1 && __builtin_isinf(b) ? 0.f : rb;
     p[i] = a8w_hi2(__float_as_uint(a), __float_as_uint(b));
   }
 }
@@ -88,7 +100,7 @@ template <> __device__ __forceinline__ float A8Raw<float, 2, true>::get(int i) c
 template <> __device__ __forceinline__ float A8Raw<float, 2, false>::get(int i) const { return v[i]; }
 
 template <typename T, int FMT, int TA, int TB, bool VEC>
-__global__ __launch_bounds__(256, 2) void a8_wgrad(const T* __restrict__ gy, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+__global__ __launch_bounds__(256, TA * TB > 128 * 128 ? 1 : 2) void a8_wgrad(const T* __restrict__ gy, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                    float* __restrict__ part, float* __restrict__ bpart, long long M, int Co, int Ci, int nb,
                                                    int tiles_n, int tiles, int rows_per, int nsplit) {
   constexpr int NP = A8Pieces<T>::n, CA = TA / 64, CB = TB / 64;
@@ -101,94 +113,85 @@ __global__ __launch_bounds__(256, 2) void a8_wgrad(const T* __restrict__ gy, con
   if (split >= nsplit) return;
   const int co0 = (tile / tiles_n) * TA, ci0 = (tile % tiles_n) * TB;
   const long long mbeg = static_cast<long long>(split) * rows_per;
-  const int nrows = static_cast<int>(min(static_cast<long long>(rows_per), M - mbeg)), nch = (nrows + A8W_KC - 1) / A8W_KC;
+  const int nrows = static_cast<int>(min(static_cast<long long>(rows_per), M - mbeg)), nch = (nrows + 2 * A8W_KC - 1) / (2 * A8W_KC) * 2;     // whole turns of the two register sets; rows past the end are zeros
 
   // staging role: rows 8 w .. 8 w + 7 of the chunk, channels CA lane .. of the gradient, CB lane .. of the checkpoint
   const T* gbase = gy + static_cast<size_t>(mbeg) * Co;
   const uint8_t* cbase = codes + static_cast<size_t>(mbeg) * Ci;
   const uint8_t* sbase = scales + static_cast<size_t>(mbeg) * nb;
-  unsigned aoff[CA], boff[CB], soff[CB];
+  constexpr int EA = VEC ? 1 : CA, EB = VEC ? 1 : CB;         // separately addressed accesses per row
+  unsigned aoff[8][EA], boff[8][EB], soff[8];
 #pragma unroll
-  for (int i = 0; i < CA; ++i) {
-    const int c = co0 + CA * lane + i;
-    aoff[i] = c < Co ? static_cast<unsigned>(8 * w * Co + c) * sizeof(T) : A8W_OOB;
-  }
+  for (int k = 0; k < 8; ++k) {
 #pragma unroll
-  for (int i = 0; i < CB; ++i) {
-    const int c = ci0 + CB * lane + i;
-    boff[i] = c < Ci ? static_cast<unsigned>(8 * w * Ci + c) : A8W_OOB;
-    soff[i] = c < Ci ? static_cast<unsigned>(8 * w * nb + c / 32) : A8W_OOB;
+    for (int i = 0; i < EA; ++i) {
+      const int c = co0 + CA * lane + i;
+      aoff[k][i] = c < Co ? static_cast<unsigned>((8 * w + k) * Co + c) * sizeof(T) : A8W_OOB;
+    }
+#pragma unroll
+    for (int i = 0; i < EB; ++i) {
+      const int c = ci0 + CB * lane + i;
+      boff[k][i] = c < Ci ? static_cast<unsigned>((8 * w + k) * Ci + c) : A8W_OOB;
+    }
+    soff[k] = ci0 + CB * lane < Ci ? static_cast<unsigned>((8 * w + k) * nb + (ci0 + CB * lane) / 32) : A8W_OOB;
   }
-  A8Raw<T, CA, VEC> ra[8];
-  unsigned rb[8], rs[8];                                      // CB code bytes; their block's scale byte (CB channels never straddle a block)
-  const bool bias = bpart != nullptr && ci0 == 0;
+  struct Set { A8Raw<T, CA, VEC> a[8]; unsigned b[8], s[8]; };  // raw values of one chunk: CB code bytes and their block's scale byte (CB channels
+                                                                // never straddle a block) per row
+  Set set0, set1;
   float bsum[CA];
 #pragma unroll
   for (int i = 0; i < CA; ++i) bsum[i] = 0.f;
 
-  auto fetch = [&](int ch) {
+  auto fetch_a = [&](Set& q, int ch) {                        // past the last row: empty descriptors, zeros
     const long long r0 = static_cast<long long>(ch) * A8W_KC, left = nrows - r0;
     const __amdgpu_buffer_rsrc_t gr = a8w_rsrc(gbase + r0 * Co, left * Co * static_cast<long long>(sizeof(T)));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q.a[k].load(gr, aoff[k]);
+  };
+  auto fetch_b = [&](Set& q, int ch) {
+    const long long r0 = static_cast<long long>(ch) * A8W_KC, left = nrows - r0;
     const __amdgpu_buffer_rsrc_t cr = a8w_rsrc(cbase + r0 * Ci, left * Ci);
     const __amdgpu_buffer_rsrc_t sr = a8w_rsrc(sbase + r0 * nb, left * nb);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      unsigned o[CA];
-#pragma unroll
-      for (int i = 0; i < CA; ++i) o[i] = aoff[i] + static_cast<unsigned>(k * Co) * sizeof(T);
-      ra[k].load(gr, o);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const unsigned ko = static_cast<unsigned>(k * Ci);
-      if (VEC && CB == 4) rb[k] = __builtin_amdgcn_raw_buffer_load_b32(cr, boff[0] + ko, 0, 0);
-      else if (VEC && CB == 2) rb[k] = static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(cr, boff[0] + ko, 0, 0));
+      if (VEC && CB == 4) q.b[k] = __builtin_amdgcn_raw_buffer_load_b32(cr, boff[k][0], 0, 0);
+      else if (VEC && CB == 2) q.b[k] = static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(cr, boff[k][0], 0, 0));
       else {
-        rb[k] = 0;
+        q.b[k] = 0;
 #pragma unroll
-        for (int i = 0; i < CB; ++i) rb[k] |= static_cast<unsigned>(static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(cr, boff[i] + ko, 0, 0))) << (8 * i);
+        for (int i = 0; i < CB; ++i)
+          q.b[k] |= static_cast<unsigned>(static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(cr, boff[k][VEC ? 0 : i], 0, 0))) << (8 * i);
       }
-      rs[k] = static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(sr, soff[0] + static_cast<unsigned>(k * nb), 0, 0));
+      q.s[k] = static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(sr, soff[k], 0, 0));
     }
   };
 
-  auto stage = [&](unsigned char* buf) {
-    float top = 0.f;                                          // the largest |gy| of this thread: infinities are rare, one test for all
-    if (NP > 1) {
+  // the staging of one chunk in NU pieces: 4 CA pieces split a pair of rows of one gradient channel, 8 decode a row's codes, CB pair a channel's
+  // rows up and write them; the gradient channels are written behind their fourth piece
+  constexpr int NU = 4 * CA + 8 + CB;
+  unsigned pa[4][3];
+  float xb[8][4];
+  auto piece = [&](int u, const Set& q, unsigned char* buf) {
+    if (u < 4 * CA) {
+      const int c = u / 4, k = u % 4;
+      const float a = q.a[2 * k].get(c), b = q.a[2 * k + 1].get(c);
+      a8w_split<NP>(a, b, pa[k]);
+      bsum[c] += a + b;
+      if (k == 3) {
+        const int row = CA * lane + c;
+        unsigned char* d = buf + (w * TA + (row ^ ((row >> 3) & 3))) * 16;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int c = 0; c < CA; ++c) top = fmaxf(top, fabsf(ra[k].get(c)));
-    }
-#pragma unroll
-    for (int c = 0; c < CA; ++c) {
-      unsigned p[4][3];
-      if (NP > 1 && __builtin_expect(top == __builtin_inff(), 0)) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a8w_split<NP, true>(ra[2 * k].get(c), ra[2 * k + 1].get(c), p[k]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a8w_split<NP, false>(ra[2 * k].get(c), ra[2 * k + 1].get(c), p[k]);
+        for (int i = 0; i < NP; ++i) *reinterpret_cast<uintx4*>(d + i * PLA) = uintx4{pa[0][i], pa[1][i], pa[2][i], pa[3][i]};
       }
-      if (bias) {
+    } else if (u < 4 * CA + 8) {
+      const int k = u - 4 * CA;
+      a8_decode4<FMT>(q.b[k], a8_scale(q.s[k]), xb[k]);
+    } else {
+      const int c = u - 4 * CA - 8, row = CB * lane + c;
+      uintx4 v;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) bsum[c] += ra[2 * k].get(c) + ra[2 * k + 1].get(c);
-      }
-      const int row = CA * lane + c;
-      unsigned char* d = buf + (w * TA + (row ^ ((row >> 4) & 3))) * 16;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) *reinterpret_cast<uintx4*>(d + i * PLA) = uintx4{p[0][i], p[1][i], p[2][i], p[3][i]};
-    }
-    float x[8][4];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) a8_decode4<FMT>(rb[k], a8_scale(rs[k]), x[k]);
-#pragma unroll
-    for (int c = 0; c < CB; ++c) {
-      const int row = CB * lane + c;
-      uintx4 u;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = a8w_hi2(__float_as_uint(x[2 * k][c]), __float_as_uint(x[2 * k + 1][c]));     // exact: bf16 numbers
-      *reinterpret_cast<uintx4*>(buf + NP * PLA + (w * TB + (row ^ ((row >> 4) & 3))) * 16) = u;
+      for (int k = 0; k < 4; ++k) v[k] = a8w_hi2(__float_as_uint(xb[2 * k][c]), __float_as_uint(xb[2 * k + 1][c]));     // exact: bf16 numbers
+      *reinterpret_cast<uintx4*>(buf + NP * PLA + (w * TB + (row ^ ((row >> 3) & 3))) * 16) = v;
     }
   };
 
@@ -203,41 +206,70 @@ __global__ __launch_bounds__(256, 2) void a8_wgrad(const T* __restrict__ gy, con
 #pragma unroll
   for (int a = 0; a < NA; ++a) {
     const int r = (wm * NA + a) * 32 + l31;
-    aaddr[a] = (half * TA + (r ^ ((r >> 4) & 3))) * 16;
+    aaddr[a] = (half * TA + (r ^ ((r >> 3) & 3))) * 16;
   }
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int r = (wn * NB + b) * 32 + l31;
-    baddr[b] = NP * PLA + (half * TB + (r ^ ((r >> 4) & 3))) * 16;
+    baddr[b] = NP * PLA + (half * TB + (r ^ ((r >> 3) & 3))) * 16;
   }
 
-  fetch(0);
-  stage(smem);
-  fetch(1);
-  __syncthreads();
-  for (int ch = 0; ch < nch; ++ch) {
-    const unsigned char* rd = smem + (ch & 1) * BUF;
+  constexpr int MF = 2 * NP * NA * NB;                        // matrix instructions of a chunk
+  // chunk `ch` from buffer `par`; `next` (chunk ch + 1) is staged into the other buffer, a piece between every few matrix
+  // instructions, and refilled with chunk ch + 3.  Steps are fenced off and ordered one by one: matrix instruction, some seven VALU (its 32
+  // cycles), and so on -- as one block of 48 the scheduler lost the order (MFMA busy 35 %, VALU 30 %, hardly overlapping).
+  auto chunk = [&](int ch, int par, Set& next) {
+    const unsigned char* rd = smem + par * BUF;
+    unsigned char* wr = smem + (par ^ 1) * BUF;
+    bf16x8 af[2][NA][NP], bf[2][NB];
+    auto operands = [&](int s) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf16x8 af[NA][NP], bf[NB];
+      for (int b = 0; b < NB; ++b) bf[s][b] = *reinterpret_cast<const bf16x8*>(rd + baddr[b] + s * 2 * TB * 16);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) bf[b] = *reinterpret_cast<const bf16x8*>(rd + baddr[b] + s * 2 * TB * 16);
+      for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
+        for (int a = 0; a < NA; ++a) af[s][a][p] = *reinterpret_cast<const bf16x8*>(rd + p * PLA + aaddr[a] + s * 2 * TA * 16);
+    };
+    operands(0);
+    piece(0, next, wr);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int a = 0; a < NA; ++a) af[a][p] = *reinterpret_cast<const bf16x8*>(rd + p * PLA + aaddr[a] + s * 2 * TA * 16);
+    for (int u = 1; u < NU + 1; ++u) {
+      if (u == NU / 4) operands(1);
+      const int m0 = (u - 1) * MF / NU, m1 = u * MF / NU;
 #pragma unroll
-      for (int p = NP - 1; p >= 0; --p)                       // the smallest pieces first
+      for (int m = m0; m < m1; ++m) {                         // the smallest pieces first
+        const int st = m / (MF / 2), r = m % (MF / 2), p = NP - 1 - r / (NA * NB), a = r % (NA * NB) / NB, b = r % NB;
+        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[st][a][p], bf[st][b], acc[a][b], 0, 0, 0);
+      }
+      if (u < NU) piece(u, next, wr);
+      if (u == 4 * CA) fetch_a(next, ch + 3);
+      if (u == NU) fetch_b(next, ch + 3);
 #pragma unroll
-        for (int a = 0; a < NA; ++a)
-#pragma unroll
-          for (int b = 0; b < NB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[a][p], bf[b], acc[a][b], 0, 0, 0);
-    }
-    if (ch + 1 < nch) {
-      stage(smem + ((ch + 1) & 1) * BUF);
-      fetch(ch + 2);                                          // (past the last chunk: empty descriptors, zeros)
+      for (int m = m0; m < m1; ++m) {
+        A8W_SGB(0x008, 1);
+        A8W_SGB(0x002, 7);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  fetch_a(set0, 0);
+  fetch_b(set0, 0);
+  fetch_a(set1, 1);
+  fetch_b(set1, 1);
+#pragma unroll
+  for (int u = 0; u < NU; ++u) piece(u, set0, smem);
+  fetch_a(set0, 2);
+  fetch_b(set0, 2);
+  __syncthreads();
+  __builtin_amdgcn_sched_barrier(0);
+  // (two bodies: with three sets and two buffers six bodies and a rest were 35 KB of code, and fetching it took longer than the chunks)
+  for (int ch = 0; ch < nch; ch += 2) {
+    chunk(ch, 0, set1);
+    chunk(ch + 1, 1, set0);
   }
 
 #pragma unroll
@@ -252,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void a8_wgrad(const T* __restrict__ gy, con
         if (co + d < Co && ci < Ci) o[static_cast<size_t>(d) * Ci] = acc[a][b][r];
       }
     }
-  if (bias) {                                                 // the four waves' rows of every channel, in order (smem is free behind the last barrier)
+  if (bpart != nullptr && ci0 == 0) {                         // the four waves' rows of every channel, in order (smem is free behind the last barrier)
     float* sb = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int c = 0; c < CA; ++c) sb[w * TA + CA * lane + c] = bsum[c];
@@ -271,16 +303,20 @@ __global__ __launch_bounds__(256) void a8_wsum(const float* __restrict__ part, c
   if (idx >= plane + (gb != nullptr ? Co : 0)) return;
   const float* p = isb ? bpart + (idx - plane) : part + idx;
   const long long step = isb ? Co : plane;
-  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-  int s = 0;
-  for (; s + 4 <= nsplit; s += 4) {
-    s0 += p[(s + 0) * step];
-    s1 += p[(s + 1) * step];
-    s2 += p[(s + 2) * step];
-    s3 += p[(s + 3) * step];
+  float c0 = 0.f, c1 = 0.f, c2 = 0.f, c3 = 0.f;
+  for (int s = 0; s < nsplit; s += 16) {                       // sixteen loads in flight, four chains
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = s + i < nsplit ? p[(s + i) * step] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      c0 += v[i];
+      c1 += v[i + 1];
+      c2 += v[i + 2];
+      c3 += v[i + 3];
+    }
   }
-  for (; s < nsplit; ++s) s0 += p[s * step];
-  (isb ? gb[idx - plane] : gw[idx]) = static_cast<T>((s0 + s1) + (s2 + s3));
+  (isb ? gb[idx - plane] : gw[idx]) = static_cast<T>((c0 + c1) + (c2 + c3));
 }
 
 struct A8WPlan { int ta, tb, tiles_n, tiles, rows_per, nsplit, grid; };
@@ -291,7 +327,7 @@ bool a8w_plan(long long M, int Ci, int Co, A8WPlan* p) {
   p->tb = Ci > 128 ? 256 : Ci > 64 ? 128 : 64;
   p->tiles_n = (Ci + p->tb - 1) / p->tb;
   p->tiles = (Co + p->ta - 1) / p->ta * p->tiles_n;
-  long long ns = 512 / p->tiles;                              // two workgroups a CU
+  long long ns = (p->ta * p->tb > 128 * 128 ? 256 : 512) / p->tiles;    // one workgroup a CU of the largest tile, two of the others
   const long long most = (M + 127) / 128;                     // at least four chunks a share
   ns = ns > most ? most : ns;
   ns = ns < 1 ? 1 : ns;

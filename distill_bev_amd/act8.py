@@ -56,6 +56,8 @@ def _dtype(t, what="x"):
 def dense_dim(x):
     """the dimension along which a tensor's blocks of 32 run: the one whose neighbours are neighbours in memory (1 for channels-last maps),
     the last one longer than 1 if there is none"""
+    if x.dim() and x.shape[-1] > 1 and x.stride(-1) == 1:
+        return x.dim() - 1
     dims = [d for d in range(x.dim()) if x.shape[d] > 1]
     unit = [d for d in dims if x.stride(d) == 1]
     return (unit or dims or [x.dim() - 1])[-1]
@@ -71,6 +73,8 @@ def _strides(shape, dim):
 
 
 def empty_dense(shape, dim, dtype, device):
+    if dim == len(shape) - 1:
+        return torch.empty(shape, dtype=dtype, device=device)
     return torch.empty_strided(tuple(shape), _strides(shape, dim), dtype=dtype, device=device)
 
 
@@ -78,10 +82,12 @@ def rows_of(x, dim):
     """x as (tensor to keep alive, rows, C, row stride) with `dim` as the unit-stride channel dimension: a view wherever the other
     dimensions are evenly spaced, a dense copy otherwise (expanded, transposed, unevenly sliced tensors)"""
     C = x.shape[dim]
-    t = x.movedim(dim, -1)
     rows = x.numel() // C if C else 0
     if C == 0 or rows == 0:
         return x, 0, C, C
+    if dim == x.dim() - 1 and x.is_contiguous():
+        return x.view(rows, C), rows, C, C
+    t = x.movedim(dim, -1)
     if C == 1 or t.stride(-1) == 1:
         try:
             v = t.view(rows, C)

@@ -4,18 +4,18 @@
 //   a8_unpack    codes, scales -> x^                       the reverse
 //   a8_act_fwd   y = act(x), and x's checkpoint            reads n * es, writes n * es + 1.03 n: the checkpoint costs no pass of its own
 //   a8_act_bwd   dx = dy * act'(x^)                        reads n * es + 1.03 n, writes n * es
-// All four are bound by HBM traffic.  A lane holds 16 bytes of a row (2 elements, or 1, where the row length, the stride or an address is
-// off), the 32 channels of a block are 4 (16-bit types) or 8 (fp32) neighbouring lanes and their maximum is taken with DPP moves; a
-// thread keeps its column and handles A8_U rows, all loads first.  Dense rows of a multiple of 32 channels are walked as rows of 32:
-// every access of a wave is then one contiguous piece whatever C is.
+// All four are bound by HBM traffic: 5.5 to 6.2 TB/s of the bytes above on 40 to 140 million values, where a copy reaches 5.1 to 5.4 (270000 x 512
+// fp32, us: pack 119, unpack 122, SiLU forward 213, backward 215; GELU 217 / 217), but for GELU in 16-bit types, which VALU work holds
+// (69633 x 1024 bf16: SiLU 62 / 62, GELU 66 / 74).
+// A lane holds 16 bytes of a row (4, 2 or 1 elements where the row length, the stride or an address is off), the 32 channels of a block are
+// 4 (16-bit types) or 8 (fp32) neighbouring lanes and their maximum is taken with DPP moves; a thread keeps its column and handles A8_U
+// rows, all loads first.  Dense rows of a multiple of 32 channels are walked as rows of 32: every access of a wave is then one contiguous
+// piece whatever C is.
 #include "act8.h"
 
 namespace {
 
-#ifndef A8_UU
-#define A8_UU 4
-#endif
-constexpr int A8_U = A8_UU;                                        // rows per thread: 64 bytes in flight per lane before the first use
+constexpr int A8_U = 2;                                        // rows per thread: with 4 the large shapes are 1 to 3 % slower, with 8 5 %
 
 struct A8Pos { int col; bool on; long long row0, step; };
 

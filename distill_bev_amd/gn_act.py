@@ -26,10 +26,11 @@ _STOCK = {"none": lambda t: t, "relu": F.relu, "silu": F.silu, "gelu": F.gelu}
 
 def _maps(x):
     """x [N, C, *] as a tensor whose memory is dense [N, *, C] (x itself if it is), and its pixels per image"""
-    N, C = x.shape[:2]
-    S = 1
-    for d in x.shape[2:]:
-        S *= d
+    N, C = x.shape[0], x.shape[1]
+    n = x.numel()
+    S = n // (N * C) if n else 0
+    if x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last):
+        return x, N, C, S
     t = x.movedim(1, -1)
     return (x if t.is_contiguous() else t.contiguous().movedim(-1, 1)), N, C, S
 
@@ -45,7 +46,7 @@ def _ptr(t):
 def _forward(x, N, C, S, G, weight, bias, eps, act, fmt, stats):
     """x dense channels-last -> y, f32 [2, N, G] of mean and rstd (None without `stats`), the checkpoint's buffer (None without `fmt`)"""
     dev = x.device
-    y = A.empty_dense(x.shape, 1, x.dtype, dev)
+    y = torch.empty_like(x)                                   # dense: x's own strides
     st = torch.empty((2, N, G), dtype=torch.float32, device=dev) if stats else None
     buf = A._buffer(N * S, C, dev) if fmt else None
     n = N * S * C

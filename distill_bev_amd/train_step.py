@@ -126,10 +126,10 @@ def parse_losses(losses):
     return sum(vals)
 
 
-def accelerate_modules(detector):
+def accelerate_modules(detector, activation_checkpoint=None):
     """Rewire parameter-free / parameter-preserving module pairs of a built, channels-last, on-GPU detector
-    (student + hidden teacher) onto the gfx950 kernels: BatchNorm2d->ReLU pairs (bn_act.fuse_bn_relu_modules),
-    bilinear align_corners nn.Upsample (UpsampleBilinearAC), NHWC teacher canvas.  State-dict keys are unchanged."""
+    (student + hidden teacher) onto the gfx950 kernels: BatchNorm2d->ReLU pairs (bn_act.fuse_bn_relu_modules), GroupNorm and
+    the activation behind it (gn_act.fuse_gn_act_modules), bilinear align_corners nn.Upsample (UpsampleBilinearAC), NHWC teacher canvas.  State-dict keys are unchanged."""
     from .bn_act import fuse_bn_relu_modules
     from .distill_loss import UpsampleBilinearAC
     from .skinny_conv import use_skinny_convs
@@ -152,6 +152,14 @@ def accelerate_modules(detector):
     detector.stem_convs = sum(use_stem_convs(r) for r in roots)        # the image backbone's 7x7 / stride-2 stem: fp32 MFMA kernel of its own
     from .colsum import use_bias_sum_convs
     detector.bias_sum_convs = sum(use_bias_sum_convs(r) for r in roots)   # remaining nn.Conv2d(bias=True): bias gradient as one streaming pass
+    from .gn_act import fuse_gn_act_modules
+    # `activation_checkpoint` ("int8" / "e4m3"): the student's group norms, linear layers, 1x1 convolutions and activations keep their
+    # inputs in 8 bits for the backward pass (the teacher runs without gradients and keeps nothing)
+    detector.fused_gn = sum(fuse_gn_act_modules(r, activation_checkpoint if r is detector else None) for r in roots)
+    detector.act8_modules = 0
+    if activation_checkpoint is not None:
+        from .act8 import use_act8
+        detector.act8_modules = use_act8(detector, activation_checkpoint)
     n_up = 0
     for r in roots:
         for mod in r.modules():
@@ -166,7 +174,7 @@ def accelerate_modules(detector):
     return n_bn, n_up
 
 
-def to_channels_last(detector):
+def to_channels_last(detector, activation_checkpoint=None):
     """Put a built, on-device detector (student + hidden teacher) into the layout bench.py times: channels-last weights of the dense
     2-D convolution modules, then `accelerate_modules`.  -> (fused norm+ReLU pairs, swapped upsample modules)"""
     # OIHW weights of the dense 2-D convolution modules only: Module.to(memory_format=) would also re-stride the sparse
@@ -177,7 +185,7 @@ def to_channels_last(detector):
             if isinstance(m, (nn.Conv2d, nn.ConvTranspose2d, ModulatedDeformConv2dPack)) and m.weight.dim() == 4:
                 m.weight.data = m.weight.data.contiguous(memory_format=torch.channels_last)
     detector.channels_last = True
-    return accelerate_modules(detector)
+    return accelerate_modules(detector, activation_checkpoint)
 
 
 def _flat_view(g):
@@ -413,7 +421,11 @@ def param_groups(detector, opt):
 
 
 class Trainer:
-    def __init__(self, model, cfg, device, world_size=1, channels_last=False):
+    def __init__(self, model, cfg, device, world_size=1, channels_last=False, activation_checkpoint=None):
+        """activation_checkpoint: None, "int8" or "e4m3" -- the form in which the rewired layers keep their inputs (act8.py); needs the
+        channels-last layout"""
+        if activation_checkpoint is not None and not channels_last:
+            raise ValueError("Trainer: activation_checkpoint needs channels_last=True")
         from .miopen_tuning import use_shipped_db
         use_shipped_db()                     # MIOpen solver tables tuned on MI355X; before the process's first convolution
         self.device = device
@@ -421,7 +433,7 @@ class Trainer:
         self.detector.train()
         self.packer = None
         if channels_last:
-            self.fused_bn_relu, self.swapped_upsample = to_channels_last(self.detector)
+            self.fused_bn_relu, self.swapped_upsample = to_channels_last(self.detector, activation_checkpoint)
             if device.type == "cuda":
                 from .packer import WeightPacker
                 self.packer = WeightPacker([self.detector])      # the trainable layers' packed weights: one launch per family and step

@@ -390,3 +390,30 @@ def test_large_batches_side_by_side_and_captured():
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(held, alone[i]))
         assert all(torch.equal(p, q) for p, q in zip(_run(*data[2 - i], 32, "silu", "int8"), alone[2 - i]))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_trainer_with_activation_checkpoints(fmt):
+    """the Trainer's option on a small detector: the first loss is the plain Trainer's, the gradients differ by the checkpoints' rounding only
+    -- relative error of a kept value at most 2^-6 (int8, of its block's largest) or 2^-4 (e4m3), independent signs: a few times 1e-2 at most
+    -- and parameters move"""
+    from test_host_act8 import _Toy
+    from distill_bev_amd.train_step import Trainer
+    x = torch.randn(4, 16, 20, 30, generator=torch.Generator().manual_seed(1)).to(DEV)
+
+    def one(option):
+        torch.manual_seed(11)
+        tr = Trainer(_Toy(), dict(), DEV, channels_last=True, activation_checkpoint=option)
+        loss = tr.step(dict(x=x))[0]
+        return tr, float(loss), [p.grad.detach().clone() for p in tr.detector.parameters()]
+
+    _, la, ga = one(None)
+    tr, lb, gb = one(fmt)
+    assert abs(la - lb) < 1e-5 * abs(la)
+    for (name, _), a, b in zip(tr.detector.named_parameters(), ga, gb):
+        if name != "neck.0.bias":                  # in front of a norm: what is left of a cancellation
+            assert float((a - b).norm() / a.norm()) < 0.05, name
+    before = [p.detach().clone() for p in tr.detector.parameters()]
+    tr.step(dict(x=x))
+    assert all(not torch.equal(p, q) for p, q in zip(before, tr.detector.parameters()))
+    tr.close()

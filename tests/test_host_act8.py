@@ -157,3 +157,37 @@ def test_modules_run_the_stock_operators_on_cpu_tensors():
     assert A.use_act8(ffn) == 4 and torch.allclose(ffn(t), ref, atol=1e-6)
     mha = nn.MultiheadAttention(8, 2)
     assert A.use_act8(mha) == 0
+
+
+class _Toy(nn.Module):
+    """a detector as Trainer sees one: a loss dictionary from forward_train"""
+
+    def __init__(self):
+        super().__init__()
+        self.neck = nn.Sequential(nn.Conv2d(16, 64, 1), nn.GroupNorm(8, 64), nn.SiLU(), nn.Conv2d(64, 64, 1, bias=False))
+        self.ffn = nn.Sequential(nn.Linear(64, 128), nn.ReLU(inplace=True), nn.Linear(128, 8))
+
+    def forward_train(self, x):
+        t = self.neck(x).flatten(2).transpose(1, 2)
+        return {"loss": self.ffn(t).square().mean()}
+
+
+def test_trainer_option_rewires_the_student_and_steps():
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    from distill_bev_amd.train_step import Trainer
+    torch.manual_seed(4)
+    x = torch.randn(2, 16, 6, 5)
+    ref = Trainer(_Toy(), dict(), torch.device("cpu"), channels_last=True)
+    assert ref.detector.fused_gn == 1 and ref.detector.act8_modules == 0
+    torch.manual_seed(4)
+    x2 = torch.randn(2, 16, 6, 5)
+    tr = Trainer(_Toy(), dict(), torch.device("cpu"), channels_last=True, activation_checkpoint="int8")
+    assert torch.equal(x, x2) and tr.detector.fused_gn == 1 and tr.detector.act8_modules == 4      # conv (bias-free), two linears, the ReLU
+    assert type(tr.detector.neck[1]) is GN.GroupNormAct and tr.detector.neck[1].act8_format == "int8"
+    assert isinstance(tr.detector.ffn[0], A.Act8Linear) and isinstance(tr.detector.ffn[1], A.Act8Activation)
+    assert torch.allclose(tr.step(dict(x=x))[0], ref.step(dict(x=x))[0], atol=1e-6)
+    with pytest.raises(ValueError):
+        Trainer(_Toy(), dict(), torch.device("cpu"), activation_checkpoint="int8")
+    with pytest.raises(ValueError):
+        Trainer(_Toy(), dict(), torch.device("cpu"), channels_last=True, activation_checkpoint="int4")

@@ -102,7 +102,7 @@ class LinearFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         xr, w = ctx.saved_tensors
-        return g @ w, g.t() @ xr, g.sum(0), None
+        return g @ w, g.t() @ xr, g.sum(0) if ctx.needs_input_grad[2] else None, None
 
 
 def group_norm(x, G, weight, bias, eps, name, fmt=None, gy=None):

@@ -317,7 +317,7 @@ def linear(x, weight, bias=None, checkpoint="int8"):
     """F.linear(x, weight, bias), differentiable; the 8-bit checkpoint of x is what the weight gradient is computed from"""
     _fmt(checkpoint)
     _check_layer(x, weight, bias, "linear")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] == 0:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
     with L.on(x.device):
         x2 = x.reshape(-1, weight.shape[1])
@@ -408,12 +408,16 @@ class Act8Linear(Bf6Linear):
         return super().extra_repr() + f", act8={self.act8_format}"
 
 
+def _plain_1x1(m):
+    return m.kernel_size == (1, 1) and m.stride == (1, 1) and m.padding == (0, 0) and m.dilation == (1, 1) and m.groups == 1
+
+
 class Act8Conv2d(Bf6Conv2d):
     """1x1, stride-1 nn.Conv2d that keeps its input as an 8-bit checkpoint while gradients of the weight are recorded"""
     act8_format = "int8"
 
     def forward(self, x):
-        if _recording(self.weight) and x.dim() == 4 and x.numel() and _module_ready(x, self.weight, self.bias):
+        if _recording(self.weight) and _plain_1x1(self) and x.dim() == 4 and x.numel() and _module_ready(x, self.weight, self.bias):
             return conv1x1(x, self.weight, self.bias, self.act8_format)
         return super().forward(x)
 
@@ -460,8 +464,7 @@ def use_act8(model, fmt="int8"):
         to = None
         if type(mod) in (nn.Linear, Bf6Linear):
             to = Act8Linear
-        elif type(mod) in (nn.Conv2d, Bf6Conv2d) and mod.kernel_size == (1, 1) and mod.stride == (1, 1) and mod.padding == (0, 0) \
-                and mod.dilation == (1, 1) and mod.groups == 1:
+        elif type(mod) in (nn.Conv2d, Bf6Conv2d) and _plain_1x1(mod):
             to = Act8Conv2d
         if to is not None:
             mod.__class__ = to

@@ -566,16 +566,28 @@ std::atomic<int> g_polls{10000};
 constexpr int GN_RF = 16;
 constexpr int gn_rb(int fmt) { return fmt == DBEV_ACT8_NONE ? 8 : 12; }
 
-// One pass where it is the faster way: rows wide enough to fill a workgroup, an image of 2 to 512 tiles (at most half of the 1024 that the chip
-// holds, so that another image's transfer covers one's wait), 2048 tiles or more in all: below, the two extra launches eat the gain
-// (8 x 128 x 128 x 128 fp32, 1024 tiles: forward 41 us against 57 of GPU time but two launches more for the host, backward 63 against 56).
+// CUs of the current device (a partition of the chip has fewer), 0 without one
+int gn_one_cus() {
+  static std::atomic<int> known[16];
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 0;
+  if (dev < 16 && (n = known[dev].load(std::memory_order_relaxed)) != 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
+  if (dev < 16) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// One pass where it is the faster way: rows wide enough to fill a workgroup, an image of 2 to 512 tiles and at most half of what the device
+// holds (four a CU), so that another image's transfer covers one's wait, and 2048 tiles or more in all: below, the two extra launches eat
+// the gain (8 x 128 x 128 x 128 fp32, 1024 tiles: forward 41 us against 57 of GPU time but two launches more for the host, backward 63
+// against 56).
 bool gn_one_plan(int dtype, int N, long long S, int C, int vec, int R, GnArgs* a, int* T) {
   const int wide = dtype == DBEV_DT_F32 ? 4 : 8;
   if (vec != wide) return false;
   a->t = a8_tile(C, wide);
   if (a->t.ncol != 1 || a->t.CH * a->t.RP < 192) return false;
   const long long rows = static_cast<long long>(a->t.RP) * R, tiles = (S + rows - 1) / rows;
-  if (tiles < 2 || tiles > 512 || tiles * N < 2048 || tiles * N > (1 << 22)) return false;
+  if (tiles < 2 || tiles > 512 || tiles * N < 2048 || tiles * N > (1 << 22) || tiles > 2LL * gn_one_cus()) return false;
   *T = static_cast<int>(tiles);
   return true;
 }

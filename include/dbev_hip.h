@@ -980,7 +980,7 @@ int dbev_act8_weight_gradient(const void* gy, int dtype, const uint8_t* codes, c
  *   variance, rstd = 1 / sqrt(var + eps); gamma / beta f32[C] or NULL (1 / 0).
  *   forward: mean, rstd f32[N, G] (both NULL at inference); fmt / codes / scales as above: x's checkpoint, written by the same pass.
  *   backward: x is read from codes / scales when fmt != DBEV_ACT8_NONE (then x may be NULL); dgamma, dbeta f32[C] (either may be NULL).
- *   Fixed summation order.  Workspace: dbev_gn_act_workspace_bytes (0: unsupported sizes).
+ *   Fixed summation order.  Workspace: dbev_gn_act_workspace_bytes (0: unsupported sizes), asked with the call's device current.
  * ---------------------------------------------------------------------------------- */
 size_t dbev_gn_act_workspace_bytes(int N, long long S, int C, int G);
 /* Large batches are done in one pass over the data, where workgroups wait -- a bounded number of looks -- for their image's sums and a further

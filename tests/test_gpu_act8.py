@@ -388,8 +388,8 @@ def test_other_streams_and_graph_replays():
     """on a stream of its own, and captured: forward, backward and weight gradient replayed on new inputs with eager work between"""
     from distill_bev_amd import act8 as A
     torch.manual_seed(4)
-    xs = [torch.randn(300, 96, device=DEV) for _ in range(4)]
-    gs = [torch.randn(300, 96, device=DEV) for _ in range(4)]
+    xs = [torch.randn(300, 256, device=DEV) for _ in range(4)]             # (256 channels: the largest tile, more than 64 KB of LDS)
+    gs = [torch.randn(300, 256, device=DEV) for _ in range(4)]
 
     def step(x, g):
         leaf = x.detach().requires_grad_(True)
@@ -421,3 +421,32 @@ def test_other_streams_and_graph_replays():
         assert all(torch.equal(a, b) for a, b in zip(held, eager[i]))
         again = step(xs[3 - i], gs[3 - i])
         assert all(torch.equal(a, b) for a, b in zip(again, eager[3 - i]))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_more_than_two_to_the_31_values(fmt):
+    """offsets beyond 32 bits: the last rows of a tensor of 2^31 + 2^20 values equal those of a call on them alone"""
+    from distill_bev_amd import act8 as A
+    rows, C = (1 << 25) + (1 << 14) + 3, 64
+    x = torch.empty((rows, C), dtype=torch.bfloat16, device=DEV)
+    x[:-1000].fill_(0.5)
+    x[-1000:] = _data(1000, C, torch.bfloat16, 1).to(DEV)
+    ck, tail = A.pack(x, fmt, -1), A.pack(x[-1000:], fmt, -1)
+    assert torch.equal(ck.codes[-1000:], tail.codes) and torch.equal(ck.scales[-1000:], tail.scales)
+    out = A.unpack(ck)
+    assert torch.equal(out[-1000:], A.unpack(tail)) and bool((out[:1000] == 0.5).all())
+    del out, ck
+    leaf = x.requires_grad_(True)
+    y = A.activation(leaf, "silu", fmt, -1)
+    gy = torch.ones((1, 1), dtype=torch.bfloat16, device=DEV).expand(rows, C).contiguous()
+    dx, = torch.autograd.grad(y, (leaf,), gy)
+    small = x[-1000:].detach().requires_grad_(True)
+    ys = A.activation(small, "silu", fmt, -1)
+    assert torch.equal(y[-1000:], ys) and torch.equal(dx[-1000:], torch.autograd.grad(ys, (small,), gy[-1000:])[0])
+    # the reduction over as many rows: ones against ones and the tail's own sums
+    ck = A.pack(x.detach(), fmt, -1)
+    g = torch.zeros((rows, 8), dtype=torch.bfloat16, device=DEV)
+    g[-1000:, :] = 1.0
+    gw, gb = A.weight_gradient(ck, g, bias=True)
+    ref = A.unpack(tail, torch.float32).double().sum(0)
+    assert float((gw.double() - ref).abs().max()) <= float(ref.abs().max()) * 2.0 ** -8 and bool((gb == 1000).all())

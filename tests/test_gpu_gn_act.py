@@ -301,6 +301,44 @@ def test_conv_module_with_group_norm_and_the_ledger():
     L.fallback_reset()
 
 
+def test_more_than_two_to_the_31_values_and_misaligned_addresses():
+    from distill_bev_amd import gn_act as GN
+    S, C, G = (1 << 25) + 77, 64, 4                                         # one image, 2^31 values and some, in 16 bits
+    x = torch.empty((1, S, C), dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for a in range(0, S, 1 << 22):
+        x[:, a:a + (1 << 22)] = torch.randn((1, min(1 << 22, S - a), C), generator=g, device=DEV)
+    w = torch.rand(C, device=DEV) + 0.5
+    y = GN.group_norm_act(x.permute(0, 2, 1), G, w, None, 1e-5, "silu").permute(0, 2, 1)
+    t = x.view(S, G, C // G)
+    mean, sq = torch.zeros(G, dtype=torch.float64, device=DEV), torch.zeros(G, dtype=torch.float64, device=DEV)
+    for a in range(0, S, 1 << 22):
+        d = t[a:a + (1 << 22)].double()
+        mean += d.sum((0, 2))
+        sq += d.square().sum((0, 2))
+    n = S * (C // G)
+    mean, rstd = mean / n, 1 / torch.sqrt(sq / n - (mean / n) ** 2 + 1e-5)
+    for sl in (slice(0, 1000), slice(S // 2, S // 2 + 1000), slice(S - 1000, S)):
+        z = ((t[sl].double() - mean[:, None]) * rstd[:, None]).reshape(-1, C) * w.double()
+        _close(y[0, sl], O.act(z, "silu")[0].cpu(), torch.bfloat16)
+    del x, y, t
+    for off in (1, 2, 3):                                                    # the same values at other addresses: the same bits
+        x, w, b, gy = _case(2, 60, 64, 8, torch.float32, 77)
+        flat, gflat = torch.zeros(2 * 60 * 64 + 4, device=DEV), torch.zeros(2 * 60 * 64 + 4, device=DEV)
+        flat[off:off + x.numel()], gflat[off:off + x.numel()] = x.view(-1).to(DEV), gy.view(-1).to(DEV)
+        at = lambda f: f[off:off + x.numel()].view(2, 6, 10, 64).permute(0, 3, 1, 2)      # noqa: E731
+        leaf = at(flat).requires_grad_(True)
+        y = GN.group_norm_act(leaf, 8, w.to(DEV), b.to(DEV), 1e-5, "gelu", "int8")
+        dx, = torch.autograd.grad(y, (leaf,), at(gflat))
+        ry, rdx, _, _, _ = O.group_norm(x.double(), 8, w.double(), b.double(), 1e-5, "gelu", "int8", gy.double())
+        _close(_rows(y), ry, torch.float32)
+        _close(_rows(dx), rdx, torch.float32, 2.0)
+    e = torch.empty((2, 32, 0, 5), device=DEV, requires_grad=True)           # images without pixels
+    wl = torch.ones(32, device=DEV, requires_grad=True)
+    GN.group_norm_act(e, 4, wl, None).sum().backward()
+    assert e.grad.shape == e.shape and torch.equal(wl.grad, torch.zeros_like(wl))
+
+
 # ---- batches that go through the one-pass kernels (csrc/gn_one.hip): 2048 register tiles or more, an image of 2 to 512 of them ----------
 ONE = [(260, 4200, 42, 64, 8), (24, 11440, 104, 256, 32), (66, 11000, 100, 80, 16), (31, 2111, 1, 1024, 512), (17, 20999, 1, 192, 3)]
 

@@ -77,6 +77,8 @@ def test_argument_checks_and_no_cpu_fallback_of_the_functions():
                  lambda: A.conv1x1(torch.randn(1, 8, 2, 2), torch.randn(4, 8, 1, 1)), lambda: GN.group_norm_act(x, 4)):
         with pytest.raises(L.DbevHipError):
             call()
+    c3 = A.Act8Conv2d(8, 4, 3, padding=1)                                # not a 1x1 layer: the stock convolution
+    assert c3(torch.randn(1, 8, 4, 4)).shape == (1, 4, 4, 4)
     with pytest.raises(ValueError):
         GN.gn_act(x, nn.GroupNorm(4, 32), "tanh")
     with pytest.raises(ValueError):

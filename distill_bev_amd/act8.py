@@ -18,8 +18,9 @@ Formats: with a = max |x| of a block of 32 channels and one power of two 2^k per
 int8 is the finer one for values that fill their block's range, e4m3 for blocks with outliers.  A block that holds an infinity or a NaN
 restores as NaN.  ReLU's derivative is taken at x^, where a positive value below half of the smallest code is zero.
 
-`use_act8(model, fmt)` swaps these layers into a built model; parameters and state-dict keys stay.  The functions above raise on what the kernels cannot take; the modules leave CPU and float64 tensors to the stock
-operators (device tensors are counted in the fallback ledger)."""
+`use_act8(model, fmt)` swaps these layers into a built model; parameters and state-dict keys stay.  The functions above raise on what the
+kernels cannot take (linear and conv1x1 under autocast too: they compute in their arguments' type); the modules leave CPU and float64 tensors
+and autocast to the stock operators (device tensors are counted in the fallback ledger)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -85,6 +86,8 @@ def rows_of(x, dim):
     rows = x.numel() // C if C else 0
     if C == 0 or rows == 0:
         return x, 0, C, C
+    if C > 1 << 30:
+        raise L.DbevHipError(f"act8: {C} channels, at most 2^30")
     if dim == x.dim() - 1 and x.is_contiguous():
         return x.view(rows, C), rows, C, C
     t = x.movedim(dim, -1)
@@ -218,11 +221,17 @@ def activation(x, act="gelu", checkpoint="int8", channel_dim=None):
     return _act_forward(x.detach(), act, None, dim)[0]
 
 
+def _gradient_ok(Ci, Co):
+    if Ci > 1 << 20 or Co > 1 << 20 or Ci * Co > 1 << 31:
+        raise L.DbevHipError(f"act8: weight gradient of {Ci} -> {Co} channels; at most 2^20 and 2^31 weights")
+
+
 def _weight_gradient(buf, fmt, Ci, gy2, bias):
     """checkpoint buffer of [M, Ci], gy2 [M, Co] dense -> (gw [Co, Ci], gb [Co] or None) in gy2's type"""
     dev = gy2.device
     M, Co = gy2.shape
     with L.on(dev):
+        _gradient_ok(Ci, Co)
         gw = torch.empty((Co, Ci), dtype=gy2.dtype, device=dev)
         gb = torch.empty((Co,), dtype=gy2.dtype, device=dev) if bias else None
         if Co and Ci:
@@ -262,6 +271,10 @@ def _check_layer(x, weight, bias, what):
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise L.DbevHipError(f"{what}: x, weight and bias of one type expected, got {x.dtype}, {weight.dtype}"
                              + ("" if bias is None else f", {bias.dtype}"))
+    if torch.is_autocast_enabled("cuda"):
+        raise L.DbevHipError(f"{what}: not under autocast (the products would be in another type than the arguments)")
+    if _recording(weight):
+        _gradient_ok(int(weight.shape[1]), int(weight.shape[0]))
     if bias is not None and bias.shape != (weight.shape[0],):
         raise ValueError(f"{what}: bias {tuple(bias.shape)} for {weight.shape[0]} outputs")
 
@@ -276,7 +289,7 @@ class _Linear8(Function):
     shape rule says so, else the library's), the weight and bias gradient come from the checkpoint of x2."""
 
     @staticmethod
-    def forward(ctx, x2, weight, bias, fmt):
+    def forward(ctx, x2, weight, bias, fmt, keep):
         from . import gemm_bf6 as G
         if G.eligible_linear(x2, weight):
             M, K = x2.shape
@@ -287,7 +300,7 @@ class _Linear8(Function):
                 y.add_(bias)
         else:
             y = F.linear(x2, weight, bias)
-        ck = pack(x2, fmt, -1) if ctx.needs_input_grad[1] else None
+        ck = pack(x2, fmt, -1) if keep else None
         ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt = fmt
         return y
@@ -310,19 +323,19 @@ class _Linear8(Function):
                 gw, gb = _weight_gradient(buf, ctx.fmt, int(weight.shape[1]), gy, ctx.needs_input_grad[2])
             elif ctx.needs_input_grad[2]:
                 gb = _bias_grad(gy)
-        return gx, gw, gb, None
+        return gx, gw, gb, None, None
 
 
 def linear(x, weight, bias=None, checkpoint="int8"):
     """F.linear(x, weight, bias), differentiable; the 8-bit checkpoint of x is what the weight gradient is computed from"""
     _fmt(checkpoint)
-    _check_layer(x, weight, bias, "linear")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] == 0:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
+    _check_layer(x, weight, bias, "linear")
     with L.on(x.device):
         x2 = x.reshape(-1, weight.shape[1])
         x2 = x2 if x2.is_contiguous() else x2.contiguous()
-        return _Linear8.apply(x2, weight, bias, checkpoint).view(*x.shape[:-1], weight.shape[0])
+        return _Linear8.apply(x2, weight, bias, checkpoint, _recording(weight)).view(*x.shape[:-1], weight.shape[0])
 
 
 class _Conv1x1_8(Function):
@@ -330,7 +343,7 @@ class _Conv1x1_8(Function):
     checkpoint of x"""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, fmt):
+    def forward(ctx, x, weight, bias, fmt, keep):
         from . import gemm_bf6 as G
         if G.eligible(x, weight):
             M = x.shape[0] * x.shape[2] * x.shape[3]
@@ -341,7 +354,7 @@ class _Conv1x1_8(Function):
                 y.add_(bias.view(1, -1, 1, 1))
         else:
             y = F.conv2d(x, weight, bias)
-        ck = pack(x, fmt, 1) if ctx.needs_input_grad[1] else None
+        ck = pack(x, fmt, 1) if keep else None
         ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt, ctx.x_shape = fmt, tuple(x.shape)
         return y
@@ -365,18 +378,18 @@ class _Conv1x1_8(Function):
                 gw = gw.view(weight.shape)                                # [Co, Ci] in memory: dense in both memory formats of a 1x1 filter
             elif ctx.needs_input_grad[2]:
                 gb = _bias_grad(gy2)
-        return gx, gw, gb, None
+        return gx, gw, gb, None, None
 
 
 def conv1x1(x, weight, bias=None, checkpoint="int8"):
     """F.conv2d(x, weight, bias) for a 1x1 filter, stride 1, differentiable; x is taken as (or copied to) a channels-last map and its 8-bit
     checkpoint is what the weight gradient is computed from"""
     _fmt(checkpoint)
-    _check_layer(x, weight, bias, "conv1x1")
     if weight.dim() != 4 or tuple(weight.shape[2:]) != (1, 1) or x.dim() != 4 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"conv1x1: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
+    _check_layer(x, weight, bias, "conv1x1")
     with L.on(x.device):
-        return _Conv1x1_8.apply(x.contiguous(memory_format=torch.channels_last), weight, bias, checkpoint)
+        return _Conv1x1_8.apply(x.contiguous(memory_format=torch.channels_last), weight, bias, checkpoint, _recording(weight))
 
 
 # ---- modules ------------------------------------------------------------------------------------------------------------------------

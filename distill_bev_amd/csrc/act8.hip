@@ -17,15 +17,18 @@ namespace {
 
 constexpr int A8_U = 2;                                        // rows per thread: with 4 the large shapes are 1 to 3 % slower, with 8 5 %
 
+constexpr int A8_GRID_Y = 1 << 16;                             // workgroups along y end here: beyond, the column ranges go along x, the rows along y
+
 struct A8Pos { int col; bool on; long long row0, step; };
 
 // column of this thread, its first row and the distance of its rows
 __device__ __forceinline__ A8Pos a8_pos(const A8Tile& t, int cv) {
   A8Pos p;
   const int rp = threadIdx.x / t.CH;
-  p.col = blockIdx.y * t.CH + (threadIdx.x - rp * t.CH);
+  const unsigned by = t.ncol < A8_GRID_Y ? blockIdx.x : blockIdx.y, bc = t.ncol < A8_GRID_Y ? blockIdx.y : blockIdx.x;
+  p.col = static_cast<int>(bc) * t.CH + (threadIdx.x - rp * t.CH);
   p.on = rp < t.RP && p.col < cv;
-  p.row0 = rp < t.RP ? static_cast<long long>(blockIdx.x) * (t.RP * A8_U) + rp : (1LL << 62);
+  p.row0 = rp < t.RP ? static_cast<long long>(by) * (t.RP * A8_U) + rp : (1LL << 62);
   p.step = t.RP;
   return p;
 }
@@ -111,7 +114,7 @@ A8Geo a8_geo(long long rows, int C, long long stride) {
 
 bool a8_shape_ok(int dtype, long long rows, int C, long long stride) {
   // (element offsets are 64-bit in the kernels)
-  return a8_dtype_ok(dtype) && rows >= 0 && C > 0 && stride >= C && C <= (1 << 24) && rows <= (1LL << 40) / C && stride <= (1LL << 40) / (rows + 1);
+  return a8_dtype_ok(dtype) && rows >= 0 && C > 0 && stride >= C && C <= (1 << 30) && rows <= (1LL << 40) / C && stride <= (1LL << 40) / (rows + 1);
 }
 
 long long a8_blocks(const A8Geo& g, const A8Tile& t) {
@@ -119,8 +122,14 @@ long long a8_blocks(const A8Geo& g, const A8Tile& t) {
   return (g.rows + per - 1) / per;
 }
 // a launch holds fewer than 2^32 threads along x (some 2^34 values or more, by vector width)
-bool a8_grid_ok(const A8Geo& g, const A8Tile& t) { return a8_blocks(g, t) * t.threads < (1LL << 32) && t.ncol < 65536; }
-dim3 a8_grid(const A8Geo& g, const A8Tile& t) { return dim3(static_cast<unsigned>(a8_blocks(g, t)), static_cast<unsigned>(t.ncol)); }
+bool a8_grid_ok(const A8Geo& g, const A8Tile& t) {
+  const long long b = a8_blocks(g, t);
+  return t.ncol < A8_GRID_Y ? b * t.threads < (1LL << 32) : b < A8_GRID_Y;
+}
+dim3 a8_grid(const A8Geo& g, const A8Tile& t) {
+  const unsigned b = static_cast<unsigned>(a8_blocks(g, t)), c = static_cast<unsigned>(t.ncol);
+  return t.ncol < A8_GRID_Y ? dim3(b, c) : dim3(c, b);
+}
 
 }  // namespace
 

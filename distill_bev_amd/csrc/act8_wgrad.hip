@@ -7,7 +7,7 @@
 // The reduction runs over m, the slow index of both operands, while a matrix instruction wants 8 consecutive m of one channel per lane:
 // a thread fetches 8 rows of a few channels (coalesced along the channels), so that a channel's 8 values sit in its registers and go to
 // LDS as one 16-byte unit [m / 8][channel]; the unit index is channel ^ ((channel >> 3) & 3), which spreads both the strided writes and
-// the reads over all banks.  Raw values come through buffer descriptors of the share's rows: a row or channel past the end reads as zero.
+// the reads over all banks.  Raw values come through buffer descriptors of the chunk's rows: a row or channel past the end reads as zero.
 //
 // Workgroup = 4 waves, tile TA output x TB input channels, chunks of 32 rows, two LDS buffers, one barrier a chunk.  The largest tile, 128 x 256,
 // has the register file to itself (one wave a SIMD): one tile of partial sums a CU.  A wave has two chunks of raw values in flight and splits
@@ -31,7 +31,7 @@ typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 #define A8W_SGB(mask_, n_) __builtin_amdgcn_sched_group_barrier((mask_), (n_), 0)
 constexpr int A8W_KC = 32;                                    // rows a chunk: two reduction steps of 16
-constexpr unsigned A8W_OOB = 0x80000000u;                     // offset of a channel past the end: beyond every descriptor (shares stay below 2 GiB)
+constexpr unsigned A8W_OOB = 0x80000000u;                     // offset of a channel past the end: beyond every descriptor (32 rows of 2^20 values at most)
 
 template <typename T> struct A8Pieces;
 template <> struct A8Pieces<float> { static constexpr int n = 3; };
@@ -42,9 +42,9 @@ __device__ __forceinline__ unsigned long long a8w_uniform(unsigned long long v) 
   const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v >> 32));
   return (static_cast<unsigned long long>(hi) << 32) | lo;
 }
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t a8w_rsrc(const void* p, long long bytes) {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t a8w_rsrc(const void* p, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(a8w_uniform(reinterpret_cast<unsigned long long>(p))), 0,
-                                           __builtin_amdgcn_readfirstlane(static_cast<int>(bytes < 0 ? 0 : bytes)), 0x00020000);
+                                           __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
 // upper halves of two dwords: (hi(b) << 16) | hi(a)
@@ -143,15 +143,15 @@ __global__ __launch_bounds__(256, TA * TB > 128 * 128 ? 1 : 2) void a8_wgrad(con
   for (int i = 0; i < CA; ++i) bsum[i] = 0.f;
 
   auto fetch_a = [&](Set& q, int ch) {                        // past the last row: empty descriptors, zeros
-    const long long r0 = static_cast<long long>(ch) * A8W_KC, left = nrows - r0;
-    const __amdgpu_buffer_rsrc_t gr = a8w_rsrc(gbase + r0 * Co, left * Co * static_cast<long long>(sizeof(T)));
+    const int r0 = ch * A8W_KC, left = max(0, min(A8W_KC, nrows - r0));
+    const __amdgpu_buffer_rsrc_t gr = a8w_rsrc(gbase + static_cast<long long>(r0) * Co, left * Co * static_cast<int>(sizeof(T)));
 #pragma unroll
     for (int k = 0; k < 8; ++k) q.a[k].load(gr, aoff[k]);
   };
   auto fetch_b = [&](Set& q, int ch) {
-    const long long r0 = static_cast<long long>(ch) * A8W_KC, left = nrows - r0;
-    const __amdgpu_buffer_rsrc_t cr = a8w_rsrc(cbase + r0 * Ci, left * Ci);
-    const __amdgpu_buffer_rsrc_t sr = a8w_rsrc(sbase + r0 * nb, left * nb);
+    const int r0 = ch * A8W_KC, left = max(0, min(A8W_KC, nrows - r0));
+    const __amdgpu_buffer_rsrc_t cr = a8w_rsrc(cbase + static_cast<long long>(r0) * Ci, left * Ci);
+    const __amdgpu_buffer_rsrc_t sr = a8w_rsrc(sbase + static_cast<long long>(r0) * nb, left * nb);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (VEC && CB == 4) q.b[k] = __builtin_amdgcn_raw_buffer_load_b32(cr, boff[k][0], 0, 0);
@@ -322,7 +322,10 @@ __global__ __launch_bounds__(256) void a8_wsum(const float* __restrict__ part, c
 struct A8WPlan { int ta, tb, tiles_n, tiles, rows_per, nsplit, grid; };
 
 bool a8w_plan(long long M, int Ci, int Co, A8WPlan* p) {
-  if (M < 0 || Ci <= 0 || Co <= 0 || Ci > 65536 || Co > 65536 || M > (1LL << 40) / (Ci > Co ? Ci : Co)) return false;
+  // up to 2^20 channels (a chunk's 32 rows are one descriptor) and 2^31 weights (a launch holds fewer than 2^32 threads)
+  if (M < 0 || Ci <= 0 || Co <= 0 || Ci > (1 << 20) || Co > (1 << 20) || static_cast<long long>(Ci) * Co > (1LL << 31) ||
+      M > (1LL << 40) / (Ci > Co ? Ci : Co))
+    return false;
   p->ta = Co > 64 ? 128 : 64;
   p->tb = Ci > 128 ? 256 : Ci > 64 ? 128 : 64;
   p->tiles_n = (Ci + p->tb - 1) / p->tb;
@@ -331,8 +334,7 @@ bool a8w_plan(long long M, int Ci, int Co, A8WPlan* p) {
   const long long most = (M + 127) / 128;                     // at least four chunks a share
   ns = ns > most ? most : ns;
   ns = ns < 1 ? 1 : ns;
-  // a share's rows are addressed with 31 bits of bytes
-  const long long cap = ((1LL << 31) - (1 << 20)) / (4LL * (Co > Ci ? Co : Ci)) / A8W_KC * A8W_KC;
+  constexpr long long cap = 1LL << 30;                        // rows of a share are counted in 32 bits
   long long rows = (M + ns - 1) / ns;
   rows = (rows + A8W_KC - 1) / A8W_KC * A8W_KC;
   if (rows > cap) rows = cap;

@@ -3,7 +3,8 @@
 //
 // Forward, two launches, no finalize launch between them:
 //   gn_stats   a workgroup owns a chunk of one image's pixels x a range of channels, a thread one vector column; sums of (x - K_c) and
-//              (x - K_c)^2 with K_c the chunk's first pixel: an offset of the data costs no digits.  Reduced to (mean, M2) per group
+//              (x - K_c)^2 with K_c the chunk's first pixel: an offset of the data costs no digits (and an outlier there, whose own
+//              square is in the sum, some rows * 2^-24 of it).  Reduced to (mean, M2) per group
 //              and chunk in LDS.
 //   gn_apply   every workgroup merges its image's chunk statistics itself -- a few KB from L2 against its share of x -- in fp64
 //              (M2 = sum of M2_i + n_i (mean_i - mean)^2), then y, and the checkpoint from the same registers.

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void gn_one_fill(ull* __restrict__ words, long
   if (i < nints) ints[i] = 0;
 }
 
-// An image is at most 256 tiles of 64 KB: addresses are a uniform image base + 32-bit offsets.  `nv`: rows of this thread inside the image.
+// An image is at most 512 tiles of 64 KB: addresses are a uniform image base + 32-bit offsets.  `nv`: rows of this thread inside the image.
 struct GnOnePos { int n, t, rp, lane, col, nv; bool on; unsigned at; };
 template <int V, int R>
 __device__ __forceinline__ GnOnePos gn_one_pos(const GnOneArgs& o, int tile) {

@@ -121,6 +121,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.shape != (C,) or t.dtype not in A.DTYPES):
             raise ValueError(f"group_norm_act: {name} {tuple(t.shape)} {t.dtype} for {C} channels")
+    if C > 1 << 16 or N > 1 << 22:
+        raise L.DbevHipError(f"group_norm_act: {N} images of {C} channels; at most 2^22 and 2^16")
     if not eps >= 0:
         raise ValueError(f"group_norm_act: eps {eps}")
     if x.numel() and x.numel() // G == 1:                         # F.group_norm's own refusal
@@ -177,11 +179,16 @@ class GroupNormAct(nn.GroupNorm):
 def fuse_gn_act_modules(model, checkpoint=None):
     """Rewire the nn.GroupNorm modules of nn.Sequential stacks and ConvModules onto the kernels, together with the ReLU / SiLU / GELU right
     behind them (replaced by nn.Identity; keys unchanged); other GroupNorm modules become GroupNormAct without an activation.
-    `checkpoint`: the format in which they keep their input, or None.  Returns how many norms changed.  Idempotent."""
+    A norm that several places share keeps the activations behind it as modules.  `checkpoint`: the format in which the norms keep their
+    input, or None.  Returns how many norms changed.  Idempotent."""
     from .registry import ConvModule
     if checkpoint is not None:
         A._fmt(checkpoint)
     n = 0
+    places = {}
+    for mod in model.modules():
+        for kid in mod._modules.values():
+            places[id(kid)] = places.get(id(kid), 0) + 1
 
     def take(norm, act):
         norm.__class__ = GroupNormAct
@@ -191,12 +198,12 @@ def fuse_gn_act_modules(model, checkpoint=None):
         if isinstance(mod, nn.Sequential):
             kids = list(mod._modules.items())
             for (_, a), (kb, b) in zip(kids, kids[1:]):
-                if type(a) is nn.GroupNorm and A.act_name(b):
+                if type(a) is nn.GroupNorm and places[id(a)] == 1 and A.act_name(b):
                     take(a, A.act_name(b))
                     mod._modules[kb] = nn.Identity()
                     n += 1
         elif isinstance(mod, ConvModule) and mod.with_norm and type(mod.norm) is nn.GroupNorm:
-            act = A.act_name(mod.activate) if mod.with_activation else None
+            act = A.act_name(mod.activate) if mod.with_activation and places[id(mod.norm)] == 1 else None
             take(mod.norm, act or "none")
             if act:
                 mod.activate = nn.Identity()

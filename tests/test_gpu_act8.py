@@ -450,3 +450,63 @@ def test_more_than_two_to_the_31_values(fmt):
     gw, gb = A.weight_gradient(ck, g, bias=True)
     ref = A.unpack(tail, torch.float32).double().sum(0)
     assert float((gw.double() - ref).abs().max()) <= float(ref.abs().max()) * 2.0 ** -8 and bool((gb == 1000).all())
+
+
+@pytest.mark.parametrize("M,Ci,Co", [(40, 8, 70001), (40, 70004, 6), (70, 66000, 3)])
+def test_weight_gradient_of_wide_layers(M, Ci, Co):
+    """rows of more than 2^16 values; whole numbers, so that every product and sum is exact"""
+    from distill_bev_amd import act8 as A
+    g = torch.Generator().manual_seed(5)
+    x = torch.randint(-60, 61, (M, Ci), generator=g).float()
+    x[:, ::32] = 64.0                                                      # every block's largest value: 2^k = 1
+    gy = torch.randint(-9, 10, (M, Co), generator=g).float()
+    gw, gb = A.weight_gradient(A.pack(x.to(DEV), "int8", -1), gy.to(DEV), bias=True)
+    assert torch.equal(gw.cpu(), gy.t() @ x) and torch.equal(gb.cpu(), gy.sum(0))
+
+
+@pytest.mark.parametrize("n", [(1 << 24) + 33, (1 << 24) + 64])
+def test_one_very_long_row(n):
+    """a flat tensor: the same blocks as its values in rows of 32 (odd length: single values a lane, more than 2^16 column ranges)"""
+    from distill_bev_amd import act8 as A
+    x = torch.randn(n, device=DEV, generator=torch.Generator(DEV).manual_seed(6))
+    ck, m = A.pack(x, "int8"), n // 32 * 32
+    rows = A.pack(x[:m].view(-1, 32), "int8", -1)
+    assert ck.rows == 1 and ck.C == n
+    assert torch.equal(ck.codes[0, :m], rows.codes.reshape(-1)) and torch.equal(ck.scales[0, :m // 32], rows.scales.reshape(-1))
+    back = A.unpack(ck)
+    assert torch.equal(back[:m], A.unpack(rows).reshape(-1))
+    if n > m:
+        tail = A.unpack(A.pack(x[m:].view(1, -1), "int8", -1)).reshape(-1)
+        assert torch.equal(back[m:], tail)
+    leaf = x.requires_grad_(True)
+    y = A.activation(leaf, "silu", "int8")
+    gy = torch.ones(n, device=DEV)
+    dx, = torch.autograd.grad(y, (leaf,), gy)
+    part = x[:m].detach().view(-1, 32).requires_grad_(True)
+    yp = A.activation(part, "silu", "int8", -1)
+    assert torch.equal(y[:m], yp.reshape(-1)) and torch.equal(dx[:m], torch.autograd.grad(yp, (part,), gy[:m].view(-1, 32))[0].reshape(-1))
+
+
+def test_layers_without_gradients_keep_nothing_and_refuse_autocast():
+    from distill_bev_amd import _lib as L
+    from distill_bev_amd import act8 as A
+    torch.manual_seed(7)
+    lin, conv = nn.Linear(64, 24).to(DEV), nn.Conv2d(64, 24, 1).to(DEV)
+    x, m = torch.randn(50, 64, device=DEV), torch.randn(2, 64, 5, 5, device=DEV).contiguous(memory_format=torch.channels_last)
+    packs = []
+    pack, A.pack = A.pack, lambda *a: packs.append(a) or pack(*a)
+    try:
+        with torch.no_grad():
+            y, z = A.linear(x, lin.weight, lin.bias), A.conv1x1(m, conv.weight, conv.bias)
+        assert not packs and not y.requires_grad and not z.requires_grad
+        assert torch.equal(y, A.linear(x, lin.weight, lin.bias)) and torch.equal(z, A.conv1x1(m, conv.weight, conv.bias)) and len(packs) == 2
+    finally:
+        A.pack = pack
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        with pytest.raises(L.DbevHipError):
+            A.linear(x, lin.weight, lin.bias)
+        with pytest.raises(L.DbevHipError):
+            A.conv1x1(m, conv.weight, conv.bias)
+    wide = torch.empty((1, 8), device=DEV).expand((1 << 20) + 1, 8).requires_grad_(True)
+    with pytest.raises(L.DbevHipError):                                    # before the product, not in the backward pass
+        A.linear(x[:, :8], wide)

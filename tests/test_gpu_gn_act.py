@@ -455,3 +455,26 @@ def test_trainer_with_activation_checkpoints(fmt):
     tr.step(dict(x=x))
     assert all(not torch.equal(p, q) for p, q in zip(before, tr.detector.parameters()))
     tr.close()
+
+
+def test_a_chunk_that_begins_with_an_outlier():
+    """The squares are taken about a chunk's first pixel; an outlier D there makes every term D^2.  n = 250 rows a chunk, chains of at most 40
+    additions: the second moment is off by at most 40 * 250 * 2^-24 D^2, and the outlier itself gives it D^2: 6e-4 of the variance, 3e-4 of y - b.
+    The chunk's mean is K + (sum of x - K) / n, sums of terms of size D: off by at most 40 * 2^-24 D in one of eight chunks, i.e. by 5 * 2^-24 D
+    in all, where a spread is at least D / sqrt(2000): 5 * 2^-24 * 44.7 = 1.34e-5 <= 2^-16 spreads, times |w| in y"""
+    from distill_bev_amd import gn_act as GN
+    x, w, b, _ = _case(1, 2000, 8, 2, torch.float32, 9)
+    x[0, 0] = 1e4
+    y = GN.group_norm_act(_maps(x, 40), 2, w.to(DEV), b.to(DEV), 1e-5)
+    ref = F.group_norm(x.double().movedim(1, 2), 2, w.double(), b.double(), 1e-5).movedim(1, 2)
+    d = (_rows(y) - ref).abs()
+    assert bool((d <= 2.0 ** -11 * (ref - b.double()).abs() + 2.0 ** -16 * w.double().abs() + 2.0 ** -22 * (1 + ref.abs())).all()), float(d.max())
+
+
+def test_sizes_beyond_the_limits_are_refused():
+    from distill_bev_amd import _lib as L
+    from distill_bev_amd import gn_act as GN
+    with pytest.raises(L.DbevHipError):
+        GN.group_norm_act(torch.empty((1, 1 << 17), device=DEV), 4)
+    with pytest.raises(L.DbevHipError):
+        GN.group_norm_act(torch.empty((1, 8), device=DEV).expand((1 << 22) + 1, 8), 4)

@@ -161,6 +161,33 @@ def test_modules_run_the_stock_operators_on_cpu_tensors():
     assert A.use_act8(mha) == 0
 
 
+def test_a_shared_group_norm_keeps_the_activations_behind_it():
+    """one norm used in two places: with the activation of one of them inside, the other would be wrong"""
+    from distill_bev_amd import gn_act as GN
+    torch.manual_seed(3)
+    gn = nn.GroupNorm(2, 8)
+    net = nn.Sequential(gn, nn.ReLU(), nn.Conv2d(8, 8, 1), gn, nn.SiLU())
+    x = torch.randn(2, 8, 3, 3)
+    ref = net(x)
+    assert GN.fuse_gn_act_modules(net) == 1 and type(gn) is GN.GroupNormAct and gn.act == "none"
+    assert torch.allclose(net(x), ref, atol=1e-6)
+
+
+def test_sizes_at_and_beyond_the_limits():
+    from distill_bev_amd import _lib as L
+    from distill_bev_amd import act8 as A
+    h = L.lib()
+    one = ctypes.c_void_p(16)
+    size = h.dbev_act8_weight_gradient_workspace_bytes
+    assert size(40, 8, 1 << 20) > 0 and size(40, 1 << 20, 2048) > 0 and size(100000, 1024, 151936) > 0
+    assert size(40, 1 << 20, 2049) == 0 and size(40, 8, (1 << 20) + 1) == 0
+    assert h.dbev_act8_pack(one, 0, 1, (1 << 30) + 1, (1 << 30) + 1, 1, one, one, None) == 10001
+    with pytest.raises(L.DbevHipError):                                   # (a C int of the library)
+        A.rows_of(torch.empty(1).expand(1, (1 << 30) + 1), 1)
+    with pytest.raises(L.DbevHipError):
+        A._gradient_ok((1 << 32) + 8, 4)
+
+
 class _Toy(nn.Module):
     """a detector as Trainer sees one: a loss dictionary from forward_train"""
 

@@ -22,7 +22,11 @@ struct A8Vec {
   typedef T vec __attribute__((ext_vector_type(V)));
   typedef float fvec __attribute__((ext_vector_type(V)));
   typedef vec Raw;
-  static __device__ __forceinline__ Raw load(const T* p) { return *reinterpret_cast<const vec*>(p); }
+  // NT: without keeping the line in the caches (a8_nt)
+  template <bool NT = false>
+  static __device__ __forceinline__ Raw load(const T* p) {
+    return NT ? __builtin_nontemporal_load(reinterpret_cast<const vec*>(p)) : *reinterpret_cast<const vec*>(p);
+  }
   static __device__ __forceinline__ void get(const Raw& t, float* v) {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = static_cast<float>(t[i]);
@@ -33,19 +37,23 @@ struct A8Vec {
     for (int i = 0; i < V; ++i) t[i] = static_cast<T>(0.f);
     return t;
   }
+  template <bool NT = false>
   static __device__ __forceinline__ void store(T* p, const float* v) {
     fvec f;
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = v[i];
-    *reinterpret_cast<vec*>(p) = __builtin_convertvector(f, vec);
+    if (NT) __builtin_nontemporal_store(__builtin_convertvector(f, vec), reinterpret_cast<vec*>(p));
+    else *reinterpret_cast<vec*>(p) = __builtin_convertvector(f, vec);
   }
 };
 template <typename T>
 struct A8Vec<T, 1> {
   typedef T Raw;
+  template <bool NT = false>
   static __device__ __forceinline__ Raw load(const T* p) { return *p; }
   static __device__ __forceinline__ void get(const Raw& t, float* v) { v[0] = static_cast<float>(t); }
   static __device__ __forceinline__ Raw zero() { return static_cast<T>(0.f); }
+  template <bool NT = false>
   static __device__ __forceinline__ void store(T* p, const float* v) { *p = static_cast<T>(v[0]); }
 };
 
@@ -207,6 +215,14 @@ static inline int a8_pick_vec(int esize, long long c, long long stride, const vo
     if (v <= wide && c % v == 0 && stride % v == 0 && a % (static_cast<uintptr_t>(v) * esize) == 0) return v;
   return 1;
 }
+
+// Tensors of more than 192 MB go past the memory-side cache (256 MB), which they would only wash out: with an operator that writes x before and
+// one that reads y behind, fp32 SiLU with an int8 checkpoint, us kept / past: 81 MB 76 / 82, 163 MB 160 / 152 (backward 157 / 161), 266 MB
+// 291 / 246 (292 / 257), 552 MB 603 / 558 (598 / 566).  16-byte accesses only.
+static inline bool a8_nt(long long bytes) { return bytes > (192LL << 20); }
+#define A8_NT_SWITCH(bytes_, ...)                                                        \
+  if (V * sizeof(T) == 16 && a8_nt(bytes_)) { constexpr bool NT = V * sizeof(T) == 16; __VA_ARGS__; } \
+  else { constexpr bool NT = false; __VA_ARGS__; }
 
 #define A8_ACT_SWITCH(act_, ...)                                             \
   switch (act_) {                                                            \

@@ -4,9 +4,9 @@
 //   a8_unpack    codes, scales -> x^                       the reverse
 //   a8_act_fwd   y = act(x), and x's checkpoint            reads n * es, writes n * es + 1.03 n: the checkpoint costs no pass of its own
 //   a8_act_bwd   dx = dy * act'(x^)                        reads n * es + 1.03 n, writes n * es
-// All four are bound by HBM traffic: 5.5 to 6.2 TB/s of the bytes above on 40 to 140 million values, where a copy reaches 5.1 to 5.4 (270000 x 512
-// fp32, us: pack 119, unpack 122, SiLU forward 213, backward 215; GELU 217 / 217), but for GELU in 16-bit types, which VALU work holds
-// (69633 x 1024 bf16: SiLU 62 / 62, GELU 66 / 74).
+// All four are bound by HBM traffic: 5.7 to 7.3 TB/s of the bytes above on 70 to 280 million values, where a copy reaches 5.1 to 5.4 (270000 x 512
+// fp32, us: pack 107, unpack 96, SiLU forward 183, backward 186; GELU 185 / 203), but for GELU in 16-bit types, which VALU work holds
+// (69633 x 1024 bf16: SiLU 65 / 66, GELU 65 / 78; 540000 x 512: 226 / 222, 240 / 264).
 // A lane holds 16 bytes of a row (4, 2 or 1 elements where the row length, the stride or an address is off), the 32 channels of a block are
 // 4 (16-bit types) or 8 (fp32) neighbouring lanes and their maximum is taken with DPP moves; a thread keeps its column and handles A8_U
 // rows, all loads first.  Dense rows of a multiple of 32 channels are walked as rows of 32: every access of a wave is then one contiguous
@@ -33,7 +33,7 @@ __device__ __forceinline__ A8Pos a8_pos(const A8Tile& t, int cv) {
   return p;
 }
 
-template <typename T, int V, int FMT, int ACT, bool WITH_Y>
+template <typename T, int V, int FMT, int ACT, bool WITH_Y, bool NT>
 __global__ __launch_bounds__(256) void a8_forward(const T* __restrict__ x, long long xs, long long rows, int cv, int nb, A8Tile t, T* __restrict__ y,
                                                   uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   constexpr int LB = 32 / V;
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void a8_forward(const T* __restrict__ x, long 
 #pragma unroll
   for (int u = 0; u < A8_U; ++u) {
     const long long r = p.row0 + u * p.step;
-    raw[u] = p.on && r < rows ? A8Vec<T, V>::load(x + r * xs + static_cast<long long>(p.col) * V) : A8Vec<T, V>::zero();
+    raw[u] = p.on && r < rows ? A8Vec<T, V>::template load<NT>(x + r * xs + static_cast<long long>(p.col) * V) : A8Vec<T, V>::zero();
   }
 #pragma unroll
   for (int u = 0; u < A8_U; ++u) {
@@ -64,13 +64,13 @@ __global__ __launch_bounds__(256) void a8_forward(const T* __restrict__ x, long 
     if (WITH_Y && p.on) {
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = a8_act<ACT, T>(v[i]);
-      A8Vec<T, V>::store(y + o, v);
+      A8Vec<T, V>::template store<NT>(y + o, v);
     }
   }
 }
 
 // out = x^ (ACT none, gy null) or gy * act'(x^)
-template <typename T, int V, int FMT, int ACT, bool WITH_GY>
+template <typename T, int V, int FMT, int ACT, bool WITH_GY, bool NT>
 __global__ __launch_bounds__(256) void a8_backward(const T* __restrict__ gy, long long gs, const uint8_t* __restrict__ codes,
                                                    const uint8_t* __restrict__ scales, long long rows, int cv, int nb, A8Tile t, T* __restrict__ out) {
   constexpr int LB = 32 / V;
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void a8_backward(const T* __restrict__ gy, lon
     if (r < rows) {
       c[u] = *reinterpret_cast<const typename A8Bytes<V>::type*>(codes + (r * cv + p.col) * V);
       b[u] = scales[r * nb + p.col / LB];
-      if (WITH_GY) graw[u] = A8Vec<T, V>::load(gy + r * gs + static_cast<long long>(p.col) * V);
+      if (WITH_GY) graw[u] = A8Vec<T, V>::template load<NT>(gy + r * gs + static_cast<long long>(p.col) * V);
     }
   }
 #pragma unroll
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256) void a8_backward(const T* __restrict__ gy, lon
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = a8_act_grad<ACT>(g[i], v[i]);
     }
-    A8Vec<T, V>::store(out + (r * cv + p.col) * V, v);
+    A8Vec<T, V>::template store<NT>(out + (r * cv + p.col) * V, v);
   }
 }
 
@@ -126,6 +126,7 @@ bool a8_grid_ok(const A8Geo& g, const A8Tile& t) {
   const long long b = a8_blocks(g, t);
   return t.ncol < A8_GRID_Y ? b * t.threads < (1LL << 32) : b < A8_GRID_Y;
 }
+long long a8_bytes(const A8Geo& g, size_t esize) { return g.rows * g.C * static_cast<long long>(esize); }
 dim3 a8_grid(const A8Geo& g, const A8Tile& t) {
   const unsigned b = static_cast<unsigned>(a8_blocks(g, t)), c = static_cast<unsigned>(t.ncol);
   return t.ncol < A8_GRID_Y ? dim3(b, c) : dim3(c, b);
@@ -142,12 +143,14 @@ extern "C" int dbev_act8_pack(const void* x, int dtype, long long rows, int C, l
   A8_TYPE_SWITCH(dtype, vec, {
     const A8Tile t = a8_tile(g.C, V);
     if (reinterpret_cast<uintptr_t>(codes) % V != 0 || !a8_grid_ok(g, t)) return DBEV_EINVAL;
-    if (fmt == DBEV_ACT8_INT8)
-      hipLaunchKernelGGL((a8_forward<T, V, DBEV_ACT8_INT8, DBEV_ACT_NONE, false>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
-                         static_cast<const T*>(x), g.stride, g.rows, g.C / V, g.nb, t, nullptr, codes, scales);
-    else
-      hipLaunchKernelGGL((a8_forward<T, V, DBEV_ACT8_E4M3, DBEV_ACT_NONE, false>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
-                         static_cast<const T*>(x), g.stride, g.rows, g.C / V, g.nb, t, nullptr, codes, scales);
+    A8_NT_SWITCH(a8_bytes(g, sizeof(T)), {
+      if (fmt == DBEV_ACT8_INT8)
+        hipLaunchKernelGGL((a8_forward<T, V, DBEV_ACT8_INT8, DBEV_ACT_NONE, false, NT>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
+                           static_cast<const T*>(x), g.stride, g.rows, g.C / V, g.nb, t, nullptr, codes, scales);
+      else
+        hipLaunchKernelGGL((a8_forward<T, V, DBEV_ACT8_E4M3, DBEV_ACT_NONE, false, NT>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
+                           static_cast<const T*>(x), g.stride, g.rows, g.C / V, g.nb, t, nullptr, codes, scales);
+    });
   });
   DBEV_LAUNCH_CHECK();
   return 0;
@@ -161,12 +164,14 @@ extern "C" int dbev_act8_unpack(const uint8_t* codes, const uint8_t* scales, int
   A8_TYPE_SWITCH(dtype, vec, {
     const A8Tile t = a8_tile(g.C, V);
     if (reinterpret_cast<uintptr_t>(codes) % V != 0 || !a8_grid_ok(g, t)) return DBEV_EINVAL;
-    if (fmt == DBEV_ACT8_INT8)
-      hipLaunchKernelGGL((a8_backward<T, V, DBEV_ACT8_INT8, DBEV_ACT_NONE, false>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
-                         nullptr, g.stride, codes, scales, g.rows, g.C / V, g.nb, t, static_cast<T*>(out));
-    else
-      hipLaunchKernelGGL((a8_backward<T, V, DBEV_ACT8_E4M3, DBEV_ACT_NONE, false>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
-                         nullptr, g.stride, codes, scales, g.rows, g.C / V, g.nb, t, static_cast<T*>(out));
+    A8_NT_SWITCH(a8_bytes(g, sizeof(T)), {
+      if (fmt == DBEV_ACT8_INT8)
+        hipLaunchKernelGGL((a8_backward<T, V, DBEV_ACT8_INT8, DBEV_ACT_NONE, false, NT>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
+                           nullptr, g.stride, codes, scales, g.rows, g.C / V, g.nb, t, static_cast<T*>(out));
+      else
+        hipLaunchKernelGGL((a8_backward<T, V, DBEV_ACT8_E4M3, DBEV_ACT_NONE, false, NT>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
+                           nullptr, g.stride, codes, scales, g.rows, g.C / V, g.nb, t, static_cast<T*>(out));
+    });
   });
   DBEV_LAUNCH_CHECK();
   return 0;
@@ -181,9 +186,10 @@ extern "C" int dbev_act8_activation_forward(const void* x, int dtype, long long 
   A8_TYPE_SWITCH(dtype, vec, {
     const A8Tile t = a8_tile(g.C, V);
     if ((fmt != DBEV_ACT8_NONE && reinterpret_cast<uintptr_t>(codes) % V != 0) || !a8_grid_ok(g, t)) return DBEV_EINVAL;
-    A8_ACT_SWITCH(act, A8_FMT_SWITCH(fmt, hipLaunchKernelGGL((a8_forward<T, V, FMT, ACT, true>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
-                                                             static_cast<const T*>(x), g.stride, g.rows, g.C / V, g.nb, t, static_cast<T*>(y),
-                                                             codes, scales)));
+    A8_NT_SWITCH(a8_bytes(g, sizeof(T)), A8_ACT_SWITCH(act, A8_FMT_SWITCH(fmt, {
+      hipLaunchKernelGGL((a8_forward<T, V, FMT, ACT, true, NT>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream), static_cast<const T*>(x),
+                         g.stride, g.rows, g.C / V, g.nb, t, static_cast<T*>(y), codes, scales);
+    })));
   });
   DBEV_LAUNCH_CHECK();
   return 0;
@@ -198,13 +204,14 @@ extern "C" int dbev_act8_activation_backward(const void* gy, int dtype, long lon
   A8_TYPE_SWITCH(dtype, vec, {
     const A8Tile t = a8_tile(g.C, V);
     if (reinterpret_cast<uintptr_t>(codes) % V != 0 || !a8_grid_ok(g, t)) return DBEV_EINVAL;
-    if (fmt == DBEV_ACT8_INT8) {
-      A8_ACT_SWITCH(act, hipLaunchKernelGGL((a8_backward<T, V, DBEV_ACT8_INT8, ACT, true>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
-                                            static_cast<const T*>(gy), g.stride, codes, scales, g.rows, g.C / V, g.nb, t, static_cast<T*>(dx)));
-    } else {
-      A8_ACT_SWITCH(act, hipLaunchKernelGGL((a8_backward<T, V, DBEV_ACT8_E4M3, ACT, true>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
-                                            static_cast<const T*>(gy), g.stride, codes, scales, g.rows, g.C / V, g.nb, t, static_cast<T*>(dx)));
-    }
+    A8_NT_SWITCH(a8_bytes(g, sizeof(T)), A8_ACT_SWITCH(act, {
+      if (fmt == DBEV_ACT8_INT8)
+        hipLaunchKernelGGL((a8_backward<T, V, DBEV_ACT8_INT8, ACT, true, NT>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
+                           static_cast<const T*>(gy), g.stride, codes, scales, g.rows, g.C / V, g.nb, t, static_cast<T*>(dx));
+      else
+        hipLaunchKernelGGL((a8_backward<T, V, DBEV_ACT8_E4M3, ACT, true, NT>), a8_grid(g, t), dim3(t.threads), 0, dbev_stream(stream),
+                           static_cast<const T*>(gy), g.stride, codes, scales, g.rows, g.C / V, g.nb, t, static_cast<T*>(dx));
+    }));
   });
   DBEV_LAUNCH_CHECK();
   return 0;

@@ -87,8 +87,9 @@ struct GnX {
   typename A8Bytes<V>::type c;
   unsigned b;
   typename A8Vec<T, V>::Raw v;
+  template <bool NT = false>
   __device__ __forceinline__ void load(const T* x, const uint8_t* codes, const uint8_t* scales, size_t row, int C, int nb, int col) {
-    if (FMT == DBEV_ACT8_NONE) v = A8Vec<T, V>::load(x + row * C + static_cast<size_t>(col) * V);
+    if (FMT == DBEV_ACT8_NONE) v = A8Vec<T, V>::template load<NT>(x + row * C + static_cast<size_t>(col) * V);
     else {
       c = *reinterpret_cast<const typename A8Bytes<V>::type*>(codes + row * C + static_cast<size_t>(col) * V);
       b = scales[row * nb + col / (32 / V)];

@@ -13,6 +13,9 @@
 //   gn_bwd_dx       dx = rstd (gamma g - A / D - xh B / D), D = S C / G; its first workgroups add the per-channel rows up instead
 // Bound by HBM: 3 n es forward and 5 n es backward (n es = bytes of x; with a checkpoint the two reads of x in the backward are 1.03
 // bytes a value).  All sums have a fixed order: run-to-run bit-identical, no atomics.
+// Measured, fp32, SiLU: 1 x 128 x 1024 x 1024 forward 280 us (1.6 GB in three passes: 5.8 TB/s, part of the second read comes from the
+// memory-side cache), backward 446; 8 x 128 x 128 x 128, int8 kept: 28 + 28 and 24 + 27 us, half of it cache; 6 x 256 x 15 x 25: 7 + 7 and 7 + 7 us,
+// launch and merge latency.
 #include "gn_act.h"
 #include "gn_one.h"
 
@@ -128,13 +131,13 @@ __device__ __forceinline__ float* gn_gather(float* sh, const GnArgs& a, const Gn
   return out;
 }
 
-template <typename T, int V, int FMT, int ACT>
+template <typename T, int V, int FMT, int ACT, bool NT>
 __global__ __launch_bounds__(256) void gn_apply(const T* __restrict__ x, GnArgs a, const float2* __restrict__ part, const float* __restrict__ gamma,
                                                 const float* __restrict__ beta, float eps, T* __restrict__ y, float* __restrict__ mean,
                                                 float* __restrict__ rstd, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   extern __shared__ float sh[];
   constexpr int LB = 32 / V;
-  const GnPos p = gn_pos(a, blockIdx.x, V);
+  const GnPos p = gn_pos(a, gridDim.x - 1 - blockIdx.x, V);
   const float* st = gn_gather<true>(sh, a, p, V, part, eps);
   if (mean != nullptr && p.chunk == 0)
     for (int gi = threadIdx.x; gi < p.g1 - p.g0; gi += blockDim.x)
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(256) void gn_apply(const T* __restrict__ x, GnArgs 
 #pragma unroll
     for (int u = 0; u < GN_U; ++u) {
       const long long ru = r + u * a.t.RP;
-      raw[u] = p.on && ru < a.S ? A8Vec<T, V>::load(x + (base + ru) * a.C + static_cast<size_t>(p.col) * V) : A8Vec<T, V>::zero();
+      raw[u] = p.on && ru < a.S ? A8Vec<T, V>::template load<NT>(x + (base + ru) * a.C + static_cast<size_t>(p.col) * V) : A8Vec<T, V>::zero();
     }
 #pragma unroll
     for (int u = 0; u < GN_U; ++u) {
@@ -178,7 +181,7 @@ __global__ __launch_bounds__(256) void gn_apply(const T* __restrict__ x, GnArgs 
       if (p.on) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = a8_act<ACT, T>(fmaf(v[i], sc[i], bt[i]));
-        A8Vec<T, V>::store(y + o, v);
+        A8Vec<T, V>::template store<NT>(y + o, v);
       }
     }
   }
@@ -280,7 +283,7 @@ __device__ __forceinline__ void gn_param_grads(double* sh, const GnArgs& a, long
   }
 }
 
-template <typename T, int V, int FMT, int ACT>
+template <typename T, int V, int FMT, int ACT, bool NT>
 __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const T* __restrict__ x, const uint8_t* __restrict__ codes,
                                                  const uint8_t* __restrict__ scales, GnArgs a, GnCoef k, const float2* __restrict__ pc,
                                                  const float2* __restrict__ pg, int N, int npar, T* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta) {
@@ -289,7 +292,7 @@ __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const
     gn_param_grads(reinterpret_cast<double*>(sh), a, static_cast<long long>(N) * a.nchunk, blockIdx.x, pc, dgamma, dbeta);
     return;
   }
-  const GnPos p = gn_pos(a, static_cast<int>(blockIdx.x) - npar, V);
+  const GnPos p = gn_pos(a, static_cast<int>(gridDim.x - 1 - blockIdx.x), V);
   const float* ab = gn_gather<false>(sh, a, p, V, pg, 0.f);
   if (!p.on) return;
   float mu[V], sc[V], bt[V], A[V], B[V];                     // dx = sc g - (rstd A) - (x - mean) (rstd^2 B), sc = rstd gamma
@@ -311,8 +314,8 @@ __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const
     for (int u = 0; u < GN_U; ++u) {
       const long long ru = r + u * a.t.RP;
       if (ru < a.S) {
-        draw[u] = A8Vec<T, V>::load(gy + (base + ru) * a.C + static_cast<size_t>(p.col) * V);
-        xv[u].load(x, codes, scales, base + ru, a.C, a.nb, p.col);
+        draw[u] = A8Vec<T, V>::template load<NT>(gy + (base + ru) * a.C + static_cast<size_t>(p.col) * V);
+        xv[u].template load<NT>(x, codes, scales, base + ru, a.C, a.nb, p.col);
       }
     }
 #pragma unroll
@@ -328,17 +331,23 @@ __global__ __launch_bounds__(256) void gn_bwd_dx(const T* __restrict__ gy, const
         const float g = a8_act_grad<ACT>(d[i], fmaf(dev, sc[i], bt[i]));
         v[i] = fmaf(sc[i], g, -fmaf(dev, B[i], A[i]));
       }
-      A8Vec<T, V>::store(dx + (base + ru) * a.C + static_cast<size_t>(p.col) * V, v);
+      A8Vec<T, V>::template store<NT>(dx + (base + ru) * a.C + static_cast<size_t>(p.col) * V, v);
     }
   }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
-// chunks per image: enough workgroups for sixteen per CU over the whole batch (twice what fits: 813 -> 776 us at 48 x 256 x 64 x 176 fp32 against
-// eight), at least two tiles each, at most 128 (every workgroup of the second launch merges its image's chunk rows).  Taking the batch in
-// slices that fit the 256 MB memory-side cache, so that the second launch would find its data there, was slower at every slice size
-// (96 MB: 894 us against 823): a launch's ramp and its merge cost more than the cache gives.
-GnArgs gn_args(int N, long long S, int C, int G, int V) {
+// Chunks per image: enough workgroups for sixteen per CU over the whole batch (twice what fits: 813 -> 776 us at 48 x 256 x 64 x 176 fp32 against
+// eight), at least two tiles each, at most 128: every workgroup of the second launch reads its image's chunk rows, 8 G bytes a chunk.  Where
+// 128 would leave fewer than four workgroups a CU, as many as make up for it, but no more than keep those rows below the chunk's own bytes.
+// With at most 128 / 256 / 512 / 1024 chunks, fp32, SiLU, forward, us: one image of 256 channels, 256 x 256: 102 / 61 / 49 / 54; four: 166 /
+// 138 / 136 / 174; one of 128 channels, 1024 x 1024: 994 / 560 / 366 / 292; eight of 128 channels, 128 x 128: 44 with 128, 47 with 181.  Taking
+// the batch in slices that fit the 256 MB memory-side cache, so that the second launch would find its data there, was slower at every slice
+// size (96 MB: 894 us against 823): a launch's ramp and its merge cost more than the cache gives.  Instead the second launch takes the
+// workgroups' shares last to first, the most recently read data first, and tensors that are larger than that cache are read and written past
+// it (backward, 48 x 256 x 64 x 176 bf16, SiLU, us: 300; last to first 282; past the cache 264; both 260.  With an operator that writes dy
+// and one that reads dx around it: 498, 483, 470, 468)
+GnArgs gn_args(int N, long long S, int C, int G, int V, int esize) {
   GnArgs a;
   a.S = S;
   a.C = C;
@@ -349,7 +358,10 @@ GnArgs gn_args(int N, long long S, int C, int G, int V) {
   a.t = a8_tile(C, V);
   const long long side = static_cast<long long>(N) * a.t.ncol, most = (S + 2 * gn_tile(a) - 1) / (2 * gn_tile(a));
   long long want = (GN_BLOCKS + side - 1) / side;
-  want = want < 1 ? 1 : want > 128 ? 128 : want;
+  long long cap = static_cast<long long>(sqrt(static_cast<double>(S) * C * esize / (8.0 * G)));
+  if (cap > (GN_BLOCKS / 4 + side - 1) / side) cap = (GN_BLOCKS / 4 + side - 1) / side;
+  if (cap < 128) cap = 128;
+  want = want < 1 ? 1 : want > cap ? cap : want;
   a.nchunk = static_cast<int>(want > most ? most : want);
   const long long tiles = (S + gn_tile(a) - 1) / gn_tile(a);
   a.tiles_each = static_cast<int>(tiles / a.nchunk);
@@ -408,13 +420,15 @@ extern "C" int dbev_gn_act_forward(const void* x, int dtype, int N, long long S,
   }
   float2* part = static_cast<float2*>(workspace);
   A8_TYPE_SWITCH(dtype, vec, {
-    const GnArgs a = gn_args(N, S, C, G, V);
+    const GnArgs a = gn_args(N, S, C, G, V, sizeof(T));
     if ((fmt != DBEV_ACT8_NONE && reinterpret_cast<uintptr_t>(codes) % V != 0) || !gn_grid_ok(N, a)) return DBEV_EINVAL;
     const dim3 grid(static_cast<unsigned>(N) * a.nchunk * a.t.ncol), block(a.t.threads);
     hipLaunchKernelGGL((gn_stats<T, V>), grid, block, gn_lds(a, V), st, static_cast<const T*>(x), a, part);
     DBEV_LAUNCH_CHECK();
-    A8_ACT_SWITCH(act, A8_FMT_SWITCH(fmt, hipLaunchKernelGGL((gn_apply<T, V, FMT, ACT>), grid, block, gn_lds(a, V), st, static_cast<const T*>(x), a, part,
-                                                             gamma, beta, eps, static_cast<T*>(y), mean, rstd, codes, scales)));
+    A8_NT_SWITCH(S * C * N * static_cast<long long>(sizeof(T)), A8_ACT_SWITCH(act, A8_FMT_SWITCH(fmt, {
+      hipLaunchKernelGGL((gn_apply<T, V, FMT, ACT, NT>), grid, block, gn_lds(a, V), st, static_cast<const T*>(x), a, part, gamma, beta, eps,
+                         static_cast<T*>(y), mean, rstd, codes, scales);
+    })));
   });
   DBEV_LAUNCH_CHECK();
   return 0;
@@ -435,7 +449,7 @@ extern "C" int dbev_gn_act_backward(const void* gy, int dtype, const void* x, in
   }
   const GnCoef k = {gamma, beta, mean, rstd};
   A8_TYPE_SWITCH(dtype, vec, {
-    const GnArgs a = gn_args(N, S, C, G, V);
+    const GnArgs a = gn_args(N, S, C, G, V, sizeof(T));
     if ((fmt != DBEV_ACT8_NONE && reinterpret_cast<uintptr_t>(codes) % V != 0) || !gn_grid_ok(N, a)) return DBEV_EINVAL;
     float2* pc = static_cast<float2*>(workspace);
     float2* pg = pc + static_cast<size_t>(N) * a.nchunk * C;
@@ -444,8 +458,10 @@ extern "C" int dbev_gn_act_backward(const void* gy, int dtype, const void* x, in
     A8_ACT_SWITCH(act, A8_FMT_SWITCH(fmt, {
       hipLaunchKernelGGL((gn_bwd_reduce<T, V, FMT, ACT>), dim3(blocks), dim3(a.t.threads), gn_lds(a, V), st, static_cast<const T*>(gy),
                          static_cast<const T*>(x), codes, scales, a, k, pc, pg);
-      hipLaunchKernelGGL((gn_bwd_dx<T, V, FMT, ACT>), dim3(blocks + npar), dim3(a.t.threads), gn_lds(a, V), st, static_cast<const T*>(gy),
-                         static_cast<const T*>(x), codes, scales, a, k, pc, pg, N, npar, static_cast<T*>(dx), dgamma, dbeta);
+      A8_NT_SWITCH(S * C * N * static_cast<long long>(sizeof(T)), {
+        hipLaunchKernelGGL((gn_bwd_dx<T, V, FMT, ACT, NT>), dim3(blocks + npar), dim3(a.t.threads), gn_lds(a, V), st, static_cast<const T*>(gy),
+                           static_cast<const T*>(x), codes, scales, a, k, pc, pg, N, npar, static_cast<T*>(dx), dgamma, dbeta);
+      });
     }));
   });
   DBEV_LAUNCH_CHECK();

@@ -7,11 +7,16 @@
 // registers.  The image's last tiles collect, four groups a workgroup: all T pairs of a group in fp64 in a fixed order, and publish the totals.
 //
 // Measured at 48 x 256 x 64 x 176 (forward / backward, us; in brackets the two launches a direction of gn_act.hip):
-//   fp32                 no activation 241 / 429 (345 / 533)   SiLU 243 / 492 (336 / 533)   GELU 253 / 509 (348 / 535)
-//   fp32, int8 kept      no activation 268 / 368 (363 / 387)   SiLU 270 / 370 (364 / 392)   GELU 291 / 378 (364 / 398)
-//   bf16 (forward only)  no activation 146 (204)   SiLU 146 (203)   GELU 166 (217); int8 kept 175 (213)   175 (213)   193 (225)
-// i.e. the forward moves its floor of 2 n es (+ 1.03 n) bytes at 4.4 to 4.6 TB/s where a copy reaches 5.3; GELU in bf16 and the backward are
-// held by VALU work (some 30 instructions an element) that a workgroup's phases overlap with the transfers only in part.
+//   fp32                 no activation 227 / 394 (300 / 481)   SiLU 224 / 450 (299 / 484)   GELU 234 / 471 (308 / 488)
+//   fp32, int8 kept      no activation 240 / 304 (327 / 334)   SiLU 246 / 317 (328 / 342)   GELU 266 / 333 (331 / 347)
+//   bf16 (forward only)  no activation 134 (166)   SiLU 143 (163)   GELU 158 (179); int8 kept 152 (187)   156 (190)   172 (201)
+// i.e. the forward moves its floor of 2 n es (+ 1.03 n) bytes at 4.7 to 5.2 TB/s in fp32 where a copy reaches 5.3, the backward at 3.8 to 4.2;
+// GELU in bf16 (3.6) and the backward are held by VALU work (some 30 instructions an element) that a workgroup's phases overlap with the
+// transfers only in part.
+//
+// These tensors are as large as the memory-side cache or larger: they are read and written past it (nontemporal).  With an operator that
+// writes x and one that reads y around the SiLU forward, us kept / past: fp32 138 MB 142 / 145, 277 MB 312 / 275, 553 MB 620 / 559; bf16 138
+// MB 160 / 160, 277 MB 324 / 298; int8 backward 185 / 181, 382 / 362, 742 / 705.
 //
 // Every published pair is ONE 64-bit word, written and read with relaxed agent-scope atomics and empty (all ones) before: a word is its own
 // flag, nothing else has to be ordered or visible, no fence writes an L2 back.  A NaN is published with the usual quiet pattern, never as
@@ -242,7 +247,7 @@ __device__ __forceinline__ void gn_one_write(const typename GnRaw<T, V>::type* r
       if (p.on) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = a8_act<ACT, T>(fmaf(v[i], sc[i], bt[i]));
-        A8Vec<T, V>::store(gn_at(yi, at * static_cast<unsigned>(sizeof(T))), v);
+        A8Vec<T, V>::template store<true>(gn_at(yi, at * static_cast<unsigned>(sizeof(T))), v);
       }
     }
     at += a.t.RP * a.C;
@@ -257,7 +262,7 @@ __device__ __forceinline__ void gn_one_load(typename GnRaw<T, V>::type* raw, con
   unsigned at = p.at * static_cast<unsigned>(sizeof(T));
 #pragma unroll
   for (int u = 0; u < R; ++u) {
-    raw[u] = p.on && u < p.nv ? *reinterpret_cast<const dw*>(gn_at(xi, at)) : dw{0, 0, 0, 0};
+    raw[u] = p.on && u < p.nv ? __builtin_nontemporal_load(reinterpret_cast<const dw*>(gn_at(xi, at))) : dw{0, 0, 0, 0};
     at += a.t.RP * a.C * static_cast<unsigned>(sizeof(T));
   }
 }
@@ -403,7 +408,7 @@ __device__ __forceinline__ void gn_one_grad(float (*g)[V], typename GnKept<T, V,
 #pragma unroll
   for (int u = 0; u < R; ++u)
     if (p.on && u < p.nv) {
-      raw[u] = *reinterpret_cast<const dw*>(gn_at(gi, (m.at + u * m.step) * static_cast<unsigned>(sizeof(T))));
+      raw[u] = __builtin_nontemporal_load(reinterpret_cast<const dw*>(gn_at(gi, (m.at + u * m.step) * static_cast<unsigned>(sizeof(T)))));
       kept[u] = GnKept<T, V, FMT>::load(xi, ci, m.at + u * m.step);
     }
   float mu[V], rs[V], sc[V], bt[V];
@@ -460,7 +465,7 @@ __device__ __forceinline__ void gn_one_dx(const float (*g)[V], typename GnKept<T
       GnKept<T, V, FMT>::get(kept[u], si, m.sat + u * m.sstep, v);
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = fmaf(sc[i], g[u][i], -fmaf(v[i] - mu[i], B[i], A[i]));
-      A8Vec<T, V>::store(gn_at(di, (m.at + u * m.step) * static_cast<unsigned>(sizeof(T))), v);
+      A8Vec<T, V>::template store<true>(gn_at(di, (m.at + u * m.step) * static_cast<unsigned>(sizeof(T))), v);
     }
   }
 }
@@ -684,7 +689,7 @@ bool gn_one_forward(const void* x, int dtype, int vec, int N, long long S, int C
 }
 
 // fp32 only: the 16-bit types would hold their gradients in twice the registers that they were read in, and the two launches are faster
-// (48 x 256 x 64 x 176 bf16, SiLU: 365 us against 296; int8 checkpoint 340 against 251)
+// (48 x 256 x 64 x 176 bf16, SiLU: 365 us against 296; int8 checkpoint 340 against 251; the two launches with nontemporal accesses: 260 and 228)
 bool gn_one_backward(const void* gy, int dtype, int vec, const void* x, int fmt, const uint8_t* codes, const uint8_t* scales, int N, long long S, int C,
                      int G, const float* gamma, const float* beta, const float* mean, const float* rstd, int act, void* dx, float* dgamma, float* dbeta,
                      void* ws, hipStream_t st) {

@@ -478,3 +478,10 @@ def test_sizes_beyond_the_limits_are_refused():
         GN.group_norm_act(torch.empty((1, 1 << 17), device=DEV), 4)
     with pytest.raises(L.DbevHipError):
         GN.group_norm_act(torch.empty((1, 8), device=DEV).expand((1 << 22) + 1, 8), 4)
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_large_image_in_many_chunks(dtype, fmt):
+    """a batch too small to fill the chip with 128 chunks an image: 400 of them"""
+    test_forward_and_backward(1, 40000, 200, 96, 12, dtype, fmt)

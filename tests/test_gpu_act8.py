@@ -510,3 +510,25 @@ def test_layers_without_gradients_keep_nothing_and_refuse_autocast():
     wide = torch.empty((1, 8), device=DEV).expand((1 << 20) + 1, 8).requires_grad_(True)
     with pytest.raises(L.DbevHipError):                                    # before the product, not in the backward pass
         A.linear(x[:, :8], wide)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tensors_beyond_the_caches_equal_their_parts(dtype, fmt):
+    """above 192 MB the accesses are other instructions: the same bits as for the two halves, which stay below"""
+    from distill_bev_amd import act8 as A
+    C = 512
+    rows = (208 << 20) // (C * torch.finfo(dtype).bits // 8)
+    x = torch.randn((rows, C), device=DEV, generator=torch.Generator(DEV).manual_seed(8)).to(dtype)
+    gy = torch.randn((rows, C), device=DEV, generator=torch.Generator(DEV).manual_seed(9)).to(dtype)
+
+    def run(x, gy):
+        ck = A.pack(x, fmt, -1)
+        leaf = x.requires_grad_(True)
+        y = A.activation(leaf, "gelu", fmt, -1)
+        return ck.codes, ck.scales, A.unpack(ck), y.detach(), torch.autograd.grad(y, (leaf,), gy)[0]
+
+    whole, h = run(x.clone(), gy), rows // 2
+    parts = [run(x[:h].clone(), gy[:h]), run(x[h:].clone(), gy[h:])]
+    for i, t in enumerate(whole):
+        assert torch.equal(t[:h], parts[0][i]) and torch.equal(t[h:], parts[1][i]), i

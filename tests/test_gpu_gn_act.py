@@ -485,3 +485,25 @@ def test_sizes_beyond_the_limits_are_refused():
 def test_one_large_image_in_many_chunks(dtype, fmt):
     """a batch too small to fill the chip with 128 chunks an image: 400 of them"""
     test_forward_and_backward(1, 40000, 200, 96, 12, dtype, fmt)
+
+
+@pytest.mark.parametrize("dtype,H", [(torch.float32, 640), (torch.bfloat16, 900)])
+def test_one_image_beyond_the_caches(dtype, H):
+    """more than 192 MB in two launches a direction (no cached accesses, last chunks first), against 64 bits on the device; norm over norm as above"""
+    from distill_bev_amd import gn_act as GN
+    g = torch.Generator(DEV).manual_seed(11)
+    x = torch.randn((1, H, H, 128), device=DEV, generator=g).to(dtype).permute(0, 3, 1, 2)
+    gy = torch.randn((1, H, H, 128), device=DEV, generator=g).to(dtype).permute(0, 3, 1, 2)
+    w, b = 1 + 0.3 * torch.randn(128, device=DEV, generator=g), 0.3 * torch.randn(128, device=DEV, generator=g)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)]
+    assert x.numel() * x.element_size() > 192 << 20
+    y = GN.group_norm_act(leaves[0], 16, leaves[1], leaves[2], 1e-5, "silu")
+    dx, dw, db = torch.autograd.grad(y, leaves, gy)
+    half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    ref = [t.detach().double().contiguous().requires_grad_(True) for t in leaves]
+    ry = F.silu(F.group_norm(ref[0], 16, ref[1], ref[2], 1e-5))
+    rdx, rdw, rdb = torch.autograd.grad(ry, ref, gy.double())
+    for got, want, slack in ((y, ry.detach(), 1.0), (dx, rdx, 2.0)):
+        assert float((got.detach().double() - want).norm()) <= (4e-6 * slack + half) * float(want.norm())
+    scale = float(gy.double().abs().sum((0, 2, 3)).max())
+    assert float((dw.double() - rdw).abs().max()) < 4e-6 * scale and float((db.double() - rdb).abs().max()) < 4e-6 * scale

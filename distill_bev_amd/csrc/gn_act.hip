@@ -1,6 +1,7 @@
 // Group norm + activation, channels-last: y = act((x - mean_g) rstd_g gamma + beta), statistics per (image, group) over S pixels x C / G
 // channels; forward (training or inference, optionally with an 8-bit checkpoint of x, act8.h) and backward (from x or the checkpoint).
 //
+// (Small images go through gn_small_fwd, large batches through gn_one_*, gn_one.hip.)
 // Forward, two launches, no finalize launch between them:
 //   gn_stats   a workgroup owns a chunk of one image's pixels x a range of channels, a thread one vector column; sums of (x - K_c) and
 //              (x - K_c)^2 with K_c the chunk's first pixel: an offset of the data costs no digits (and an outlier there, whose own
@@ -14,8 +15,8 @@
 // Bound by HBM: 3 n es forward and 5 n es backward (n es = bytes of x; with a checkpoint the two reads of x in the backward are 1.03
 // bytes a value).  All sums have a fixed order: run-to-run bit-identical, no atomics.
 // Measured, fp32, SiLU: 1 x 128 x 1024 x 1024 forward 280 us (1.6 GB in three passes: 5.8 TB/s, part of the second read comes from the
-// memory-side cache), backward 446; 8 x 128 x 128 x 128, int8 kept: 28 + 28 and 24 + 27 us, half of it cache; 6 x 256 x 15 x 25: 7 + 7 and 7 + 7 us,
-// launch and merge latency.
+// memory-side cache), backward 446; 8 x 128 x 128 x 128, int8 kept: 28 + 28 and 24 + 27 us, half of it cache; 6 x 256 x 15 x 25 backward: 7 + 7
+// us, launch and merge latency.
 #include "gn_act.h"
 #include "gn_one.h"
 
@@ -414,7 +415,8 @@ extern "C" int dbev_gn_act_forward(const void* x, int dtype, int N, long long S,
   const int vec = a8_pick_vec(a8_elem_size(dtype), C, C, x, y, nullptr);
   hipStream_t st = dbev_stream(stream);
   if ((fmt == DBEV_ACT8_NONE || reinterpret_cast<uintptr_t>(codes) % 8 == 0) &&
-      gn_one_forward(x, dtype, vec, N, S, C, G, gamma, beta, eps, act, y, mean, rstd, fmt, codes, scales, workspace, st)) {
+      (gn_small_forward(x, dtype, vec, N, S, C, G, gamma, beta, eps, act, y, mean, rstd, fmt, codes, scales, st) ||
+       gn_one_forward(x, dtype, vec, N, S, C, G, gamma, beta, eps, act, y, mean, rstd, fmt, codes, scales, workspace, st))) {
     DBEV_LAUNCH_CHECK();
     return 0;
   }

@@ -8,6 +8,9 @@ __attribute__((visibility("hidden"))) size_t gn_one_bytes(int N, long long S, in
 __attribute__((visibility("hidden"))) bool gn_one_forward(const void* x, int dtype, int vec, int N, long long S, int C, int G, const float* gamma,
                                                           const float* beta, float eps, int act, void* y, float* mean, float* rstd, int fmt,
                                                           uint8_t* codes, uint8_t* scales, void* ws, hipStream_t st);
+__attribute__((visibility("hidden"))) bool gn_small_forward(const void* x, int dtype, int vec, int N, long long S, int C, int G, const float* gamma,
+                                                            const float* beta, float eps, int act, void* y, float* mean, float* rstd, int fmt,
+                                                            uint8_t* codes, uint8_t* scales, hipStream_t st);
 __attribute__((visibility("hidden"))) bool gn_one_backward(const void* gy, int dtype, int vec, const void* x, int fmt, const uint8_t* codes,
                                                            const uint8_t* scales, int N, long long S, int C, int G, const float* gamma,
                                                            const float* beta, const float* mean, const float* rstd, int act, void* dx, float* dgamma,

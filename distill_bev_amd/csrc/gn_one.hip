@@ -211,7 +211,7 @@ __device__ __forceinline__ float* gn_one_out(float* sh, const GnArgs& a) {      
 }
 
 // y (and the checkpoint) of one tile from the values in `raw`
-template <typename T, int V, int R, int FMT, int ACT>
+template <typename T, int V, int R, int FMT, int ACT, bool NT>
 __device__ __forceinline__ void gn_one_write(const typename GnRaw<T, V>::type* raw, const float* out, const GnOneArgs& o, GnOnePos p,
                                              const float* gamma, const float* beta, T* y, uint8_t* codes, uint8_t* scales) {
   constexpr int LB = 32 / V;
@@ -247,7 +247,7 @@ __device__ __forceinline__ void gn_one_write(const typename GnRaw<T, V>::type* r
       if (p.on) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = a8_act<ACT, T>(fmaf(v[i], sc[i], bt[i]));
-        A8Vec<T, V>::template store<true>(gn_at(yi, at * static_cast<unsigned>(sizeof(T))), v);
+        A8Vec<T, V>::template store<NT>(gn_at(yi, at * static_cast<unsigned>(sizeof(T))), v);
       }
     }
     at += a.t.RP * a.C;
@@ -255,30 +255,22 @@ __device__ __forceinline__ void gn_one_write(const typename GnRaw<T, V>::type* r
   }
 }
 
-template <typename T, int V, int R>
+template <typename T, int V, int R, bool NT>
 __device__ __forceinline__ void gn_one_load(typename GnRaw<T, V>::type* raw, const T* x, const GnArgs& a, const GnOnePos& p) {
   typedef typename GnRaw<T, V>::type dw;
   const T* xi = x + static_cast<size_t>(p.n) * a.S * a.C;
   unsigned at = p.at * static_cast<unsigned>(sizeof(T));
 #pragma unroll
   for (int u = 0; u < R; ++u) {
-    raw[u] = p.on && u < p.nv ? __builtin_nontemporal_load(reinterpret_cast<const dw*>(gn_at(xi, at))) : dw{0, 0, 0, 0};
+    if (p.on && u < p.nv) raw[u] = NT ? __builtin_nontemporal_load(reinterpret_cast<const dw*>(gn_at(xi, at))) : *reinterpret_cast<const dw*>(gn_at(xi, at));
+    else raw[u] = dw{0, 0, 0, 0};
     at += a.t.RP * a.C * static_cast<unsigned>(sizeof(T));
   }
 }
 
-template <typename T, int V, int R, int FMT, int ACT>
-__global__ __launch_bounds__(256, 4) void gn_one_fwd(const T* __restrict__ x, GnOneArgs o, const float* __restrict__ gamma, const float* __restrict__ beta,
-                                                     float eps, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
-                                                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  extern __shared__ float sh[];
-  const GnArgs& a = o.a;
-  const GnOnePos p = gn_one_pos<V, R>(o, blockIdx.x);
-  float* out = gn_one_out<V>(sh, a);
-  typename GnRaw<T, V>::type raw[R];
-  gn_one_load<T, V, R>(raw, x, a, p);
-  // the tile's mean per group, then the squares about it: both from the registers
-  const int rows = min(a.t.RP * R, static_cast<int>(a.S) - p.t * (a.t.RP * R));
+// the tile's mean per group, then the squares about it, both from the registers: done(g, mean, M2) by one thread a group, out[2 g] = mean
+template <typename T, int V, int R, typename F>
+__device__ __forceinline__ void gn_one_stats(typename GnRaw<T, V>::type* raw, float* sh, float* out, const GnArgs& a, const GnOnePos& p, int rows, F done) {
   const int lanes = gn_lanes(a.G), sub = threadIdx.x % lanes;
   float s[V];
 #pragma unroll
@@ -322,13 +314,59 @@ __global__ __launch_bounds__(256, 4) void gn_one_fwd(const T* __restrict__ x, Gn
     float m2 = 0.f;
     for (int c = sub; c < a.cpg; c += lanes) m2 += sh[g * a.cpg + c];
     m2 = gn_lane_sum(m2, lanes);
-    if (sub == 0) gn_publish(o.b.part + (static_cast<size_t>(p.n) * a.G + g) * o.T + p.t, out[2 * g], m2);
+    if (sub == 0) done(g, out[2 * g], m2);
   }
   __syncthreads();                                            // out[] is read above and written below
+}
+
+template <typename T, int V, int R, int FMT, int ACT>
+__global__ __launch_bounds__(256, 4) void gn_one_fwd(const T* __restrict__ x, GnOneArgs o, const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                     float eps, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
+                                                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  extern __shared__ float sh[];
+  const GnArgs& a = o.a;
+  const GnOnePos p = gn_one_pos<V, R>(o, blockIdx.x);
+  float* out = gn_one_out<V>(sh, a);
+  typename GnRaw<T, V>::type raw[R];
+  gn_one_load<T, V, R, true>(raw, x, a, p);
+  gn_one_stats<T, V, R>(raw, sh, out, a, p, min(a.t.RP * R, static_cast<int>(a.S) - p.t * (a.t.RP * R)),
+                        [&](int g, float m, float m2) { gn_publish(o.b.part + (static_cast<size_t>(p.n) * a.G + g) * o.T + p.t, m, m2); });
   if (!gn_one_totals<true, R>(out, o, p, eps, mean, rstd)) return;
 #pragma unroll
   for (int u = 0; u < R; ++u) gn_opaque(raw[u]);
-  gn_one_write<T, V, R, FMT, ACT>(raw, out, o, p, gamma, beta, y, codes, scales);
+  gn_one_write<T, V, R, FMT, ACT, true>(raw, out, o, p, gamma, beta, y, codes, scales);
+}
+
+// Small images, forward: one workgroup holds all pixels of W channels of an image (whole groups, a multiple of 32 or all) in registers.  One
+// launch, nothing exchanged; bound by the latency of load -> two LDS folds -> store.  The helpers see the image's W channels through
+// shifted pointers.
+template <typename T, int V, int R, int FMT, int ACT>
+__global__ __launch_bounds__(256, 4) void gn_small_fwd(const T* __restrict__ x, GnOneArgs o, int W, int nblk, const float* __restrict__ gamma,
+                                                       const float* __restrict__ beta, float eps, T* __restrict__ y, float* __restrict__ mean,
+                                                       float* __restrict__ rstd, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  extern __shared__ float sh[];
+  const int n = blockIdx.x / nblk, c0 = (blockIdx.x - n * nblk) * W, w = min(W, o.a.C - c0);
+  const size_t first = static_cast<size_t>(n) * o.a.G + c0 / o.a.cpg;
+  o.a.cv = w / V;
+  o.a.G = w / o.a.cpg;
+  const GnArgs& a = o.a;
+  const GnOnePos p = gn_one_pos<V, R>(o, n);
+  float* out = gn_one_out<V>(sh, a);
+  typename GnRaw<T, V>::type raw[R];
+  gn_one_load<T, V, R, false>(raw, x + c0, a, p);
+  const double D = static_cast<double>(a.S) * a.cpg;
+  gn_one_stats<T, V, R>(raw, sh, out, a, p, static_cast<int>(a.S), [&](int g, float m, float m2) {
+    const float r = static_cast<float>(1.0 / sqrt(m2 / D + static_cast<double>(eps)));
+    out[2 * g + 1] = r;
+    if (mean != nullptr) {
+      mean[first + g] = m;
+      rstd[first + g] = r;
+    }
+  });
+#pragma unroll
+  for (int u = 0; u < R; ++u) gn_opaque(raw[u]);
+  gn_one_write<T, V, R, FMT, ACT, false>(raw, out, o, p, gamma == nullptr ? nullptr : gamma + c0, beta == nullptr ? nullptr : beta + c0, y + c0,
+                                         FMT == DBEV_ACT8_NONE ? nullptr : codes + c0, FMT == DBEV_ACT8_NONE ? nullptr : scales + c0 / 32);
 }
 
 // the tiles that gave up waiting, from memory
@@ -350,8 +388,8 @@ __global__ __launch_bounds__(256, 2) void gn_one_fwd_rest(const T* __restrict__ 
         rstd[static_cast<size_t>(p.n) * a.G + g] = out[2 * g + 1];
       }
     typename GnRaw<T, V>::type raw[R];
-    gn_one_load<T, V, R>(raw, x, a, p);
-    gn_one_write<T, V, R, FMT, ACT>(raw, out, o, p, gamma, beta, y, codes, scales);
+    gn_one_load<T, V, R, true>(raw, x, a, p);
+    gn_one_write<T, V, R, FMT, ACT, true>(raw, out, o, p, gamma, beta, y, codes, scales);
     __syncthreads();
   }
 }
@@ -667,6 +705,46 @@ size_t gn_one_bytes(int N, long long S, int C, int G) {
     case DBEV_DT_BF16: { typedef a8_bf16 T; constexpr int V = 8; __VA_ARGS__; break; }  \
     default: { typedef a8_f16 T; constexpr int V = 8; __VA_ARGS__; break; }             \
   }
+
+// Small images: W channels (whole groups, whole blocks of 32, or all of them), at most GN_RF rows a thread (fp32, 32 channels: 512 pixels);
+// wider while every thread still has a row of its own.  Against the two launches, SiLU, us on the GPU: fp32 6 x 256 x 8 x 22 7.1 (11.2), 6 x 256
+// x 15 x 25 7.7 (11.7), 48 x 512 x 22 x 22 17.9 (33.7), 200 x 256 x 16 x 32 35 (58: 210 MB at 6 TB/s); bf16 9.0 (13.5), 9.7 (13.8), 19.4 (26.9), 33
+// (44); 40000 images of one pixel, 256 channels: 228 (229), bf16 406 (388)
+bool gn_small_plan(int dtype, long long S, int C, int G, int vec, GnArgs* a, int* W) {
+  const int wide = dtype == DBEV_DT_F32 ? 4 : 8, cpg = C / G;
+  if (vec != wide || S > 256 * GN_RF) return false;
+  int unit = cpg;
+  while (unit % 32 != 0 && unit < C) unit += cpg;
+  if (unit > C) unit = C;
+  for (int w = unit;; w = 2 * w < C ? 2 * w : C) {
+    const A8Tile t = a8_tile(w, wide);
+    if (t.ncol != 1 || S > static_cast<long long>(t.RP) * (w == unit ? GN_RF : 1)) break;
+    a->t = t;
+    *W = w;
+    if (w == C) return true;
+  }
+  return a8_tile(unit, wide).ncol == 1 && S <= static_cast<long long>(a8_tile(unit, wide).RP) * GN_RF;
+}
+
+bool gn_small_forward(const void* x, int dtype, int vec, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps, int act,
+                      void* y, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  GnOneArgs o;
+  int W;
+  if (!gn_small_plan(dtype, S, C, G, vec, &o.a, &W)) return false;
+  const int nblk = (C + W - 1) / W;
+  if (static_cast<long long>(N) * nblk * o.a.t.threads >= (1LL << 32)) return false;
+  o.a = gn_one_args(o.a, S, C, G, vec);
+  o.T = 1;
+  o.polls = 0;
+  o.b = GnOneBufs{};
+  GnArgs local = o.a;
+  local.G = W / o.a.cpg;
+  GN_ONE_TYPES(dtype, A8_ACT_SWITCH(act, A8_FMT_SWITCH(fmt, {
+    hipLaunchKernelGGL((gn_small_fwd<T, V, GN_RF, FMT, ACT>), dim3(static_cast<unsigned>(N) * nblk), dim3(o.a.t.threads), gn_one_lds<V>(local), st,
+                       static_cast<const T*>(x), o, W, nblk, gamma, beta, eps, static_cast<T*>(y), mean, rstd, codes, scales);
+  })));
+  return true;
+}
 
 bool gn_one_forward(const void* x, int dtype, int vec, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps, int act, void* y,
                     float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales, void* ws, hipStream_t st) {

@@ -2,7 +2,7 @@
 
 Host-side mirror of ``norm_cfg=dict(type='GN', num_groups=G)`` layers: nn.GroupNorm -> activation of the ConvModules (mmcv order
 conv -> norm -> act; mmdet3d/models/necks/fpn.py:77-95, lss_fpn.py:30-60).  Unlike the BatchNorm kernels (bn_act.py) these take float32,
-bfloat16 and float16, any channel count, ReLU, SiLU and GELU, and any [N, C, *] shape: two launches forward, two backward, nothing but
+bfloat16 and float16, any channel count, ReLU, SiLU and GELU, and any [N, C, *] shape: one or two launches over the data a direction, nothing but
 the output written and -- under autograd -- x or its checkpoint kept (act8.py: 1.03 bytes a value, written by the forward's own pass).
 
     group_norm_act(x, num_groups, weight, bias, eps, act="silu", checkpoint="int8")     # F.group_norm + activation

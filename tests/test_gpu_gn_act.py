@@ -507,3 +507,12 @@ def test_one_image_beyond_the_caches(dtype, H):
         assert float((got.detach().double() - want).norm()) <= (4e-6 * slack + half) * float(want.norm())
     scale = float(gy.double().abs().sum((0, 2, 3)).max())
     assert float((dw.double() - rdw).abs().max()) < 4e-6 * scale and float((db.double() - rdb).abs().max()) < 4e-6 * scale
+
+
+@pytest.mark.parametrize("fmt", [None, "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,S,H,C,G", [(3, 300, 20, 200, 25), (5, 2, 1, 200, 25), (2, 512, 16, 72, 9), (2, 513, 27, 72, 9), (2, 1024, 32, 40, 5), (1, 1025, 41, 40, 5),
+                                       (70, 3, 1, 1040, 65), (2, 16, 4, 2048, 1), (2, 17, 1, 2056, 257)])
+def test_small_images(N, S, H, C, G, dtype, fmt):
+    """one workgroup an image and range of channels: last ranges of a few channels, pixel counts at the limit of a workgroup and one beyond it"""
+    test_forward_and_backward(N, S, H, C, G, dtype, fmt)

@@ -143,7 +143,7 @@ __device__ __forceinline__ void a8_decode(typename A8Bytes<V>::type c, float s, 
 }
 
 // ---- activations ------------------------------------------------------------------------------------------------------------------
-// exp2 and the reciprocal are the hardware's (1 ulp); relative error of silu ~ (1 + |z|) 2^-23.
+// exp2 and the reciprocal are the hardware's (1 ulp).
 __device__ __forceinline__ float a8_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z)); }
 
 // 1 - Phi(|z|) = exp(-z^2 / 2) * t R(t), t = 1 / (1 + p |z|): R is a least-maximum fit of erfcx / (2 t) over |z| <= 14 made for this file.
@@ -177,7 +177,13 @@ __device__ __forceinline__ void a8_normal_tail(float z, float* e, float* t, floa
 template <int ACT, typename T>
 __device__ __forceinline__ float a8_act(float z) {
   if (ACT == DBEV_ACT_RELU) return z < 0.f ? 0.f : z;              // a NaN passes
-  if (ACT == DBEV_ACT_SILU) return z * a8_sigmoid(z);
+  if (ACT == DBEV_ACT_SILU) {
+    // from q = sigmoid(-|z|), z (1 - q) or z q: where z > 0 the errors of exp2 and the reciprocal count with q / (1 - q) only, 1 - q and the
+    // product are off by half a step each.  (z times the reciprocal of 1 + exp(-z) itself is off by up to 1.5 2^-23 there, which put
+    // bf16's 5.9375 -- 9.5e-8 from a tie -- on the wrong side.)  For z < 0 off by some (1.5 |z| + 8) 2^-24
+    const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * fabsf(z)), q = e * __builtin_amdgcn_rcpf(1.f + e);
+    return z * (z > 0.f ? 1.f - q : q);
+  }
   if (ACT == DBEV_ACT_GELU) {
     float e, t, r;
     a8_normal_tail<sizeof(T) == 2>(z, &e, &t, &r);

@@ -532,3 +532,21 @@ def test_tensors_beyond_the_caches_equal_their_parts(dtype, fmt):
     parts = [run(x[:h].clone(), gy[:h]), run(x[h:].clone(), gy[h:])]
     for i, t in enumerate(whole):
         assert torch.equal(t[:h], parts[0][i]) and torch.equal(t[h:], parts[1][i]), i
+
+
+def test_silu_of_positive_bf16_values_is_correctly_rounded():
+    """y = z (1 - q), q = sigmoid(-z).  q is off by (1.5 z + 8) U of itself (exp2's argument, exp2, 1 +, reciprocal, product), which is q / (1 - q)
+    times that of y; 1 - q is rounded by half a step of [1/2, 1), 2^-25; the product by half a step of fp32, U / mantissa of y.  A tie of bf16
+    is an fp32 value, so wherever the exact y is further than these from the nearest tie the result is the exact one's.  That
+    leaves out 2^-7 alone (there y = z / 2 + z^2 / 4 to 2e-8, a tie); the closest of the others is 5.9375, 9.5e-8 from one"""
+    from distill_bev_amd import act8 as A
+    x = torch.arange(0x0080, 0x7f80, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)               # every positive normal value
+    z = x.double()
+    q = torch.sigmoid(-z)
+    y = z * (1 - q)
+    m = torch.frexp(y)[0] * 256
+    tie = (m - torch.floor(m) - 0.5).abs() / m
+    sure = tie > q / (1 - q) * (1.5 * z + 8) * U + 0.5 * U / (1 - q) + U / (m / 128)
+    assert bool(sure[x == 5.9375]) and int((~sure).sum()) == 1
+    got = A.activation(x.to(DEV), "silu").cpu()
+    assert torch.equal(got[sure], y.to(torch.bfloat16)[sure])

@@ -340,16 +340,24 @@ def linear(x, weight, bias=None, checkpoint="int8"):
 
 class _Conv1x1_8(Function):
     """F.conv2d(x, weight, bias) for a 1x1 filter on a channels-last map, products as in gemm_bf6, weight and bias gradient from the
-    checkpoint of x"""
+    checkpoint of x.  `stats` (bias-free layers): also the output's partial BatchNorm statistics rows, from the epilogue of the bf16x6 GEMM
+    ("bf6") or of the fp32 one ("f32", bn_act.conv1x1_stats); the caller has asked that kernel's rule"""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, fmt, keep):
+    def forward(ctx, x, weight, bias, fmt, keep, stats=None):
         from . import gemm_bf6 as G
-        if G.eligible(x, weight):
+        part = None
+        if stats == "f32":
+            from .bn_act import conv1x1_stats_product
+            y, part = conv1x1_stats_product(x, weight)
+        elif G.eligible(x, weight):
             M = x.shape[0] * x.shape[2] * x.shape[3]
             if ctx.needs_input_grad[0] and G.shape_ok(M, int(weight.shape[0]), int(weight.shape[1])):
                 G.pack_both(weight, M)
-            y = G.product(x, weight, bias=bias if bias is not None and bias.is_contiguous() else None)
+            if stats:
+                y, part = G.product(x, weight, stats=True)
+            else:
+                y = G.product(x, weight, bias=bias if bias is not None and bias.is_contiguous() else None)
             if bias is not None and not bias.is_contiguous():
                 y.add_(bias.view(1, -1, 1, 1))
         else:
@@ -357,14 +365,20 @@ class _Conv1x1_8(Function):
         ck = pack(x, fmt, 1) if keep else None
         ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt, ctx.x_shape = fmt, tuple(x.shape)
-        return y
+        if stats is None:
+            return y
+        ctx.mark_non_differentiable(part)
+        ctx.set_materialize_grads(False)                                  # no zero tensor for the statistics' (never used) gradient
+        return y, part
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, gy):
+    def backward(ctx, gy, _gpart=None):
         from . import gemm_bf6 as G
         weight, buf = ctx.saved_tensors
         gx = gw = gb = None
+        if gy is None:
+            return None, None, None, None, None, None
         with L.on(gy.device):
             gy = gy.contiguous(memory_format=torch.channels_last)
             gy2 = gy.permute(0, 2, 3, 1).reshape(-1, gy.shape[1])
@@ -378,7 +392,7 @@ class _Conv1x1_8(Function):
                 gw = gw.view(weight.shape)                                # [Co, Ci] in memory: dense in both memory formats of a 1x1 filter
             elif ctx.needs_input_grad[2]:
                 gb = _bias_grad(gy2)
-        return gx, gw, gb, None, None
+        return gx, gw, gb, None, None, None
 
 
 def conv1x1(x, weight, bias=None, checkpoint="int8"):
@@ -390,6 +404,19 @@ def conv1x1(x, weight, bias=None, checkpoint="int8"):
     _check_layer(x, weight, bias, "conv1x1")
     with L.on(x.device):
         return _Conv1x1_8.apply(x.contiguous(memory_format=torch.channels_last), weight, bias, checkpoint, _recording(weight))
+
+
+def conv1x1_stats(conv, x, kernel):
+    """(conv(x), partial BatchNorm statistics rows of it) for a layer that `keeps` x, by the epilogue of `kernel` ("bf6": gemm_bf6.eligible
+    says so; "f32": bn_act.conv1x1_bn_ready does)"""
+    return _Conv1x1_8.apply(x, conv.weight, None, conv.act8_format, True, kernel)
+
+
+def keeps(conv, x):
+    """does this call of a 1x1 convolution module keep x as an 8-bit checkpoint?  For code that runs a module's product without its forward
+    (nets.Bottleneck, colsum.conv_bn_cancelled_bias)"""
+    return (getattr(conv, "act8_format", None) is not None and _plain_1x1(conv) and _recording(conv.weight) and x.dim() == 4 and x.numel() > 0
+            and _module_ready(x, conv.weight, conv.bias))
 
 
 # ---- modules ------------------------------------------------------------------------------------------------------------------------

@@ -246,24 +246,29 @@ def bn_act_dual(x, bn, xd, bn_d, relu=True, pre=None, pre_d=None, fork=False):
     return bn_act(x, bn, bn_act(xd, bn_d, None, False, pre=pre_d), relu, pre=pre, fork=fork)
 
 
+def conv1x1_stats_product(x, w):
+    """z = conv1x1(x, w) on the fp32 matrix cores with the BatchNorm partial statistics of z in the epilogue (dbev_conv1x1_forward); no autograd"""
+    dev = x.device
+    N, Ci, H, W = x.shape
+    Co = w.shape[0]
+    M = N * H * W
+    z = torch.empty((N, Co, H, W), dtype=torch.float32, device=dev, memory_format=torch.channels_last)
+    rows = int(L.call("dbev_conv1x1_stats_rows", M, Ci, Co))
+    part = torch.empty((rows, 2, Co), dtype=torch.float32, device=dev)
+    w2 = w.reshape(Co, Ci)
+    w2 = w2 if w2.is_contiguous() else w2.contiguous()
+    with torch.cuda.device(dev):
+        L.call("dbev_conv1x1_forward", L.ptr(x), L.ptr(w2), L.ptr(z), L.ptr(part), M, Ci, Co, Ci, L.stream_ptr(dev),
+               alg_bytes=4 * M * (Ci + Co))
+    return z, part
+
+
 class _Conv1x1Stats(Function):
-    """z = conv1x1(x, w) on the fp32 matrix cores with the BatchNorm partial statistics of z in the epilogue
-    (dbev_conv1x1_forward); backward = the library convolution's data / weight gradients."""
+    """`conv1x1_stats_product`; backward = the library convolution's data / weight gradients."""
 
     @staticmethod
     def forward(ctx, x, w):
-        dev = x.device
-        N, Ci, H, W = x.shape
-        Co = w.shape[0]
-        M = N * H * W
-        z = torch.empty((N, Co, H, W), dtype=torch.float32, device=dev, memory_format=torch.channels_last)
-        rows = int(L.call("dbev_conv1x1_stats_rows", M, Ci, Co))
-        part = torch.empty((rows, 2, Co), dtype=torch.float32, device=dev)
-        w2 = w.reshape(Co, Ci)
-        w2 = w2 if w2.is_contiguous() else w2.contiguous()
-        with torch.cuda.device(dev):
-            L.call("dbev_conv1x1_forward", L.ptr(x), L.ptr(w2), L.ptr(z), L.ptr(part), M, Ci, Co, Ci, L.stream_ptr(dev),
-                   alg_bytes=4 * M * (Ci + Co))
+        z, part = conv1x1_stats_product(x, w)
         ctx.save_for_backward(x, w)
         ctx.mark_non_differentiable(part)
         ctx.set_materialize_grads(False)                  # no zero tensor for the (never used) gradient of the statistics output
@@ -295,7 +300,7 @@ def conv1x1_bn_ready(conv, bn, x):
     library than the hand-written kernel with the statistics in its epilogue -- measured (tools/kbench_c1x1.py,
     profiles/r03_conv1x1_vs_miopen.txt): the >= 300 k-pixel maps of the image backbone's first stage (64 <-> 256 channels, HBM-bound:
     conv + statistics 0.21 vs 0.30 ms); at stage 2 the two are even, from stage 3 on the library's kernels win."""
-    if not (_C1["enabled"] and _state["enabled"] and type(conv).__name__ in ("Conv2d", "Bf6Conv2d") and isinstance(conv, nn.Conv2d)
+    if not (_C1["enabled"] and _state["enabled"] and type(conv).__name__ in ("Conv2d", "Bf6Conv2d", "Act8Conv2d") and isinstance(conv, nn.Conv2d)
             and conv.kernel_size == (1, 1) and conv.stride == (1, 1)
             and conv.padding == (0, 0) and conv.dilation == (1, 1) and conv.groups == 1 and conv.bias is None):
         return False
@@ -310,6 +315,9 @@ def conv1x1_bn_ready(conv, bn, x):
 
 def conv1x1_stats(conv, x):
     """-> (conv(x), partial statistics rows) for a pair accepted by conv1x1_bn_ready"""
+    from . import act8
+    if act8.keeps(conv, x):
+        return act8.conv1x1_stats(conv, x, "f32")
     return _Conv1x1Stats.apply(x, conv.weight)
 
 

@@ -30,12 +30,16 @@ from .registry import (MODELS, ConvModule, build_activation_layer, build_conv_la
 def _conv1x1_stats(conv, bn, x):
     """a bottleneck's 1x1 convolution -> (z, partial statistics rows of z or None): the bf16x6 GEMM with the norm's statistics in its
     epilogue where it takes the layer, else the fp32-MFMA GEMM with the same epilogue on the first stage's large maps
-    (conv1x1_bn_ready: the round-3 kernel, 0.4 ms per step slower than the bf16x6 one on the layers both take), else the module"""
+    (conv1x1_bn_ready: the round-3 kernel, 0.4 ms per step slower than the bf16x6 one on the layers both take), else the module.
+    A layer that keeps its input in 8 bits (act8.Act8Conv2d) does so in all of them"""
+    from . import act8
     from . import bn_act as BA
     from . import gemm_bf6 as G
     if (G._STATS and conv.bias is None and G.eligible(x, conv.weight, conv.stride, conv.padding, conv.dilation, conv.groups)
             and BA._state["enabled"] and type(bn) in BA._BN_TYPES and bn.affine and bn.training and bn.momentum is not None
             and bn.running_mean is not None and BA._channels_ok(conv.out_channels)):
+        if act8.keeps(conv, x):
+            return act8.conv1x1_stats(conv, x, "bf6")
         return G.conv1x1_stats(x, conv.weight)                # (also without autograd: the detached frame)
     if (G._STATS and conv.bias is None and tuple(conv.stride) == (2, 2)
             and G.eligible_s2(x, conv.weight, conv.stride, conv.padding, conv.dilation, conv.groups)

@@ -550,3 +550,72 @@ def test_silu_of_positive_bf16_values_is_correctly_rounded():
     assert bool(sure[x == 5.9375]) and int((~sure).sum()) == 1
     got = A.activation(x.to(DEV), "silu").cpu()
     assert torch.equal(got[sure], y.to(torch.bfloat16)[sure])
+
+
+def _kept_bytes(run, own):
+    """bytes of the tensors that `run` saves for its backward pass, storages counted once, those of `own` left out"""
+    held = {}
+
+    def save(t):
+        held[t.untyped_storage().data_ptr()] = t.untyped_storage().nbytes()
+        keep.append(t)                                                     # (no address is used twice)
+        return t
+
+    keep = []
+    with torch.autograd.graph.saved_tensors_hooks(save, lambda t: t):
+        out = run()
+    skip = {q.untyped_storage().data_ptr() for q in own}
+    return out, sum(b for a, b in held.items() if a not in skip)
+
+
+@pytest.mark.parametrize("inplanes,planes,n,h,w", [(256, 64, 4, 120, 120), (96, 32, 4, 280, 281)])
+def test_bottleneck_keeps_its_one_by_one_inputs_in_8_bits(inplanes, planes, n, h, w):
+    """nets.Bottleneck runs its 1x1 convolutions without their modules' forward, with the norm's statistics from the product's epilogue (bf16x6
+    in the first case, the fp32 GEMM in the second): both inputs are kept as checkpoints, the output is the same bits, and a layer's weight
+    gradient is the checkpoint's"""
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import bn_act as BA
+    from distill_bev_amd import gemm_bf6 as G
+    from distill_bev_amd import nets
+    from distill_bev_amd.train_step import to_channels_last
+    x = torch.randn(n, inplanes, h, w, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(memory_format=torch.channels_last)
+    gy = torch.randn(n, 4 * planes, h, w, device=DEV, generator=torch.Generator(DEV).manual_seed(2)).to(memory_format=torch.channels_last)
+
+    def one(fmt):
+        torch.manual_seed(3)
+        ds = None if inplanes == 4 * planes else nn.Sequential(nn.Conv2d(inplanes, 4 * planes, 1, bias=False), nn.BatchNorm2d(4 * planes))
+        m = nets.Bottleneck(inplanes, planes, downsample=ds).to(DEV).train()
+        to_channels_last(m, fmt)
+        leaf = x.clone().requires_grad_(True)
+        y, kept = _kept_bytes(lambda: m(leaf), list(m.parameters()) + list(m.buffers()))
+        y.backward(gy)
+        return m, y.detach(), kept, leaf.grad, {k: q.grad for k, q in m.named_parameters()}
+
+    mod, y, kept, gx, grads = one(None)
+    m8, y8, kept8, gx8, grads8 = one("int8")
+    assert m8.act8_modules == (2 if inplanes == 4 * planes else 3) and torch.equal(y, y8)
+    M, inputs = n * h * w, {(256, 64): 256 + 64, (96, 32): 96 + 32}[(inplanes, planes)]     # (conv1 and the downsample share one fp32 input)
+    codes = inputs + (0 if inplanes == 4 * planes else 96)
+    assert kept - kept8 >= M * (4 * inputs - 33 / 32 * codes) - (1 << 16), (kept, kept8)
+    # relative error of a kept value 2^-7 of its block's largest (3 spreads or less): a hundredth at random signs
+    for k in grads:
+        assert float((grads[k] - grads8[k]).norm()) < 0.03 * float(grads[k].norm()), k
+    assert float((gx - gx8).norm()) < 1e-5 * float(gx.norm())              # the data gradients do not see the checkpoint
+    conv, bn = m8.conv1, getattr(m8, m8.norm1_name)
+    kernel = "bf6" if G.eligible(x, conv.weight) else "f32"
+    assert kernel == ("bf6" if inplanes == 256 else "f32") and (kernel == "bf6" or BA.conv1x1_bn_ready(conv, bn, x)) and A.keeps(conv, x)
+    gz = gy[:, :planes].contiguous(memory_format=torch.channels_last)
+    leaf = x.clone().requires_grad_(True)
+    z, rows = nets._conv1x1_stats(conv, bn, leaf)
+    a = torch.autograd.grad(z, (leaf, conv.weight), gz)
+    conv.act8_format = None                                                 # the same layer without a checkpoint
+    z0, rows0 = nets._conv1x1_stats(conv, bn, leaf)
+    b = torch.autograd.grad(z0, (leaf, conv.weight), gz)
+    assert torch.equal(z, z0) and torch.equal(rows, rows0) and not rows.requires_grad
+    assert float((a[0] - b[0]).norm()) <= 1e-6 * float(b[0].norm())
+    assert torch.equal(a[1].view(planes, inplanes), A.weight_gradient(A.pack(x, "int8", 1), gz))
+    with torch.no_grad():
+        assert torch.equal(nets._conv1x1_stats(conv, bn, x)[0], z)
+    m8.eval()
+    with torch.no_grad():
+        assert torch.equal(m8(x), mod.eval()(x))

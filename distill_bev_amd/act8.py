@@ -497,7 +497,10 @@ def use_act8(model, fmt="int8"):
     """Let the plain Linear and 1x1 / stride-1 convolution modules of `model` (bf16x6 ones included) keep their input as an 8-bit checkpoint,
     and the activations whose input nothing else keeps: every SiLU / GELU, and a ReLU right behind one of those layers in an nn.Sequential
     (elsewhere a ReLU's output is kept by the layer behind it anyway).  nn.MultiheadAttention reads its projections' weights itself and
-    stays as it is.  Returns how many modules changed.  Idempotent for one format."""
+    stays as it is.  Returns how many modules changed class.  Idempotent for one format.
+    The biased 1x1 layers of a model that has been through train_step.accelerate_modules (BiasSumConv2d) stay what they are and are given the
+    format; two kernels that take such a layer as a whole keep its input their own way: the depth head's and the adaptation loss's."""
+    from .colsum import BiasSumConv2d
     _fmt(fmt)
     n = 0
     for mod in model.modules():
@@ -509,7 +512,7 @@ def use_act8(model, fmt="int8"):
         if to is not None:
             mod.__class__ = to
             n += 1
-        if isinstance(mod, (Act8Linear, Act8Conv2d, Act8Activation)):
+        if isinstance(mod, (Act8Linear, Act8Conv2d, Act8Activation)) or type(mod) is BiasSumConv2d and _plain_1x1(mod):
             mod.act8_format = fmt
     for mod in list(model.modules()):
         kids = list(mod._modules.items())

@@ -78,9 +78,15 @@ class _BiasConv(Function):
 
 class BiasSumConv2d(nn.Conv2d):
     """nn.Conv2d with a bias whose bias gradient is `channel_sum` of the output gradient when the input is a channels-last fp32 device
-    tensor and gradients are recorded; the stock module otherwise.  Same parameters and state-dict keys."""
+    tensor and gradients are recorded; the stock module otherwise.  Same parameters and state-dict keys.  `act8_format` ("int8" / "e4m3",
+    set by act8.use_act8; 1x1 layers at stride 1): the input is kept as an 8-bit checkpoint"""
+    act8_format = None
 
     def forward(self, x):
+        if self.act8_format is not None:
+            from . import act8
+            if act8.keeps(self, x):
+                return act8.conv1x1(x, self.weight, self.bias, self.act8_format)
         if (self.bias is not None and self.padding_mode == "zeros" and torch.is_tensor(x) and x.is_cuda
                 and x.dtype == torch.float32 and _nhwc(x) and x.numel() > 0 and not isinstance(self.padding, str)):
             from . import gemm_bf6 as G                       # a 1x1 layer the bf16x6 GEMM takes: its kernels + this module's bias handling
@@ -133,15 +139,22 @@ def conv_bn_cancelled_bias(conv, bn, x, bn_call):
     bn.running_mean with mean(z), which is then moved by momentum * bias.  Only in front of the fused norm kernels (bn_act.eligible):
     they update the running statistics through raw pointers and save neither of them, the library's BatchNorm saves both for its
     backward (a later in-place update raises) -- there the convolution keeps its bias."""
+    from . import act8
     from . import bn_act as BA
     from . import gemm_bf6 as G
     part = None
+    kept = act8.keeps(conv, x)                                      # the input as an 8-bit checkpoint (act8.use_act8)
     if G.eligible(x, conv.weight, conv.stride, conv.padding, conv.dilation, conv.groups):
         if G._STATS and BA._channels_ok(conv.out_channels) and BA._state["enabled"] and type(bn) in BA._BN_TYPES and bn.affine:
-            z, part = G.conv1x1_stats(x, conv.weight)               # the norm's statistics from the GEMM's epilogue
+            # the norm's statistics from the GEMM's epilogue
+            z, part = act8.conv1x1_stats(conv, x, "bf6") if kept else G.conv1x1_stats(x, conv.weight)
+        elif kept:
+            z = act8.conv1x1(x, conv.weight, None, conv.act8_format)
         else:
             z = G.conv1x1(x, conv.weight) if torch.is_grad_enabled() and (x.requires_grad or conv.weight.requires_grad) \
                 else G.product(x, conv.weight)
+    elif kept:
+        z = act8.conv1x1(x, conv.weight, None, conv.act8_format)
     else:
         z = F.conv2d(x, conv.weight, None, conv.stride, conv.padding, conv.dilation, conv.groups)
     if not BA.eligible(z, bn):

@@ -156,10 +156,12 @@ def accelerate_modules(detector, activation_checkpoint=None):
     # `activation_checkpoint` ("int8" / "e4m3"): the student's group norms, linear layers, 1x1 convolutions and activations keep their
     # inputs in 8 bits for the backward pass (the teacher runs without gradients and keeps nothing)
     detector.fused_gn = sum(fuse_gn_act_modules(r, activation_checkpoint if r is detector else None) for r in roots)
-    detector.act8_modules = 0
+    detector.act8_modules = detector.act8_bias_convs = 0              # modules of a class of their own; biased 1x1 convolutions given the format
     if activation_checkpoint is not None:
         from .act8 import use_act8
+        from .colsum import BiasSumConv2d
         detector.act8_modules = use_act8(detector, activation_checkpoint)
+        detector.act8_bias_convs = sum(type(m) is BiasSumConv2d and m.act8_format is not None for m in detector.modules())
     n_up = 0
     for r in roots:
         for mod in r.modules():

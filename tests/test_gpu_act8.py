@@ -619,3 +619,40 @@ def test_bottleneck_keeps_its_one_by_one_inputs_in_8_bits(inplanes, planes, n, h
     m8.eval()
     with torch.no_grad():
         assert torch.equal(m8(x), mod.eval()(x))
+
+
+@pytest.mark.parametrize("n,h,w", [(2, 9, 11), (4, 120, 120)])
+def test_biased_one_by_one_layers_of_an_accelerated_model(n, h, w):
+    """BiasSumConv2d alone and in front of a BatchNorm that cancels its bias, in sizes of the library's product and of the bf16x6 GEMM's: the input
+    is kept in 8 bits, the forward pass is that of the layer without a checkpoint"""
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import colsum
+    from distill_bev_amd.detectors import ThreeLayer
+    from distill_bev_amd.train_step import to_channels_last
+    x = torch.randn(n, 64, h, w, device=DEV, generator=torch.Generator(DEV).manual_seed(4)).to(memory_format=torch.channels_last)
+    gy = torch.randn(n, 64, h, w, device=DEV, generator=torch.Generator(DEV).manual_seed(5)).to(memory_format=torch.channels_last)
+
+    def one(build, fmt):
+        torch.manual_seed(6)
+        m = build().to(DEV).train()
+        to_channels_last(m, fmt)
+        leaf = x.clone().requires_grad_(True)
+        y, kept = _kept_bytes(lambda: m(leaf), list(m.parameters()) + list(m.buffers()))
+        y.backward(gy)
+        return m, y.detach(), kept, leaf.grad, {k: q.grad for k, q in m.named_parameters()}
+
+    for build, layers in ((lambda: nn.Sequential(nn.Conv2d(64, 64, 1)), 1), (lambda: ThreeLayer(64, 64, 64, kernel_size=1, stride=1), 3)):
+        mod, y, kept, gx, grads = one(build, None)
+        m8, y8, kept8, gx8, grads8 = one(build, "e4m3")
+        convs = [m for m in m8.modules() if isinstance(m, nn.Conv2d)]
+        assert m8.act8_modules == 0 and m8.act8_bias_convs == layers == len(convs) and all(type(m) is colsum.BiasSumConv2d for m in convs)
+        assert torch.allclose(y8, y, rtol=0, atol=2e-6 * float(y.abs().max()))                # (the bias is added in another place)
+        assert kept - kept8 >= layers * n * h * w * 64 * (4 - 33 / 32) - (1 << 12), (kept, kept8)
+        assert float((gx - gx8).norm()) < 1e-5 * float(gx.norm())
+        for k in grads:                          # e4m3: at most 2^-4 of each value, random signs
+            if layers == 1 or not k.startswith("conv") or not k.endswith("bias"):
+                assert float((grads[k] - grads8[k]).norm()) < 0.05 * float(grads[k].norm()), k
+        if layers == 1:
+            gw, gb = A.weight_gradient(A.pack(x, "e4m3", 1), gy, bias=True)
+            assert torch.equal(grads8["0.weight"].view(64, 64), gw) and torch.equal(grads8["0.bias"], gb)
+    assert A.use_act8(m8, "e4m3") == 0

@@ -220,3 +220,22 @@ def test_trainer_option_rewires_the_student_and_steps():
         Trainer(_Toy(), dict(), torch.device("cpu"), activation_checkpoint="int8")
     with pytest.raises(ValueError):
         Trainer(_Toy(), dict(), torch.device("cpu"), channels_last=True, activation_checkpoint="int4")
+
+
+def test_trainer_option_marks_biased_one_by_one_layers():
+    """they were re-classed for their bias gradient before the option's turn: they keep that class and get the format"""
+    from distill_bev_amd.colsum import BiasSumConv2d
+    from distill_bev_amd.train_step import Trainer
+    torch.manual_seed(4)
+    tr = Trainer(_Toy(), dict(), torch.device("cpu"), channels_last=True, activation_checkpoint="e4m3")
+    conv = tr.detector.neck[0]
+    assert type(conv) is BiasSumConv2d and conv.act8_format == "e4m3" and tr.detector.act8_bias_convs == 1
+    torch.manual_seed(4)
+    ref = Trainer(_Toy(), dict(), torch.device("cpu"), channels_last=True)
+    assert ref.detector.act8_bias_convs == 0 and ref.detector.neck[0].act8_format is None
+    x = torch.randn(2, 16, 6, 5)
+    assert torch.allclose(tr.step(dict(x=x))[0], ref.step(dict(x=x))[0], atol=1e-6)
+    plain = nn.Conv2d(8, 8, 3, padding=1)
+    plain.__class__ = BiasSumConv2d                                       # not a 1x1 layer
+    from distill_bev_amd import act8 as A
+    assert A.use_act8(nn.Sequential(plain)) == 0 and plain.act8_format is None

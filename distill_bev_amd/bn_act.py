@@ -89,6 +89,14 @@ def _alias(y):
     return torch.empty((0,), dtype=y.dtype, device=y.device).set_(y.untyped_storage(), y.storage_offset(), y.size(), y.stride())
 
 
+def _version_of(t):
+    """an empty tensor that shares t's version counter and not its storage: saved for the backward pass, it makes autograd notice an in-place
+    write to t without keeping t's memory"""
+    v = t.detach()
+    v.data = torch.empty((0,), dtype=t.dtype, device=t.device)
+    return v
+
+
 def _two_addends(dy, dy2):
     """incoming gradients of a forked output -> (first, second or None), channels-last"""
     if dy is None:
@@ -130,13 +138,14 @@ class _BNActTrain(Function):
                    alg_bytes=4 * M * C * (3 + (residual is not None) - (pre is not None)))     # x (stats), x (apply) [+ res] + y
         L.touched(running_mean, running_var, nbt)
         y2 = _alias(y) if fork else None
-        # both handles of a forked output are SAVED (whether or not the backward reads y): they share one storage but have separate
-        # version counters, so an in-place op on either handle (`feat += ...`, `relu_`) would silently change what the other handle's
-        # consumer saved for its backward -- saved, autograd's version check turns that into its usual "modified by an inplace
-        # operation" error when this node's backward unpacks them (ADVICE r3).  Contract: forked outputs are never written in place.
+        # the version counters of both handles of a forked output are SAVED (whether or not the backward reads y): they share one storage but
+        # have separate version counters, so an in-place op on either handle (`feat += ...`, `relu_`) would silently change what the other
+        # handle's consumer saved for its backward -- saved, autograd's version check turns that into its usual "modified by an inplace
+        # operation" error when this node's backward unpacks them.  Contract: forked outputs are never written in place.
         # (the gate mask travels through save_for_backward like everything else the backward reads: saved-tensor hooks / offloading see
-        # it -- ADVICE r5; when it exists the backward does not read y, which stays saved only as a forked handle, see above)
-        ctx.save_for_backward(x, y if ((need_y and gmask is None) or fork) else None, weight, save_mean, save_invstd, coef, y2, gmask)
+        # it; when it exists the backward does not read y, and the map lives on only if a consumer keeps it)
+        ykept = y if need_y and gmask is None else _version_of(y) if fork else None
+        ctx.save_for_backward(x, ykept, weight, save_mean, save_invstd, coef, _version_of(y2) if fork else None, gmask)
         ctx.cfg = (M, C, bool(relu), residual is not None, need_y)
         if fork:
             ctx.set_materialize_grads(False)
@@ -194,7 +203,8 @@ class _BNDualTrain(Function):
                    alg_bytes=4 * M * C * (5 - (pre is not None) - (pre_d is not None)))
         L.touched(rm, rv, nbt, rmd, rvd, nbtd)
         y2 = _alias(y) if fork else None
-        ctx.save_for_backward(x, xd, y if ((relu and gmask is None) or fork) else None, w, wd, stats, y2, gmask)     # both handles saved: see _BNActTrain.forward
+        ykept = y if relu and gmask is None else _version_of(y) if fork else None              # both versions saved: see _BNActTrain.forward
+        ctx.save_for_backward(x, xd, ykept, w, wd, stats, _version_of(y2) if fork else None, gmask)
         ctx.cfg = (M, C, bool(relu))
         if fork:
             ctx.set_materialize_grads(False)

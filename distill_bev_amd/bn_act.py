@@ -385,7 +385,7 @@ def _infer(x, residual, bn, relu):
 
 
 def bn_act(x, bn, residual=None, relu=True, pre=None, fork=False):
-    """relu(bn(x) + residual) with the module `bn`'s parameters, statistics and mode.  `pre`: partial statistics rows of x taken by
+    """relu(bn(x) + residual) with the module `bn`'s parameters, statistics and mode (a group norm is taken too).  `pre`: partial statistics rows of x taken by
     its producer (conv1x1_stats) -- only handed over when the training-mode kernel path applies (conv1x1_bn_ready).  `fork`: the
     result is a residual block's output; under autograd it then carries a second handle (`forked(y)`) for the next block's identity
     branch (see _BNActTrain.forward)."""
@@ -396,6 +396,12 @@ def bn_act(x, bn, residual=None, relu=True, pre=None, fork=False):
             return _fork_out(_BNActTrain.apply(x, residual, bn.weight, bn.bias, bn.running_mean, bn.running_var,
                                                bn.num_batches_tracked, bn.momentum, bn.eps, relu, pre, fk), fk)
         return _infer(x, residual, bn, relu)
+    from .gn_act import GroupNormAct, norm_act
+    if type(bn) is GroupNormAct:                              # kernels and ledger of their own (gn_act.gn_act)
+        if residual is None:
+            return norm_act(x, bn, "relu" if relu else "none")
+        out = norm_act(x, bn) + residual
+        return F.relu(out) if relu else out
     if x.is_cuda and _state["enabled"] and x.numel() > 0:
         L.note_fallback("bn_act", _why_not(x, bn, residual))
     out = nn.BatchNorm2d.forward(bn, x) if isinstance(bn, BatchNormAct2d) else bn(x)

@@ -8,6 +8,7 @@ the output written and -- under autograd -- x or its checkpoint kept (act8.py: 1
     group_norm_act(x, num_groups, weight, bias, eps, act="silu", checkpoint="int8")     # F.group_norm + activation
     gn_act(x, gn, act, checkpoint)                                                       # the same with a module's parameters
     GroupNormAct                                                                         # nn.GroupNorm + activation, same state-dict keys
+    norm_act(x, norm, act)                                                               # act(norm(x)) of any norm module, in one operator where it can be
     fuse_gn_act_modules(model, checkpoint=None)                                          # rewires a built model
 
 `group_norm_act` raises on what the kernels cannot take (a tensor in another layout is copied to channels-last first); the modules leave
@@ -157,6 +158,16 @@ def gn_act(x, gn, act="none", checkpoint=None):
     return _STOCK[act](F.group_norm(x, gn.num_groups, gn.weight, gn.bias, gn.eps))
 
 
+def norm_act(x, norm, act="none"):
+    """act(norm(x)) for any norm module; `act`: a name or an activation module.  One operator where the norm is a GroupNormAct without an activation
+    of its own and the activation is one of act8.ACTS -- for blocks that hold the two as separate attributes (nets.BasicBlock, Bottleneck)"""
+    name = act if isinstance(act, str) else act.act if type(act) is A.Act8Activation else A.act_name(act)
+    if type(norm) is GroupNormAct and norm.act == "none" and name:
+        return gn_act(x, norm, name, norm.act8_format)
+    y = norm(x)
+    return _STOCK[act](y) if isinstance(act, str) else act(y)
+
+
 class GroupNormAct(nn.GroupNorm):
     """nn.GroupNorm that also applies the activation behind it (`act`, one of act8.ACTS) and may keep its input as an 8-bit checkpoint
     (`act8_format`: None, "int8" or "e4m3"); parameters and state-dict keys are nn.GroupNorm's"""
@@ -178,7 +189,8 @@ class GroupNormAct(nn.GroupNorm):
 
 def fuse_gn_act_modules(model, checkpoint=None):
     """Rewire the nn.GroupNorm modules of nn.Sequential stacks and ConvModules onto the kernels, together with the ReLU / SiLU / GELU right
-    behind them (replaced by nn.Identity; keys unchanged); other GroupNorm modules become GroupNormAct without an activation.
+    behind them (replaced by nn.Identity; keys unchanged); other GroupNorm modules become GroupNormAct without an activation (the residual
+    blocks of nets.py put theirs in by `norm_act`).
     A norm that several places share keeps the activations behind it as modules.  `checkpoint`: the format in which the norms keep their
     input, or None.  Returns how many norms changed.  Idempotent."""
     from .registry import ConvModule

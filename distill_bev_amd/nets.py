@@ -21,6 +21,7 @@ import torch.nn.functional as F
 import torch.utils.checkpoint as cp
 
 from .bn_act import bn_act, bn_act_dual, conv1x1_bn_ready, conv1x1_stats, forked, split_downsample
+from .gn_act import norm_act
 from .pool import conv_norm_relu_max_pool, max_pool
 from .wino import conv3x3_bn_ready, conv3x3_stats
 from .registry import (MODELS, ConvModule, build_activation_layer, build_conv_layer, build_norm_layer,
@@ -89,7 +90,7 @@ class BasicBlock(nn.Module):
 
     def _inner(self, x):
         identity = x
-        out = self.act1(getattr(self, self.norm1_name)(self.conv1(x)))
+        out = norm_act(self.conv1(x), getattr(self, self.norm1_name), self.act1)
         out = getattr(self, self.norm2_name)(self.conv2(out))
         if self.downsample is not None:
             identity = self.downsample(x)
@@ -146,8 +147,8 @@ class Bottleneck(nn.Module):
 
     def _inner(self, x):
         identity = x
-        out = self.act1(getattr(self, self.norm1_name)(self.conv1(x)))
-        out = self.act2(getattr(self, self.norm2_name)(self.conv2(out)))
+        out = norm_act(self.conv1(x), getattr(self, self.norm1_name), self.act1)
+        out = norm_act(self.conv2(out), getattr(self, self.norm2_name), self.act2)
         out = getattr(self, self.norm3_name)(self.conv3(out))
         if self.downsample is not None:
             identity = self.downsample(x)

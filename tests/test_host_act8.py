@@ -239,3 +239,19 @@ def test_trainer_option_marks_biased_one_by_one_layers():
     plain.__class__ = BiasSumConv2d                                       # not a 1x1 layer
     from distill_bev_amd import act8 as A
     assert A.use_act8(nn.Sequential(plain)) == 0 and plain.act8_format is None
+
+
+@pytest.mark.parametrize("act", ["ReLU", "SiLU", "LeakyReLU"])
+def test_residual_blocks_with_group_norm_compute_the_same(act):
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    from distill_bev_amd import nets
+    torch.manual_seed(5)
+    x = torch.randn(2, 16, 6, 5)
+    for cls in (nets.BasicBlock, nets.Bottleneck):
+        m = cls(16, 16 // cls.expansion, norm_cfg=dict(type="GN", num_groups=2), act_cfg=dict(type=act))
+        ref = m(x)
+        assert GN.fuse_gn_act_modules(m) == (2 if cls is nets.BasicBlock else 3)
+        assert torch.allclose(m(x), ref, atol=1e-6)
+        A.use_act8(m)
+        assert torch.allclose(m(x), ref, atol=1e-6)

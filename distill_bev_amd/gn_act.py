@@ -191,8 +191,8 @@ def fuse_gn_act_modules(model, checkpoint=None):
     """Rewire the nn.GroupNorm modules of nn.Sequential stacks and ConvModules onto the kernels, together with the ReLU / SiLU / GELU right
     behind them (replaced by nn.Identity; keys unchanged); other GroupNorm modules become GroupNormAct without an activation (the residual
     blocks of nets.py put theirs in by `norm_act`).
-    A norm that several places share keeps the activations behind it as modules.  `checkpoint`: the format in which the norms keep their
-    input, or None.  Returns how many norms changed.  Idempotent."""
+    A norm that several places share keeps the activations behind it as modules.  `checkpoint`: the format in which all norms of the model
+    keep their input; None leaves that to each norm (a GroupNormAct's own `act8_format`; plain norms keep x).  Returns how many norms changed.  Idempotent."""
     from .registry import ConvModule
     if checkpoint is not None:
         A._fmt(checkpoint)
@@ -224,6 +224,6 @@ def fuse_gn_act_modules(model, checkpoint=None):
         if type(mod) is nn.GroupNorm:
             take(mod, "none")
             n += 1
-        elif type(mod) is GroupNormAct:
+        elif type(mod) is GroupNormAct and checkpoint is not None:
             mod.act8_format = checkpoint
     return n

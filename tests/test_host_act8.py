@@ -255,3 +255,19 @@ def test_residual_blocks_with_group_norm_compute_the_same(act):
         assert torch.allclose(m(x), ref, atol=1e-6)
         A.use_act8(m)
         assert torch.allclose(m(x), ref, atol=1e-6)
+
+
+def test_a_norms_own_format_survives_a_trainer_without_the_option():
+    from distill_bev_amd import gn_act as GN
+    from distill_bev_amd.train_step import Trainer
+    torch.manual_seed(6)
+    toy = _Toy()
+    toy.neck = nn.Sequential(nn.Conv2d(16, 64, 1), GN.GroupNormAct(8, 64, act="silu", checkpoint="int8"), nn.Conv2d(64, 64, 1), nn.GroupNorm(4, 64))
+    tr = Trainer(toy, dict(), torch.device("cpu"), channels_last=True)
+    assert tr.detector.neck[1].act8_format == "int8" and tr.detector.neck[1].act == "silu" and tr.detector.neck[3].act8_format is None
+    toy = _Toy()
+    assert GN.fuse_gn_act_modules(toy, "int8") == 1
+    Trainer(toy, dict(), torch.device("cpu"), channels_last=True)
+    assert toy.neck[1].act8_format == "int8"
+    Trainer(toy, dict(), torch.device("cpu"), channels_last=True, activation_checkpoint="e4m3")       # asked for: all norms
+    assert toy.neck[1].act8_format == "e4m3"

@@ -161,8 +161,8 @@ def gn_act(x, gn, act="none", checkpoint=None):
 def norm_act(x, norm, act="none"):
     """act(norm(x)) for any norm module; `act`: a name or an activation module.  One operator where the norm is a GroupNormAct without an activation
     of its own and the activation is one of act8.ACTS -- for blocks that hold the two as separate attributes (nets.BasicBlock, Bottleneck)"""
-    name = act if isinstance(act, str) else act.act if type(act) is A.Act8Activation else A.act_name(act)
-    if type(norm) is GroupNormAct and norm.act == "none" and name:
+    name = act if isinstance(act, str) else act.act if type(act) is A.Act8Activation and not A.hooked(act) else A.act_name(act)
+    if type(norm) is GroupNormAct and norm.act == "none" and name and not A.hooked(norm):
         return gn_act(x, norm, name, norm.act8_format)
     y = norm(x)
     return _STOCK[act](y) if isinstance(act, str) else act(y)
@@ -191,9 +191,11 @@ def fuse_gn_act_modules(model, checkpoint=None):
     """Rewire the nn.GroupNorm modules of nn.Sequential stacks and ConvModules onto the kernels, together with the ReLU / SiLU / GELU right
     behind them (replaced by nn.Identity; keys unchanged); other GroupNorm modules become GroupNormAct without an activation (the residual
     blocks of nets.py put theirs in by `norm_act`).
-    A norm that several places share keeps the activations behind it as modules.  `checkpoint`: the format in which all norms of the model
+    A norm that several places share, or that carries hooks, keeps the activations behind it as modules, and so do one with hooks of its own and
+    stacks whose forward is not the class's.  `checkpoint`: the format in which all norms of the model
     keep their input; None leaves that to each norm (a GroupNormAct's own `act8_format`; plain norms keep x).  Returns how many norms changed.  Idempotent."""
     from .registry import ConvModule
+    from .wino import ConvNormSequential
     if checkpoint is not None:
         A._fmt(checkpoint)
     n = 0
@@ -206,16 +208,19 @@ def fuse_gn_act_modules(model, checkpoint=None):
         norm.__class__ = GroupNormAct
         norm.act, norm.act8_format = act, checkpoint
 
+    def alone(norm):
+        return places[id(norm)] == 1 and not A.hooked(norm)
+
     for mod in list(model.modules()):
-        if isinstance(mod, nn.Sequential):
+        if type(mod).forward in (nn.Sequential.forward, ConvNormSequential.forward):
             kids = list(mod._modules.items())
             for (_, a), (kb, b) in zip(kids, kids[1:]):
-                if type(a) is nn.GroupNorm and places[id(a)] == 1 and A.act_name(b):
+                if type(a) is nn.GroupNorm and alone(a) and A.act_name(b):
                     take(a, A.act_name(b))
                     mod._modules[kb] = nn.Identity()
                     n += 1
-        elif isinstance(mod, ConvModule) and mod.with_norm and type(mod.norm) is nn.GroupNorm:
-            act = A.act_name(mod.activate) if mod.with_activation and places[id(mod.norm)] == 1 else None
+        elif type(mod).forward is ConvModule.forward and mod.with_norm and type(mod.norm) is nn.GroupNorm:
+            act = A.act_name(mod.activate) if mod.with_activation and alone(mod.norm) else None
             take(mod.norm, act or "none")
             if act:
                 mod.activate = nn.Identity()

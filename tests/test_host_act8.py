@@ -271,3 +271,34 @@ def test_a_norms_own_format_survives_a_trainer_without_the_option():
     assert toy.neck[1].act8_format == "int8"
     Trainer(toy, dict(), torch.device("cpu"), channels_last=True, activation_checkpoint="e4m3")       # asked for: all norms
     assert toy.neck[1].act8_format == "e4m3"
+
+
+def test_modules_with_hooks_and_stacks_with_a_forward_of_their_own_are_not_folded():
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    from distill_bev_amd import nets
+    from distill_bev_amd.registry import ConvModule
+
+    class Skip(nn.Sequential):
+        def forward(self, x):
+            h = self[0](x)
+            return h + self[1](h)
+
+    torch.manual_seed(7)
+    x = torch.randn(2, 8, 4, 5)
+    skip = Skip(nn.GroupNorm(2, 8), nn.SiLU())
+    ref = skip(x)
+    assert GN.fuse_gn_act_modules(skip) == 1 and torch.allclose(skip(x), ref, atol=1e-6)
+    for at in (0, 1):                                                     # a hook on the norm, on the activation
+        for build in (lambda: nn.Sequential(nn.GroupNorm(2, 8), nn.SiLU()),
+                      lambda: ConvModule(8, 8, 1, norm_cfg=dict(type="GN", num_groups=2), act_cfg=dict(type="SiLU")),
+                      lambda: nets.BasicBlock(8, 8, norm_cfg=dict(type="GN", num_groups=2), act_cfg=dict(type="SiLU"))):
+            torch.manual_seed(8)
+            m = build()
+            pair = ([k for k in m.modules() if type(k) is nn.GroupNorm][0], [k for k in m.modules() if type(k) is nn.SiLU][0])
+            seen = []
+            pair[at].register_forward_hook(lambda mod, i, o: seen.append(o.detach().clone()))
+            ref = m(x)
+            GN.fuse_gn_act_modules(m, "int8")
+            A.use_act8(m)
+            assert torch.allclose(m(x), ref, atol=1e-6) and len(seen) == 2 and torch.allclose(seen[0], seen[1], atol=1e-6)

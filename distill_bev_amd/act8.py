@@ -19,8 +19,8 @@ int8 is the finer one for values that fill their block's range, e4m3 for blocks 
 restores as NaN.  ReLU's derivative is taken at x^, where a positive value below half of the smallest code is zero.
 
 `use_act8(model, fmt)` swaps these layers into a built model; parameters and state-dict keys stay.  The functions above raise on what the
-kernels cannot take (linear and conv1x1 under autocast too: they compute in their arguments' type); the modules leave CPU and float64 tensors
-and autocast to the stock operators (device tensors are counted in the fallback ledger)."""
+kernels cannot take (linear and conv1x1 under autocast too: they compute in their arguments' type); the modules leave CPU and float64 tensors,
+autocast and layers of more than 2^20 channels or 2^31 weights to the stock operators (device tensors are counted in the fallback ledger)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -221,8 +221,12 @@ def activation(x, act="gelu", checkpoint="int8", channel_dim=None):
     return _act_forward(x.detach(), act, None, dim)[0]
 
 
+def _gradient_fits(Ci, Co):
+    return Ci <= 1 << 20 and Co <= 1 << 20 and Ci * Co <= 1 << 31
+
+
 def _gradient_ok(Ci, Co):
-    if Ci > 1 << 20 or Co > 1 << 20 or Ci * Co > 1 << 31:
+    if not _gradient_fits(Ci, Co):
         raise L.DbevHipError(f"act8: weight gradient of {Ci} -> {Co} channels; at most 2^20 and 2^31 weights")
 
 
@@ -420,14 +424,19 @@ def keeps(conv, x):
 
 
 # ---- modules ------------------------------------------------------------------------------------------------------------------------
-def _module_ready(x, *params):
-    """may a module's call go to the kernels?  Device tensors of one supported type; a device tensor that may not is counted."""
+def _module_ready(x, weight=None, bias=None):
+    """may a module's call go to the kernels?  Device tensors of one supported type, a weight whose gradient fits; a device tensor that may not is
+    counted."""
     if not (torch.is_tensor(x) and x.is_cuda):
         return False
-    if x.dtype not in DTYPES or any(p is not None and p.dtype != x.dtype for p in params) or torch.is_autocast_enabled("cuda"):
-        L.note_fallback("act8", f"dtype {x.dtype}" + (" under autocast" if torch.is_autocast_enabled("cuda") else ""))
-        return False
-    return True
+    why = None
+    if x.dtype not in DTYPES or any(p is not None and p.dtype != x.dtype for p in (weight, bias)) or torch.is_autocast_enabled("cuda"):
+        why = f"dtype {x.dtype}" + (" under autocast" if torch.is_autocast_enabled("cuda") else "")
+    elif weight is not None and not _gradient_fits(int(weight.shape[1]), int(weight.shape[0])):
+        why = f"{int(weight.shape[1])} -> {int(weight.shape[0])} channels"
+    if why:
+        L.note_fallback("act8", why)
+    return why is None
 
 
 def _recording(*tensors):

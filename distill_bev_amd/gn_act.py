@@ -12,7 +12,7 @@ the output written and -- under autograd -- x or its checkpoint kept (act8.py: 1
     fuse_gn_act_modules(model, checkpoint=None)                                          # rewires a built model
 
 `group_norm_act` raises on what the kernels cannot take (a tensor in another layout is copied to channels-last first); the modules leave
-CPU and float64 tensors to the stock operators (device tensors are counted in the fallback ledger)."""
+CPU and float64 tensors, autocast and sizes beyond the kernels' to the stock operators (device tensors are counted in the fallback ledger)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -104,6 +104,13 @@ class _GroupNormAct(Function):
         return dx if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None
 
 
+def _fits(x):
+    """the kernels' limits (dbev_gn_act_workspace_bytes has the same)"""
+    N, C = x.shape[:2]
+    S = x.numel() // (N * C) if x.numel() else 0
+    return C <= 1 << 16 and N <= 1 << 22 and S <= 1 << 30 and S * C <= 1 << 36
+
+
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", checkpoint=None):
     """act(F.group_norm(x, num_groups, weight, bias, eps)) for a device tensor x [N, C, *], act one of act8.ACTS; the result is
     channels-last.  `checkpoint` ("int8" / "e4m3"): under autograd the 8-bit checkpoint of x is kept instead of x, and the gradients are
@@ -122,8 +129,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.shape != (C,) or t.dtype not in A.DTYPES):
             raise ValueError(f"group_norm_act: {name} {tuple(t.shape)} {t.dtype} for {C} channels")
-    if C > 1 << 16 or N > 1 << 22:
-        raise L.DbevHipError(f"group_norm_act: {N} images of {C} channels; at most 2^22 and 2^16")
+    if not _fits(x):
+        raise L.DbevHipError(f"group_norm_act: {N} images of {C} channels, {tuple(x.shape)}; at most 2^22 and 2^16, of 2^30 pixels and 2^36 values")
     if not eps >= 0:
         raise ValueError(f"group_norm_act: eps {eps}")
     if x.numel() and x.numel() // G == 1:                         # F.group_norm's own refusal
@@ -136,13 +143,15 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
 
 
 def _ready(x, gn):
-    if not (torch.is_tensor(x) and x.is_cuda and x.numel()):
+    if not (torch.is_tensor(x) and x.is_cuda and x.numel() and x.dim() >= 2):
         return False
     why = None
     if x.dtype not in A.DTYPES or (gn.weight is not None and gn.weight.dtype not in A.DTYPES):
         why = f"dtype {x.dtype}"
     elif torch.is_autocast_enabled("cuda"):
         why = "autocast"
+    elif not _fits(x):
+        why = f"size {tuple(x.shape)}"
     if why:
         L.note_fallback("gn_act", why)
     return why is None

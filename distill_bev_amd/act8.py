@@ -20,11 +20,12 @@ restores as NaN.  ReLU's derivative is taken at x^, where a positive value below
 
 `use_act8(model, fmt)` swaps these layers into a built model; parameters and state-dict keys stay.  The functions above raise on what the
 kernels cannot take (linear and conv1x1 under autocast too: they compute in their arguments' type); the modules leave CPU and float64 tensors,
-autocast and layers of more than 2^20 channels or 2^31 weights to the stock operators (device tensors are counted in the fallback ledger)."""
+autocast, layers of more than 2^20 channels or 2^31 weights, and calls under torch.jit.trace, forward-mode differentiation or a torch.func
+transform to the stock operators (device tensors are counted in the fallback ledger)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -52,6 +53,23 @@ def _dtype(t, what="x"):
     if t.dtype not in DTYPES:
         raise L.DbevHipError(f"{what}: float32, bfloat16 or float16 expected, got {t.dtype}")
     return DTYPES[t.dtype]
+
+
+def transformed():
+    """is this call traced, differentiated forward, or inside a torch.func transform?  The kernels fill tensors through their addresses, which none
+    of these sees: such a call takes the stock operators (modules) or raises (functions)"""
+    return torch.jit.is_tracing() or forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
+
+
+def no_trace(what):
+    if torch.jit.is_tracing():
+        raise L.DbevHipError(f"{what}: torch.jit.trace cannot record it (the modules trace as the stock operators)")
+
+
+def _no_derivative(what):
+    no_trace(what)
+    if transformed():
+        raise L.DbevHipError(f"{what}: not under forward-mode differentiation or a torch.func transform (it has no derivative)")
 
 
 def dense_dim(x):
@@ -144,6 +162,12 @@ def _dim(x, channel_dim):
 def pack(x, fmt="int8", channel_dim=None):
     """the 8-bit checkpoint of a device tensor (no autograd).  `channel_dim`: the dimension along which the blocks of 32 run; by default
     the one that is dense in memory (`dense_dim`)."""
+    _fmt(fmt), _dtype(x)
+    _no_derivative("pack")
+    return _pack(x, fmt, channel_dim)
+
+
+def _pack(x, fmt, channel_dim):
     f, dt = _fmt(fmt), _dtype(x)
     dev = L.require_cuda(x)
     dim = _dim(x, channel_dim)
@@ -161,6 +185,7 @@ def unpack(ck, dtype=None):
     dtype = ck.dtype if dtype is None else dtype
     if dtype not in DTYPES:
         raise L.DbevHipError(f"unpack: float32, bfloat16 or float16 expected, got {dtype}")
+    _no_derivative("unpack")
     dev = L.require_cuda(ck.buf)
     with L.on(dev):
         out = empty_dense(ck.shape, ck.dim, dtype, dev)
@@ -213,10 +238,11 @@ class _Activation8(Function):
 
 def activation(x, act="gelu", checkpoint="int8", channel_dim=None):
     """act(x), act one of `ACTS` (gelu: the erf form); under autograd the 8-bit checkpoint of x is kept and dx = gy * act'(x^)"""
+    no_trace("activation")
     _act(act), _fmt(checkpoint), _dtype(x)
     L.require_cuda(x)
     dim = _dim(x, channel_dim)
-    if x.requires_grad and torch.is_grad_enabled():
+    if x.requires_grad and torch.is_grad_enabled() or transformed():        # (transformed: the function raises)
         return _Activation8.apply(x, act, checkpoint, dim)
     return _act_forward(x.detach(), act, None, dim)[0]
 
@@ -255,6 +281,7 @@ def weight_gradient(ck, gy, bias=False):
     """gy^T x^ [Co, Ci] (and with `bias` the sums of gy over its rows, [Co]) in gy's type, for the checkpoint of a layer's input and the
     gradient of its output: gy has the checkpoint's shape but for the channel dimension.  fp32 sums, fp32 accuracy for fp32 gy."""
     _dtype(gy, "gy")
+    _no_derivative("weight_gradient")
     dev = L.require_cuda(ck.buf, gy)
     dim, want = ck.dim, ck.shape
     if gy.dim() != len(want) or any(gy.shape[d] != want[d] for d in range(len(want)) if d != dim):
@@ -304,7 +331,7 @@ class _Linear8(Function):
                 y.add_(bias)
         else:
             y = F.linear(x2, weight, bias)
-        ck = pack(x2, fmt, -1) if keep else None
+        ck = _pack(x2, fmt, -1) if keep else None
         ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt = fmt
         return y
@@ -332,6 +359,7 @@ class _Linear8(Function):
 
 def linear(x, weight, bias=None, checkpoint="int8"):
     """F.linear(x, weight, bias), differentiable; the 8-bit checkpoint of x is what the weight gradient is computed from"""
+    no_trace("linear")
     _fmt(checkpoint)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] == 0:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
@@ -366,7 +394,7 @@ class _Conv1x1_8(Function):
                 y.add_(bias.view(1, -1, 1, 1))
         else:
             y = F.conv2d(x, weight, bias)
-        ck = pack(x, fmt, 1) if keep else None
+        ck = _pack(x, fmt, 1) if keep else None
         ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt, ctx.x_shape = fmt, tuple(x.shape)
         if stats is None:
@@ -402,6 +430,7 @@ class _Conv1x1_8(Function):
 def conv1x1(x, weight, bias=None, checkpoint="int8"):
     """F.conv2d(x, weight, bias) for a 1x1 filter, stride 1, differentiable; x is taken as (or copied to) a channels-last map and its 8-bit
     checkpoint is what the weight gradient is computed from"""
+    no_trace("conv1x1")
     _fmt(checkpoint)
     if weight.dim() != 4 or tuple(weight.shape[2:]) != (1, 1) or x.dim() != 4 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"conv1x1: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
@@ -434,6 +463,8 @@ def _module_ready(x, weight=None, bias=None):
         why = f"dtype {x.dtype}" + (" under autocast" if torch.is_autocast_enabled("cuda") else "")
     elif weight is not None and not _gradient_fits(int(weight.shape[1]), int(weight.shape[0])):
         why = f"{int(weight.shape[1])} -> {int(weight.shape[0])} channels"
+    elif transformed():
+        why = "traced or transformed"
     if why:
         L.note_fallback("act8", why)
     return why is None

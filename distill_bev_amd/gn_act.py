@@ -12,7 +12,8 @@ the output written and -- under autograd -- x or its checkpoint kept (act8.py: 1
     fuse_gn_act_modules(model, checkpoint=None)                                          # rewires a built model
 
 `group_norm_act` raises on what the kernels cannot take (a tensor in another layout is copied to channels-last first); the modules leave
-CPU and float64 tensors, autocast and sizes beyond the kernels' to the stock operators (device tensors are counted in the fallback ledger)."""
+CPU and float64 tensors, autocast, sizes beyond the kernels' and calls under torch.jit.trace, forward-mode differentiation or a torch.func
+transform to the stock operators (device tensors are counted in the fallback ledger)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -115,6 +116,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     """act(F.group_norm(x, num_groups, weight, bias, eps)) for a device tensor x [N, C, *], act one of act8.ACTS; the result is
     channels-last.  `checkpoint` ("int8" / "e4m3"): under autograd the 8-bit checkpoint of x is kept instead of x, and the gradients are
     those of the formula with x^ in place of x (mean and rstd stay x's own)."""
+    A.no_trace("group_norm_act")
     A._act(act)
     if checkpoint is not None:
         A._fmt(checkpoint)
@@ -135,7 +137,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
         raise ValueError(f"group_norm_act: eps {eps}")
     if x.numel() and x.numel() // G == 1:                         # F.group_norm's own refusal
         raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    if A._recording(x, weight, bias) or A.transformed():          # (transformed: the function raises)
         return _GroupNormAct.apply(x, weight, bias, G, float(eps), act, checkpoint)
     with L.on(dev):
         xd, N, C, S = _maps(x.detach())
@@ -152,6 +154,8 @@ def _ready(x, gn):
         why = "autocast"
     elif not _fits(x):
         why = f"size {tuple(x.shape)}"
+    elif A.transformed():
+        why = "traced or transformed"
     if why:
         L.note_fallback("gn_act", why)
     return why is None

@@ -40,3 +40,75 @@ def test_modules_beyond_the_limits_take_the_stock_operators():
     A.use_act8(conv)
     y, n = _stock(conv, torch.ones(1, 8, 2, 2, device=DEV))
     assert n["act8"] == 1 and y.shape == (1, (1 << 20) + 1, 2, 2)
+
+
+def _net():
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    torch.manual_seed(1)
+    stock = nn.Sequential(nn.Conv2d(16, 32, 1), nn.GroupNorm(4, 32), nn.SiLU(), nn.Flatten(2), nn.GELU(), nn.Linear(35, 24))
+    mod = nn.Sequential(nn.Conv2d(16, 32, 1), nn.GroupNorm(4, 32), nn.SiLU(), nn.Flatten(2), nn.GELU(), nn.Linear(35, 24))
+    mod.load_state_dict(stock.state_dict())
+    stock, mod = stock.to(DEV), mod.to(DEV).to(memory_format=torch.channels_last)
+    assert GN.fuse_gn_act_modules(mod, "int8") == 1 and A.use_act8(mod, "int8") == 3
+    x = torch.randn(2, 16, 5, 7, device=DEV).to(memory_format=torch.channels_last)
+    return stock, mod, x
+
+
+def test_forward_mode_derivatives_pass_through_the_modules_and_are_refused_by_the_functions():
+    import torch.autograd.forward_ad as fw
+    from distill_bev_amd import _lib as L
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    stock, mod, x = _net()
+    for m in (stock, mod):
+        m.requires_grad_(False)                                            # a frozen network: nothing requires grad
+    t = torch.randn_like(x)
+    with fw.dual_level():
+        ref = fw.unpack_dual(stock(fw.make_dual(x, t)))
+        (out, n) = _stock(mod, fw.make_dual(x, t))
+        out = fw.unpack_dual(out)
+        assert out.tangent is not None and torch.allclose(out.primal, ref.primal, atol=1e-5) and torch.allclose(out.tangent, ref.tangent, atol=1e-5)
+        assert n["gn_act"] == 1
+        d = fw.make_dual(x, t)
+        rows = fw.make_dual(torch.randn(6, 32, device=DEV), torch.randn(6, 32, device=DEV))
+        with pytest.raises(NotImplementedError):
+            GN.group_norm_act(d, 4)
+        for call in (lambda: A.activation(rows), lambda: A.linear(rows, torch.randn(8, 32, device=DEV)),
+                     lambda: A.conv1x1(d, torch.randn(8, 16, 1, 1, device=DEV))):
+            with pytest.raises(NotImplementedError):
+                call()
+        with pytest.raises(L.DbevHipError):
+            A.pack(rows)
+    jvp = torch.func.jvp(lambda v: _stock(mod, v)[0], (x,), (t,))
+    assert torch.allclose(jvp[1], ref.tangent, atol=1e-5)
+    params = dict(mod.named_parameters())
+    grads = torch.func.grad(lambda p: torch.func.functional_call(mod, p, (x,)).square().sum())(params)
+    want = torch.autograd.grad(stock.requires_grad_(True)(x).square().sum(), list(stock.parameters()))
+    for g, w in zip(grads.values(), want):
+        assert torch.allclose(g, w.view(g.shape), rtol=1e-4, atol=1e-4 * float(w.abs().max()))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda v: GN.group_norm_act(v, 4).sum())(x)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_modules_trace_as_the_stock_operators_and_functions_refuse(grad):
+    from distill_bev_amd import _lib as L
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    stock, mod, x = _net()
+    for m in (stock, mod):
+        m.requires_grad_(grad)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        traced = torch.jit.trace(mod, (x,))
+        other = torch.randn_like(x)
+        assert torch.allclose(traced(other), stock(other), atol=1e-5)
+        rows = torch.randn(6, 32, device=DEV)
+        w, lw = torch.randn(16, device=DEV, requires_grad=grad), torch.randn(8, 32, device=DEV, requires_grad=grad)
+        cw = torch.randn(4, 16, 1, 1, device=DEV, requires_grad=grad)
+        for f, a in ((lambda v: GN.group_norm_act(v, 4, w, act="silu", checkpoint="int8"), x), (lambda v: A.activation(v, "gelu"), rows),
+                     (lambda v: A.linear(v, lw), rows), (lambda v: A.conv1x1(v, cw), x), (lambda v: A.unpack(A.pack(v)), rows)):
+            f(a)
+            with pytest.raises(L.DbevHipError, match="trace"):
+                torch.jit.trace(f, (a,), check_trace=False)

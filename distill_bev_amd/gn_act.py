@@ -65,44 +65,67 @@ def _forward(x, N, C, S, G, weight, bias, eps, act, fmt, stats):
     return y, st, buf
 
 
+def _gradients(ctx, gy):
+    kept, weight, bias, st = ctx.saved_tensors
+    G, eps, act, fmt = ctx.cfg
+    dev = gy.device
+    _, need_w, need_b = ctx.needs_input_grad[:3]
+    with L.on(dev):
+        w, b = _f32(weight), _f32(bias)
+        dx = A.empty_dense(gy.shape, 1, gy.dtype, dev)
+        gy, N, C, S = _maps(gy)
+        n = N * S * C
+        new = torch.empty if n else torch.zeros
+        dwb = new((2, C), dtype=torch.float32, device=dev) if need_w or need_b else None
+        if n:
+            nbytes = int(L.call("dbev_gn_act_workspace_bytes", N, S, C, G))
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            mean, k, dw = st.data_ptr(), kept.data_ptr(), _ptr(dwb)
+            L.call("dbev_gn_act_backward", gy.data_ptr(), A.DTYPES[gy.dtype], None if fmt else k, A.FORMATS[fmt] if fmt else 0,
+                   k if fmt else None, k + n if fmt else None, N, S, C, G, _ptr(w), _ptr(b), mean, mean + 4 * N * G, A.ACTS[act],
+                   dx.data_ptr(), dw if need_w else None, dw + 4 * C if need_b else None, ws.data_ptr(), nbytes, L.raw_stream(dev),
+                   alg_bytes=2 * n * gy.element_size() + (n if fmt else n * gy.element_size()))
+        dw = db = None
+        if need_w:
+            dw = dwb[0] if weight.dtype == torch.float32 else dwb[0].to(weight.dtype)
+        if need_b:
+            db = dwb[1] if bias.dtype == torch.float32 else dwb[1].to(bias.dtype)
+    return dx if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None
+
+
 class _GroupNormAct(Function):
+    """x dense channels-last"""
+
     @staticmethod
     def forward(ctx, x, weight, bias, G, eps, act, fmt):
         with L.on(x.device):
             xd, N, C, S = _maps(x)
-            w, b = _f32(weight), _f32(bias)
-            y, st, buf = _forward(xd, N, C, S, G, w, b, eps, act, fmt, True)
-        ctx.save_for_backward(buf if fmt else xd, w, b, st)
-        ctx.cfg = (G, act, fmt, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+            y, st, buf = _forward(xd, N, C, S, G, _f32(weight), _f32(bias), eps, act, fmt, True)
+        ctx.save_for_backward(buf if fmt else x, weight, bias, st)
+        ctx.cfg = (G, eps, act, fmt)
         return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        if not torch.is_grad_enabled():
+            return _gradients(ctx, gy)
+        # gradients that will be differentiated again: those of the stock operators (nn.GroupNorm has second derivatives too)
+        x, weight, bias, _ = ctx.saved_tensors
+        G, eps, act, _ = ctx.cfg
+        f32 = lambda t: None if t is None else t.float()                  # noqa: E731
+        y = _STOCK[act](F.group_norm(x.float(), G, f32(weight), f32(bias), eps)).to(x.dtype)
+        need = ctx.needs_input_grad[:3]
+        grads = iter(torch.autograd.grad(y, [t for t, n in zip((x, weight, bias), need) if n], gy, create_graph=True))
+        return (*(next(grads) if n else None for n in need), None, None, None, None)
+
+
+class _GroupNormAct8(_GroupNormAct):
+    """the same from a checkpoint: no second derivatives"""
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        kept, w, b, st = ctx.saved_tensors
-        G, act, fmt, wt, bt = ctx.cfg
-        dev = gy.device
-        _, need_w, need_b = ctx.needs_input_grad[:3]
-        with L.on(dev):
-            dx = A.empty_dense(gy.shape, 1, gy.dtype, dev)
-            gy, N, C, S = _maps(gy)
-            n = N * S * C
-            new = torch.empty if n else torch.zeros
-            dwb = new((2, C), dtype=torch.float32, device=dev) if need_w or need_b else None
-            if n:
-                nbytes = int(L.call("dbev_gn_act_workspace_bytes", N, S, C, G))
-                ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-                mean, k, dw = st.data_ptr(), kept.data_ptr(), _ptr(dwb)
-                L.call("dbev_gn_act_backward", gy.data_ptr(), A.DTYPES[gy.dtype], None if fmt else k, A.FORMATS[fmt] if fmt else 0,
-                       k if fmt else None, k + n if fmt else None, N, S, C, G, _ptr(w), _ptr(b), mean, mean + 4 * N * G, A.ACTS[act],
-                       dx.data_ptr(), dw if need_w else None, dw + 4 * C if need_b else None, ws.data_ptr(), nbytes, L.raw_stream(dev),
-                       alg_bytes=2 * n * gy.element_size() + (n if fmt else n * gy.element_size()))
-            dw = db = None
-            if need_w:
-                dw = dwb[0] if wt == torch.float32 else dwb[0].to(wt)
-            if need_b:
-                db = dwb[1] if bt == torch.float32 else dwb[1].to(bt)
-        return dx if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None
+        return _gradients(ctx, gy)
 
 
 def _fits(x):
@@ -138,7 +161,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     if x.numel() and x.numel() // G == 1:                         # F.group_norm's own refusal
         raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
     if A._recording(x, weight, bias) or A.transformed():          # (transformed: the function raises)
-        return _GroupNormAct.apply(x, weight, bias, G, float(eps), act, checkpoint)
+        x = _maps(x)[0]                                               # (a copy of another layout is a step of the graph by itself)
+        return (_GroupNormAct8 if checkpoint else _GroupNormAct).apply(x, weight, bias, G, float(eps), act, checkpoint)
     with L.on(dev):
         xd, N, C, S = _maps(x.detach())
         return _forward(xd, N, C, S, G, _f32(weight), _f32(bias), float(eps), act, None, False)[0]

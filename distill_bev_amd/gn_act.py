@@ -12,8 +12,8 @@ the output written and -- under autograd -- x or its checkpoint kept (act8.py: 1
     fuse_gn_act_modules(model, checkpoint=None)                                          # rewires a built model
 
 `group_norm_act` raises on what the kernels cannot take (a tensor in another layout is copied to channels-last first); the modules leave
-CPU and float64 tensors, autocast, sizes beyond the kernels' and calls under torch.jit.trace, forward-mode differentiation or a torch.func
-transform to the stock operators (device tensors are counted in the fallback ledger)."""
+CPU and float64 tensors, other layouts that keep no checkpoint, autocast, sizes beyond the kernels' and calls under torch.jit.trace, forward-mode
+differentiation or a torch.func transform to the stock operators (device tensors are counted in the fallback ledger)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -185,13 +185,27 @@ def _ready(x, gn):
     return why is None
 
 
+def _channels_last(x):
+    if x.dim() == 2 or x.numel() == x.shape[0] * x.shape[1]:                # one pixel
+        return x.is_contiguous()
+    return (x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last)
+            or x.dim() == 5 and x.is_contiguous(memory_format=torch.channels_last_3d))
+
+
 def gn_act(x, gn, act="none", checkpoint=None):
-    """act(gn(x)) with the module `gn`'s parameters: the kernels for device tensors they take, the stock operators otherwise"""
+    """act(gn(x)) with the module `gn`'s parameters: the kernels for device tensors they take, the stock operators otherwise.  A channels-last map
+    (or [N, C]) stays one.  A tensor of another layout gives a contiguous one, as torch's operator does, and goes to the kernels -- by copies
+    in and out -- only to keep a checkpoint or where the parameters are of another type than x, which torch's does not take"""
     A._act(act)
     if checkpoint is not None:
         A._fmt(checkpoint)
     if _ready(x, gn):
-        return group_norm_act(x, gn.num_groups, gn.weight, gn.bias, gn.eps, act, checkpoint)
+        args = (gn.num_groups, gn.weight, gn.bias, gn.eps, act, checkpoint)
+        if _channels_last(x):
+            return group_norm_act(x, *args)
+        if checkpoint is not None and A._recording(x, gn.weight, gn.bias) or gn.weight is not None and gn.weight.dtype != x.dtype:
+            return group_norm_act(x, *args).contiguous()
+        L.note_fallback("gn_act", f"layout {tuple(x.shape)} {x.stride()}")
     return _STOCK[act](F.group_norm(x, gn.num_groups, gn.weight, gn.bias, gn.eps))
 
 

@@ -138,3 +138,37 @@ def test_second_derivatives_without_a_checkpoint(act, layout):
     torch.autograd.grad(torch.autograd.grad(mod(leaves[0]).square().sum(), (leaves[0],), create_graph=True)[0].square().sum(), (leaves[0],))
     with pytest.raises(RuntimeError):
         penalty(lambda x, w, b: GN.group_norm_act(x, 4, w, b, act=act, checkpoint="int8"), leaves, gy.to(DEV))
+
+
+def test_modules_give_the_layout_that_they_were_given():
+    """channels-last maps stay channels-last; a dense tensor of another layout comes out contiguous, by the stock operator unless a checkpoint is kept"""
+    from distill_bev_amd import _lib as L
+    from distill_bev_amd import gn_act as GN
+    torch.manual_seed(3)
+    for shape, fmt in (((2, 16, 7), None), ((2, 16, 5, 6), None), ((2, 16, 3, 4, 5), None), ((2, 16), None),
+                       ((2, 16, 5, 6), torch.channels_last), ((2, 16, 3, 4, 5), torch.channels_last_3d)):
+        x = torch.randn(shape, device=DEV)
+        x = (x if fmt is None else x.contiguous(memory_format=fmt)).requires_grad_(True)
+        gy = torch.randn(shape, device=DEV)
+        dense = fmt is None and len(shape) > 2
+        for ck in (None, "int8"):
+            mod = GN.GroupNormAct(4, 16, act="silu", checkpoint=ck).to(DEV)
+            y, n = _stock(mod, x)
+            ref = F.silu(F.group_norm(x, 4, mod.weight, mod.bias))
+            assert torch.allclose(y, ref, atol=1e-5) and n["gn_act"] == int(dense and ck is None)
+            assert y.is_contiguous() if fmt is None else y.is_contiguous(memory_format=fmt)
+            if fmt is None:
+                y.view(-1)
+            with torch.no_grad():
+                y, n = _stock(mod, x)                                      # nothing to keep
+                assert torch.allclose(y, ref, atol=1e-5) and n["gn_act"] == int(dense)
+            a, = torch.autograd.grad(mod(x), (x,), gy)
+            b, = torch.autograd.grad(ref, (x,), gy)
+            # a checkpoint's values are off by 2^-7 of their block's largest at most (some 3 spreads)
+            assert float((a - b).norm()) < (1e-5 if ck is None else 0.03) * float(b.norm())
+    L.fallback_reset()
+    t = torch.randn(2, 9, 16, device=DEV).transpose(1, 2)                  # neither: contiguous, as the stock operator's
+    assert GN.GroupNormAct(4, 16).to(DEV)(t).is_contiguous() and L.fallback_counts()["gn_act"] == 1
+    L.fallback_reset()
+    half = GN.GroupNormAct(4, 16).to(DEV)(torch.randn(2, 16, 9, device=DEV, dtype=torch.bfloat16))         # fp32 parameters
+    assert half.dtype == torch.bfloat16 and half.is_contiguous() and L.fallback_counts()["gn_act"] == 0

@@ -55,10 +55,12 @@ def _dtype(t, what="x"):
     return DTYPES[t.dtype]
 
 
-def transformed():
-    """is this call traced, differentiated forward, or inside a torch.func transform?  The kernels fill tensors through their addresses, which none
-    of these sees: such a call takes the stock operators (modules) or raises (functions)"""
-    return torch.jit.is_tracing() or forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
+def transformed(*tensors):
+    """is this call traced, differentiated forward (with `tensors`: is one of them a dual tensor), or inside a torch.func transform?  The kernels
+    fill tensors through their addresses, which none of these sees: such a call takes the stock operators (modules) or raises (functions)"""
+    if torch.jit.is_tracing() or torch._C._functorch.peek_interpreter_stack() is not None:
+        return True
+    return forward_ad._current_level >= 0 and (not tensors or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors))
 
 
 def no_trace(what):
@@ -66,9 +68,9 @@ def no_trace(what):
         raise L.DbevHipError(f"{what}: torch.jit.trace cannot record it (the modules trace as the stock operators)")
 
 
-def _no_derivative(what):
+def _no_derivative(what, x):
     no_trace(what)
-    if transformed():
+    if transformed(x):
         raise L.DbevHipError(f"{what}: not under forward-mode differentiation or a torch.func transform (it has no derivative)")
 
 
@@ -162,13 +164,8 @@ def _dim(x, channel_dim):
 def pack(x, fmt="int8", channel_dim=None):
     """the 8-bit checkpoint of a device tensor (no autograd).  `channel_dim`: the dimension along which the blocks of 32 run; by default
     the one that is dense in memory (`dense_dim`)."""
-    _fmt(fmt), _dtype(x)
-    _no_derivative("pack")
-    return _pack(x, fmt, channel_dim)
-
-
-def _pack(x, fmt, channel_dim):
     f, dt = _fmt(fmt), _dtype(x)
+    _no_derivative("pack", x)
     dev = L.require_cuda(x)
     dim = _dim(x, channel_dim)
     with L.on(dev):
@@ -185,7 +182,7 @@ def unpack(ck, dtype=None):
     dtype = ck.dtype if dtype is None else dtype
     if dtype not in DTYPES:
         raise L.DbevHipError(f"unpack: float32, bfloat16 or float16 expected, got {dtype}")
-    _no_derivative("unpack")
+    _no_derivative("unpack", ck.buf)
     dev = L.require_cuda(ck.buf)
     with L.on(dev):
         out = empty_dense(ck.shape, ck.dim, dtype, dev)
@@ -281,7 +278,7 @@ def weight_gradient(ck, gy, bias=False):
     """gy^T x^ [Co, Ci] (and with `bias` the sums of gy over its rows, [Co]) in gy's type, for the checkpoint of a layer's input and the
     gradient of its output: gy has the checkpoint's shape but for the channel dimension.  fp32 sums, fp32 accuracy for fp32 gy."""
     _dtype(gy, "gy")
-    _no_derivative("weight_gradient")
+    _no_derivative("weight_gradient", gy)
     dev = L.require_cuda(ck.buf, gy)
     dim, want = ck.dim, ck.shape
     if gy.dim() != len(want) or any(gy.shape[d] != want[d] for d in range(len(want)) if d != dim):
@@ -331,7 +328,7 @@ class _Linear8(Function):
                 y.add_(bias)
         else:
             y = F.linear(x2, weight, bias)
-        ck = _pack(x2, fmt, -1) if keep else None
+        ck = pack(x2, fmt, -1) if keep else None
         ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt = fmt
         return y
@@ -394,7 +391,7 @@ class _Conv1x1_8(Function):
                 y.add_(bias.view(1, -1, 1, 1))
         else:
             y = F.conv2d(x, weight, bias)
-        ck = _pack(x, fmt, 1) if keep else None
+        ck = pack(x, fmt, 1) if keep else None
         ctx.save_for_backward(weight, None if ck is None else ck.buf)
         ctx.fmt, ctx.x_shape = fmt, tuple(x.shape)
         if stats is None:

@@ -80,6 +80,9 @@ def test_forward_mode_derivatives_pass_through_the_modules_and_are_refused_by_th
                 call()
         with pytest.raises(L.DbevHipError):
             A.pack(rows)
+        plain, lw = torch.randn(6, 32, device=DEV), torch.randn(8, 32, device=DEV, requires_grad=True)
+        a = A.linear(plain, lw)                                            # (nothing here is a dual tensor)
+        assert torch.autograd.grad(a.sum(), (lw,))[0].shape == lw.shape and A.unpack(A.pack(plain)).shape == plain.shape
     jvp = torch.func.jvp(lambda v: _stock(mod, v)[0], (x,), (t,))
     assert torch.allclose(jvp[1], ref.tangent, atol=1e-5)
     params = dict(mod.named_parameters())

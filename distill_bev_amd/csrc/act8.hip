@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void a8_forward(const T* __restrict__ x, long 
     }
     if (WITH_Y && p.on) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = a8_act<ACT, T>(v[i]);
+      for (int i = 0; i < V; ++i) v[i] = a8_act<ACT>(v[i]);
       A8Vec<T, V>::template store<NT>(y + o, v);
     }
   }

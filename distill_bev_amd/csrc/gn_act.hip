@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void gn_apply(const T* __restrict__ x, GnArgs 
       }
       if (p.on) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = a8_act<ACT, T>(fmaf(v[i], sc[i], bt[i]));
+        for (int i = 0; i < V; ++i) v[i] = a8_act<ACT>(fmaf(v[i], sc[i], bt[i]));
         A8Vec<T, V>::template store<NT>(y + o, v);
       }
     }

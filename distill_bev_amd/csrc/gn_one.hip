@@ -246,7 +246,7 @@ __device__ __forceinline__ void gn_one_write(const typename GnRaw<T, V>::type* r
       }
       if (p.on) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = a8_act<ACT, T>(fmaf(v[i], sc[i], bt[i]));
+        for (int i = 0; i < V; ++i) v[i] = a8_act<ACT>(fmaf(v[i], sc[i], bt[i]));
         A8Vec<T, V>::template store<NT>(gn_at(yi, at * static_cast<unsigned>(sizeof(T))), v);
       }
     }

@@ -175,3 +175,23 @@ def test_modules_give_the_layout_that_they_were_given():
     L.fallback_reset()
     half = GN.GroupNormAct(4, 16).to(DEV)(torch.randn(2, 16, 9, device=DEV, dtype=torch.bfloat16))         # fp32 parameters
     assert half.dtype == torch.bfloat16 and half.is_contiguous() and L.fallback_counts()["gn_act"] == 0
+
+
+def test_gelu_of_every_fp16_value_is_the_neighbour_only_where_fp32_cannot_tell():
+    """q = 1 - Phi(|z|) is off by (z^2 + 16) 2^-24 of itself, y = z q or z (1 - q): wherever the exact y is further from fp16's nearest tie than
+    that (and 2 * 2^-24 for 1 - q and the product) the result is correctly rounded; these are all but one in 300 of the normal results"""
+    import math
+    from distill_bev_amd import act8 as A
+    x = torch.arange(0, 1 << 16, dtype=torch.int32).to(torch.int16).view(torch.float16)
+    x = x[torch.isfinite(x) & (x != 0)]
+    z = x.double()
+    q = 0.5 * torch.special.erfc(z.abs() / math.sqrt(2))
+    y = torch.where(z > 0, z * (1 - q), z * q)
+    ok = (y.abs() >= 2.0 ** -14) & (y.abs() < 65504)
+    x, z, q, y = x[ok], z[ok], q[ok], y[ok]
+    m = torch.frexp(y.abs())[0] * 2048
+    tie = (m - torch.floor(m) - 0.5).abs() / m
+    err = torch.where(z > 0, q / (1 - q), torch.ones_like(q)) * (z * z + 16) * 2.0 ** -24 + 2 * 2.0 ** -24
+    sure = tie > err
+    assert float(sure.double().mean()) > 1 - 1 / 300
+    assert torch.equal(A.activation(x.to(DEV), "gelu").cpu()[sure], y.half()[sure])

@@ -35,6 +35,7 @@ FORMATS = {"int8": 1, "e4m3": 2}                               # DBEV_ACT8_*
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}            # DBEV_ACT_*
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # DBEV_DT_*
 BLOCK = 32
+_tracing_state, _transform_stack = torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack      # None outside
 
 
 def _fmt(fmt):
@@ -58,13 +59,13 @@ def _dtype(t, what="x"):
 def transformed(*tensors):
     """is this call traced, differentiated forward (with `tensors`: is one of them a dual tensor), or inside a torch.func transform?  The kernels
     fill tensors through their addresses, which none of these sees: such a call takes the stock operators (modules) or raises (functions)"""
-    if torch.jit.is_tracing() or torch._C._functorch.peek_interpreter_stack() is not None:
+    if _tracing_state() is not None or _transform_stack() is not None:
         return True
     return forward_ad._current_level >= 0 and (not tensors or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors))
 
 
 def no_trace(what):
-    if torch.jit.is_tracing():
+    if _tracing_state() is not None:
         raise L.DbevHipError(f"{what}: torch.jit.trace cannot record it (the modules trace as the stock operators)")
 
 

@@ -23,6 +23,14 @@ __device__ __forceinline__ int gn_rows(const GnArgs& a, int chunk) {
   return (a.tiles_each + (chunk < a.extra ? 1 : 0)) * (a.t.RP * GN_U) - (chunk == a.last ? a.lack : 0);
 }
 
+// ... of them, those of row phase rp
+__device__ __forceinline__ int gn_phase_rows(const GnArgs& a, int chunk, int rp) {
+  const int n = (a.tiles_each + (chunk < a.extra ? 1 : 0)) * GN_U;
+  if (chunk != a.last) return n;
+  const int left = a.t.RP * GN_U - a.lack - rp;               // pixels of the image's last tile from this phase on
+  return n - GN_U + (left > 0 ? (left + a.t.RP - 1) / a.t.RP : 0);
+}
+
 // (image, pixel chunk, column range) of this workgroup
 struct GnPos { int n, chunk, cc, col, c0, c1, g0, g1, rp; bool on; long long r0, step; };
 __device__ __forceinline__ GnPos gn_pos(const GnArgs& a, int block, int V) {

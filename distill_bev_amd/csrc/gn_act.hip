@@ -3,10 +3,10 @@
 //
 // (Small images go through gn_small_fwd, large batches through gn_one_*, gn_one.hip.)
 // Forward, two launches, no finalize launch between them:
-//   gn_stats   a workgroup owns a chunk of one image's pixels x a range of channels, a thread one vector column; sums of (x - K_c) and
-//              (x - K_c)^2 with K_c the chunk's first pixel: an offset of the data costs no digits (and an outlier there, whose own
-//              square is in the sum, some rows * 2^-24 of it).  Reduced to (mean, M2) per group
-//              and chunk in LDS.
+//   gn_stats   a workgroup owns a chunk of one image's pixels x a range of channels, a thread one vector column: (mean, M2) of x - K_c, K_c
+//              the chunk's first pixel, so that an offset of the data costs no digits.  Four rows at a time: their own mean, the squares
+//              about it, merged with those before (M2 += M2_4 + delta^2 n 4 / (n + 4)): M2 is a sum of positive terms, wherever K_c and
+//              outliers are.  Reduced to (mean, M2) per group and chunk in LDS.
 //   gn_apply   every workgroup merges its image's chunk statistics itself -- a few KB from L2 against its share of x -- in fp64
 //              (M2 = sum of M2_i + n_i (mean_i - mean)^2), then y, and the checkpoint from the same registers.
 // Backward, two launches, xh = (x - mean) rstd, g = dy act'(gamma xh + beta):
@@ -14,7 +14,7 @@
 //   gn_bwd_dx       dx = rstd (gamma g - A / D - xh B / D), D = S C / G; its first workgroups add the per-channel rows up instead
 // Bound by HBM: 3 n es forward and 5 n es backward (n es = bytes of x; with a checkpoint the two reads of x in the backward are 1.03
 // bytes a value).  All sums have a fixed order: run-to-run bit-identical, no atomics.
-// Measured, fp32, SiLU: 1 x 128 x 1024 x 1024 forward 280 us (1.6 GB in three passes: 5.8 TB/s, part of the second read comes from the
+// Measured, fp32, SiLU: 1 x 128 x 1024 x 1024 forward 290 us (1.6 GB in three passes: 5.6 TB/s, part of the second read comes from the
 // memory-side cache), backward 446; 8 x 128 x 128 x 128, int8 kept: 28 + 28 and 24 + 27 us, half of it cache; 6 x 256 x 15 x 25 backward: 7 + 7
 // us, launch and merge latency.
 #include "gn_act.h"
@@ -27,38 +27,83 @@ __global__ __launch_bounds__(256) void gn_stats(const T* __restrict__ x, GnArgs 
   extern __shared__ float sh[];
   const GnPos p = gn_pos(a, blockIdx.x, V);
   const T* xi = x + static_cast<size_t>(p.n) * a.S * a.C + static_cast<size_t>(p.on ? p.col : 0) * V;
-  float k[V], s[V], q[V];
+  float k[V], m[V], q[V];                                     // offset; mean - offset and M2 of the rows so far
 #pragma unroll
-  for (int i = 0; i < V; ++i) k[i] = s[i] = q[i] = 0.f;
+  for (int i = 0; i < V; ++i) k[i] = m[i] = q[i] = 0.f;
   if (p.on) {
     A8Vec<T, V>::get(A8Vec<T, V>::load(xi + p.r0 * a.C), k);
+    float n = 0.f;
     for (long long r = p.r0 + p.rp; r < a.S; r += p.step) {
       typename A8Vec<T, V>::Raw raw[GN_U];
 #pragma unroll
       for (int u = 0; u < GN_U; ++u) raw[u] = A8Vec<T, V>::load(xi + min(r + u * a.t.RP, a.S - 1) * a.C);
+      float d[GN_U][V];
 #pragma unroll
       for (int u = 0; u < GN_U; ++u) {
-        if (r + u * a.t.RP >= a.S) break;
-        float v[V];
-        A8Vec<T, V>::get(raw[u], v);
+        A8Vec<T, V>::get(raw[u], d[u]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[u][i] -= k[i];
+      }
+      const bool full = r + (GN_U - 1) * a.t.RP < a.S;
+      const float nb = full ? static_cast<float>(GN_U) : static_cast<float>((a.S - r + a.t.RP - 1) / a.t.RP);
+      const float f = nb * __builtin_amdgcn_rcpf(n + nb), nf = n * f;
+      const auto batch = [&](bool all, float inv) {           // (two bodies: only an image's last tile has rows to leave out)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = v[i] - k[i];
-          s[i] += d;
-          q[i] = fmaf(d, d, q[i]);
+          float sum = 0.f, sq = 0.f;
+#pragma unroll
+          for (int u = 0; u < GN_U; ++u) sum += all || u < nb ? d[u][i] : 0.f;
+          const float mb = sum * inv, delta = mb - m[i];
+#pragma unroll
+          for (int u = 0; u < GN_U; ++u) {
+            const float e = d[u][i] - mb;
+            sq = all || u < nb ? fmaf(e, e, sq) : sq;
+          }
+          q[i] += fmaf(delta * delta, nf, sq);
+          m[i] = fmaf(delta, f, m[i]);
         }
-      }
+      };
+      if (full) batch(true, 1.f / GN_U);
+      else batch(false, __builtin_amdgcn_rcpf(nb));
+      n += nb;
     }
   }
-  gn_fold<V>(sh, a, p, s, q);
-  // per channel: mean and M2 of the chunk's pixels
-  const int w = a.t.CH * V;
+  // per channel: the row phases merged the same way, mean and M2 of the chunk's pixels in sh[0 .. CH V), sh[CH V ..)
+  const int w = a.t.CH * V, lane = threadIdx.x - p.rp * a.t.CH;
+  float *t1 = sh + 2 * w, *t2 = t1 + a.t.RP * w;
+  if (p.rp < a.t.RP) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      t1[p.rp * w + lane * V + i] = m[i];
+      t2[p.rp * w + lane * V + i] = q[i];
+    }
+  }
+  __syncthreads();
   const float rows = static_cast<float>(gn_rows(a, p.chunk));
   const T* x0 = x + static_cast<size_t>(p.n) * a.S * a.C + p.r0 * a.C + p.c0;
+  const float each = static_cast<float>(gn_phase_rows(a, p.chunk, 0));
+  const bool even = p.chunk != a.last;                        // all phases have as many rows
   for (int c = threadIdx.x; c < p.c1 - p.c0; c += blockDim.x) {
-    const float d = sh[c] / rows;
-    sh[w + c] = fmaxf(sh[w + c] - sh[c] * d, 0.f) + 0.f * d;  // (a NaN stays one)
-    sh[c] = static_cast<float>(x0[c]) + d;
+    float mean = 0.f, m2 = 0.f;
+    if (even) {
+#pragma unroll 4
+      for (int r = 0; r < a.t.RP; ++r) mean += t1[r * w + c];
+      mean /= static_cast<float>(a.t.RP);
+#pragma unroll 4
+      for (int r = 0; r < a.t.RP; ++r) {
+        const float e = t1[r * w + c] - mean;
+        m2 += fmaf(each * e, e, t2[r * w + c]);
+      }
+    } else {
+      for (int r = 0; r < a.t.RP; ++r) mean = fmaf(static_cast<float>(gn_phase_rows(a, p.chunk, r)), t1[r * w + c], mean);
+      mean /= rows;
+      for (int r = 0; r < a.t.RP; ++r) {
+        const float e = t1[r * w + c] - mean;
+        m2 += fmaf(static_cast<float>(gn_phase_rows(a, p.chunk, r)) * e, e, t2[r * w + c]);
+      }
+    }
+    sh[c] = static_cast<float>(x0[c]) + mean;
+    sh[w + c] = m2;
   }
   __syncthreads();
   const int ng = p.g1 - p.g0, lanes = gn_lanes(ng), sub = threadIdx.x % lanes;

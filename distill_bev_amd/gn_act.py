@@ -128,10 +128,8 @@ class _GroupNormAct8(_GroupNormAct):
         return _gradients(ctx, gy)
 
 
-def _fits(x):
+def _fits(N, C, S):
     """the kernels' limits (dbev_gn_act_workspace_bytes has the same)"""
-    N, C = x.shape[:2]
-    S = x.numel() // (N * C) if x.numel() else 0
     return C <= 1 << 16 and N <= 1 << 22 and S <= 1 << 30 and S * C <= 1 << 36
 
 
@@ -139,7 +137,9 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     """act(F.group_norm(x, num_groups, weight, bias, eps)) for a device tensor x [N, C, *], act one of act8.ACTS; the result is
     channels-last.  `checkpoint` ("int8" / "e4m3"): under autograd the 8-bit checkpoint of x is kept instead of x, and the gradients are
     those of the formula with x^ in place of x (mean and rstd stay x's own)."""
-    A.no_trace("group_norm_act")
+    special = A.transformed()
+    if special:
+        A.no_trace("group_norm_act")
     A._act(act)
     if checkpoint is not None:
         A._fmt(checkpoint)
@@ -154,15 +154,17 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.shape != (C,) or t.dtype not in A.DTYPES):
             raise ValueError(f"group_norm_act: {name} {tuple(t.shape)} {t.dtype} for {C} channels")
-    if not _fits(x):
+    S = x.numel() // (N * C) if N else 0
+    if not _fits(N, C, S):
         raise L.DbevHipError(f"group_norm_act: {N} images of {C} channels, {tuple(x.shape)}; at most 2^22 and 2^16, of 2^30 pixels and 2^36 values")
     if not eps >= 0:
         raise ValueError(f"group_norm_act: eps {eps}")
-    if x.numel() and x.numel() // G == 1:                         # F.group_norm's own refusal
+    if N * S * C == G:                                            # F.group_norm's own refusal
         raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
-    if A._recording(x, weight, bias) or A.transformed():          # (transformed: the function raises)
+    if special or torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                               or (bias is not None and bias.requires_grad)):
         x = _maps(x)[0]                                               # (a copy of another layout is a step of the graph by itself)
-        return (_GroupNormAct8 if checkpoint else _GroupNormAct).apply(x, weight, bias, G, float(eps), act, checkpoint)
+        return (_GroupNormAct8 if checkpoint else _GroupNormAct).apply(x, weight, bias, G, float(eps), act, checkpoint)     # (raises if special)
     with L.on(dev):
         xd, N, C, S = _maps(x.detach())
         return _forward(xd, N, C, S, G, _f32(weight), _f32(bias), float(eps), act, None, False)[0]
@@ -176,7 +178,7 @@ def _ready(x, gn):
         why = f"dtype {x.dtype}"
     elif torch.is_autocast_enabled("cuda"):
         why = "autocast"
-    elif not _fits(x):
+    elif not _fits(x.shape[0], x.shape[1], x.numel() // (x.shape[0] * x.shape[1])):
         why = f"size {tuple(x.shape)}"
     elif A.transformed():
         why = "traced or transformed"

@@ -109,9 +109,10 @@ __global__ __launch_bounds__(256) void gn_stats(const T* __restrict__ x, GnArgs 
   const int ng = p.g1 - p.g0, lanes = gn_lanes(ng), sub = threadIdx.x % lanes;
   for (int gi = threadIdx.x / lanes; gi < ng; gi += blockDim.x / lanes) {
     const int g = p.g0 + gi, cb = max(p.c0, g * a.cpg) - p.c0, ce = min(p.c1, (g + 1) * a.cpg) - p.c0;
+    const float ref = sh[cb];                                 // (sums of offsets would cost digits)
     float m = 0.f;
-    for (int c = cb + sub; c < ce; c += lanes) m += sh[c];
-    m = gn_lane_sum(m, lanes) / static_cast<float>(ce - cb);
+    for (int c = cb + sub; c < ce; c += lanes) m += sh[c] - ref;
+    m = ref + gn_lane_sum(m, lanes) / static_cast<float>(ce - cb);
     float m2 = 0.f;
     for (int c = cb + sub; c < ce; c += lanes) {
       const float d = sh[c] - m;

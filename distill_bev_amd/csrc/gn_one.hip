@@ -78,6 +78,19 @@ template <typename T>
 __device__ __forceinline__ T* gn_at(T* image, unsigned bytes) {
   return reinterpret_cast<T*>(reinterpret_cast<char*>(const_cast<typename std::remove_const<T>::type*>(image)) + bytes);
 }
+// groups of a thread's V channels: one division where groups are whole vectors
+template <int V>
+__device__ __forceinline__ void gn_groups(const GnArgs& a, const GnOnePos& p, int* g) {
+  const int first = p.on ? p.col * V : 0;
+  if (a.cpg % V == 0) {
+    g[0] = first / a.cpg;
+#pragma unroll
+    for (int i = 1; i < V; ++i) g[i] = g[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] = (first + i) / a.cpg;
+  }
+}
 template <typename T, int V> struct GnRaw {                   // one 16-byte vector as dwords
   typedef unsigned type __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ void get(type t, float* v) { A8Vec<T, V>::get(__builtin_bit_cast(typename A8Vec<T, V>::Raw, t), v); }
@@ -217,11 +230,13 @@ __device__ __forceinline__ void gn_one_write(const typename GnRaw<T, V>::type* r
   constexpr int LB = 32 / V;
   const GnArgs& a = o.a;
   float sc[V], bt[V];
+  int gr[V];
+  gn_groups<V>(a, p, gr);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = p.on ? p.col * V + i : 0, g = c / a.cpg;
-    sc[i] = out[2 * g + 1] * (gamma != nullptr ? gamma[c] : 1.f);
-    bt[i] = fmaf(-out[2 * g], sc[i], beta != nullptr ? beta[c] : 0.f);
+    const int c = p.on ? p.col * V + i : i;
+    sc[i] = out[2 * gr[i] + 1] * (gamma != nullptr ? gamma[c] : 1.f);
+    bt[i] = fmaf(-out[2 * gr[i]], sc[i], beta != nullptr ? beta[c] : 0.f);
   }
   const size_t image = static_cast<size_t>(p.n) * a.S;
   T* yi = y + image * a.C;
@@ -268,32 +283,50 @@ __device__ __forceinline__ void gn_one_load(typename GnRaw<T, V>::type* raw, con
   }
 }
 
-// the tile's mean per group, then the squares about it, both from the registers: done(g, mean, M2) by one thread a group, out[2 g] = mean
+// the tile's mean per group, then the squares about it, both from the registers: done(g, mean, M2) by one thread a group, out[2 g] = mean.  x0: the
+// tile's first pixel.  Its value in a group's first channel is taken off every thread's sum, so that the sums over threads are of numbers of the
+// spread's size whatever offset the data have: an offset of 1000 spreads costs the mean its last rounding (and every thread's sum of 16
+// rows, which averages out), not those of a sum over all
 template <typename T, int V, int R, typename F>
-__device__ __forceinline__ void gn_one_stats(typename GnRaw<T, V>::type* raw, float* sh, float* out, const GnArgs& a, const GnOnePos& p, int rows, F done) {
+__device__ __forceinline__ void gn_one_stats(typename GnRaw<T, V>::type* raw, const T* x0, float* sh, float* out, const GnArgs& a, const GnOnePos& p,
+                                             int rows, F done) {
   const int lanes = gn_lanes(a.G), sub = threadIdx.x % lanes;
-  float s[V];
+  float s[V], ref[V];
+  int gr[V];
+  gn_groups<V>(a, p, gr);
+  if (a.cpg % V == 0) {
+    ref[0] = static_cast<float>(x0[gr[0] * a.cpg]);
+#pragma unroll
+    for (int i = 1; i < V; ++i) ref[i] = ref[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) ref[i] = static_cast<float>(x0[gr[i] * a.cpg]);
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = 0.f;
 #pragma unroll
-  for (int u = 0; u < R; ++u) {                               // (rows past the end are zeros)
-    float v[V];
+  for (int u = 0; u < R; u += 2) {                            // (rows past the end are zeros)
+    float v[V], v2[V];
     GnRaw<T, V>::get(raw[u], v);
+    GnRaw<T, V>::get(raw[u + 1], v2);
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] += v[i];
+    for (int i = 0; i < V; ++i) s[i] += v[i] + v2[i];
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = fmaf(-static_cast<float>(p.nv), ref[i], s[i]);
   gn_one_fold<V, 1>(sh, a, p, s, s);
   for (int g = threadIdx.x / lanes; g < a.G; g += blockDim.x / lanes) {
+    const float r = static_cast<float>(x0[g * a.cpg]);
     float m = 0.f;
     for (int c = sub; c < a.cpg; c += lanes) m += sh[g * a.cpg + c];
     m = gn_lane_sum(m, lanes);
-    if (sub == 0) out[2 * g] = m / (static_cast<float>(rows) * static_cast<float>(a.cpg));
+    if (sub == 0) out[2 * g] = r + m / (static_cast<float>(rows) * static_cast<float>(a.cpg));
   }
   __syncthreads();
   float mu[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    mu[i] = out[2 * ((p.on ? p.col * V + i : 0) / a.cpg)];
+    mu[i] = out[2 * gr[i]];
     s[i] = 0.f;
   }
 #pragma unroll
@@ -329,7 +362,8 @@ __global__ __launch_bounds__(256, 4) void gn_one_fwd(const T* __restrict__ x, Gn
   float* out = gn_one_out<V>(sh, a);
   typename GnRaw<T, V>::type raw[R];
   gn_one_load<T, V, R, true>(raw, x, a, p);
-  gn_one_stats<T, V, R>(raw, sh, out, a, p, min(a.t.RP * R, static_cast<int>(a.S) - p.t * (a.t.RP * R)),
+  const int r0 = p.t * (a.t.RP * R);
+  gn_one_stats<T, V, R>(raw, x + (static_cast<size_t>(p.n) * a.S + r0) * a.C, sh, out, a, p, min(a.t.RP * R, static_cast<int>(a.S) - r0),
                         [&](int g, float m, float m2) { gn_publish(o.b.part + (static_cast<size_t>(p.n) * a.G + g) * o.T + p.t, m, m2); });
   if (!gn_one_totals<true, R>(out, o, p, eps, mean, rstd)) return;
 #pragma unroll
@@ -355,7 +389,7 @@ __global__ __launch_bounds__(256, 4) void gn_small_fwd(const T* __restrict__ x, 
   typename GnRaw<T, V>::type raw[R];
   gn_one_load<T, V, R, false>(raw, x + c0, a, p);
   const double D = static_cast<double>(a.S) * a.cpg;
-  gn_one_stats<T, V, R>(raw, sh, out, a, p, static_cast<int>(a.S), [&](int g, float m, float m2) {
+  gn_one_stats<T, V, R>(raw, x + c0 + static_cast<size_t>(n) * a.S * a.C, sh, out, a, p, static_cast<int>(a.S), [&](int g, float m, float m2) {
     const float r = static_cast<float>(1.0 / sqrt(m2 / D + static_cast<double>(eps)));
     out[2 * g + 1] = r;
     if (mean != nullptr) {
@@ -450,11 +484,13 @@ __device__ __forceinline__ void gn_one_grad(float (*g)[V], typename GnKept<T, V,
       kept[u] = GnKept<T, V, FMT>::load(xi, ci, m.at + u * m.step);
     }
   float mu[V], rs[V], sc[V], bt[V];
+  int gr[V];
+  gn_groups<V>(a, p, gr);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = p.on ? p.col * V + i : 0, gr = c / a.cpg;
-    mu[i] = k.mean[static_cast<size_t>(p.n) * a.G + gr];
-    rs[i] = k.rstd[static_cast<size_t>(p.n) * a.G + gr];
+    const int c = p.on ? p.col * V + i : i;
+    mu[i] = k.mean[static_cast<size_t>(p.n) * a.G + gr[i]];
+    rs[i] = k.rstd[static_cast<size_t>(p.n) * a.G + gr[i]];
     sc[i] = rs[i] * (k.gamma != nullptr ? k.gamma[c] : 1.f);
     bt[i] = k.beta != nullptr ? k.beta[c] : 0.f;
     s[i] = q[i] = 0.f;
@@ -486,14 +522,16 @@ __device__ __forceinline__ void gn_one_dx(const float (*g)[V], typename GnKept<T
   T* di = dx + m.row * a.C;
   const uint8_t* si = FMT == DBEV_ACT8_NONE ? nullptr : scales + m.row * a.nb;
   float mu[V], sc[V], A[V], B[V];                             // dx = sc g - (rstd A) - (x - mean) (rstd^2 B), sc = rstd gamma
+  int gr[V];
+  gn_groups<V>(a, p, gr);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = p.col * V + i, gr = c / a.cpg;
-    const float rs = k.rstd[static_cast<size_t>(p.n) * a.G + gr];
-    mu[i] = k.mean[static_cast<size_t>(p.n) * a.G + gr];
+    const int c = p.col * V + i;
+    const float rs = k.rstd[static_cast<size_t>(p.n) * a.G + gr[i]];
+    mu[i] = k.mean[static_cast<size_t>(p.n) * a.G + gr[i]];
     sc[i] = rs * (k.gamma != nullptr ? k.gamma[c] : 1.f);
-    A[i] = rs * out[2 * gr];
-    B[i] = rs * rs * out[2 * gr + 1];
+    A[i] = rs * out[2 * gr[i]];
+    B[i] = rs * rs * out[2 * gr[i] + 1];
   }
 #pragma unroll
   for (int u = 0; u < R; ++u) {

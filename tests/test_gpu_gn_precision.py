@@ -39,3 +39,32 @@ def test_an_outlier_in_the_first_pixel(N, S, H, C, G, size):
     ref = _reference(x, G, w, b)
     rel = ((y - ref).abs() / (ref - b.double()).abs())[:, 0]
     assert float(rel.max()) < 55 * 2.0 ** -24, float(rel.max())
+
+
+def _mean(x, G):
+    """the mean that the forward pass keeps, [N, G], of x [N, S, C] on the device"""
+    from distill_bev_amd import _lib as L
+    N, S, C = x.shape
+    y, st = torch.empty_like(x), torch.empty((2, N, G), device=DEV)
+    ws = torch.empty((int(L.call("dbev_gn_act_workspace_bytes", N, S, C, G)),), dtype=torch.uint8, device=DEV)
+    L.call("dbev_gn_act_forward", x.data_ptr(), 0, N, S, C, G, None, None, 1e-5, 0, y.data_ptr(), st[0].data_ptr(), st[1].data_ptr(), 0, None, None,
+           ws.data_ptr(), ws.numel(), L.raw_stream(DEV))
+    return st[0], y
+
+
+@pytest.mark.parametrize("N,S,C,G,roundings", [(2, 500, 64, 8, 1), (6, 176, 256, 32, 1), (12, 11440, 256, 32, 2), (40, 4200, 64, 8, 2), (2, 3000, 64, 8, 3),
+                                               (1, 9000, 30, 2, 3)])
+def test_large_offsets_leave_the_mean_its_digits(N, S, C, G, roundings):
+    """mean / spread = 1000, a step of the mean is 2^-14 spreads: one rounding, 2^-15, where a workgroup holds the image; one in every tile and
+    one behind their sum in the one-pass form; one of a channel's mean, one of the group's, one of all chunks' in the two launches.
+    A thread of the first two forms adds up 16 rows of its channels, in pairs, and takes the offset off the sum: eight roundings of sums up to
+    16000, root mean square 3.8e-5 of a row, independent over the 32 or more threads and channels that a group has: 7e-6, two
+    of them 2^-16 (the tiles' average out).  Everything else is computed on differences of the size of the spread"""
+    x = torch.randn(N, S, C, generator=torch.Generator().manual_seed(3)).add_(1000.0).to(DEV)
+    mean, y = _mean(x, G)
+    ref = x.double().view(N, S, G, C // G).mean((1, 3))
+    assert float((mean.double() - ref).abs().max()) <= roundings * 2.0 ** -15 + 2.0 ** -16
+    # y: that, times rstd, and the rounding of mean * rstd, which may be beyond 1024, in its constant term
+    z = x.double().view(N, S, G, C // G)
+    z = (z - ref[:, None, :, None]) / torch.sqrt(z.var((1, 3), correction=0, keepdim=True) + 1e-5)
+    assert float((y.double() - z.view(N, S, C)).abs().max()) <= 1.1 * (roundings * 2.0 ** -15 + 2.0 ** -16) + 2.0 ** -14 + 2.0 ** -18

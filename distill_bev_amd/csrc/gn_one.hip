@@ -744,11 +744,12 @@ size_t gn_one_bytes(int N, long long S, int C, int G) {
     default: { typedef a8_f16 T; constexpr int V = 8; __VA_ARGS__; break; }             \
   }
 
-// Small images: W channels (whole groups, whole blocks of 32, or all of them), at most GN_RF rows a thread (fp32, 32 channels: 512 pixels);
-// wider while every thread still has a row of its own.  Against the two launches, SiLU, us on the GPU: fp32 6 x 256 x 8 x 22 7.1 (11.2), 6 x 256
-// x 15 x 25 7.7 (11.7), 48 x 512 x 22 x 22 17.9 (33.7), 200 x 256 x 16 x 32 35 (58: 210 MB at 6 TB/s); bf16 9.0 (13.5), 9.7 (13.8), 19.4 (26.9), 33
-// (44); 40000 images of one pixel, 256 channels: 228 (229), bf16 406 (388)
-bool gn_small_plan(int dtype, long long S, int C, int G, int vec, GnArgs* a, int* W) {
+// Small images: W channels (whole groups, whole blocks of 32, or all of them), at most GN_RF rows a thread (fp32, 32 channels: 512 pixels); wider
+// while every thread still has a row of its own, and, with several rows a thread, while two workgroups a CU remain (5000 x 256 x 4 x 4, fp32 /
+// bf16: 109 / 112 us with 64 channels a workgroup, 37 / 62 with all; 500 x 256 x 8 x 8 27 / 43 -> 14 / 17).  Against the two launches, without an
+// activation, us a call: fp32 6 x 256 x 8 x 22 13 (16), 48 x 512 x 22 x 22 18 (34), 200 x 256 x 16 x 32 35 (60), 1000 x 256 x 4 x 4 14 (17), 5000 x 256 x 4 x 4
+// 37 (58), 40000 images of one pixel 195 (272); bf16 13 (16), 19 (27), 37 (48), 15 (22), 62 (84), 399 (460)
+bool gn_small_plan(int dtype, int N, long long S, int C, int G, int vec, GnArgs* a, int* W) {
   const int wide = dtype == DBEV_DT_F32 ? 4 : 8, cpg = C / G;
   if (vec != wide || S > 256 * GN_RF) return false;
   int unit = cpg;
@@ -756,7 +757,8 @@ bool gn_small_plan(int dtype, long long S, int C, int G, int vec, GnArgs* a, int
   if (unit > C) unit = C;
   for (int w = unit;; w = 2 * w < C ? 2 * w : C) {
     const A8Tile t = a8_tile(w, wide);
-    if (t.ncol != 1 || S > static_cast<long long>(t.RP) * (w == unit ? GN_RF : 1)) break;
+    const bool many = static_cast<long long>(N) * ((C + w - 1) / w) >= 512;
+    if (t.ncol != 1 || S > static_cast<long long>(t.RP) * (w == unit || many ? GN_RF : 1)) break;
     a->t = t;
     *W = w;
     if (w == C) return true;
@@ -768,7 +770,7 @@ bool gn_small_forward(const void* x, int dtype, int vec, int N, long long S, int
                       void* y, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales, hipStream_t st) {
   GnOneArgs o;
   int W;
-  if (!gn_small_plan(dtype, S, C, G, vec, &o.a, &W)) return false;
+  if (!gn_small_plan(dtype, N, S, C, G, vec, &o.a, &W)) return false;
   const int nblk = (C + W - 1) / W;
   if (static_cast<long long>(N) * nblk * o.a.t.threads >= (1LL << 32)) return false;
   o.a = gn_one_args(o.a, S, C, G, vec);

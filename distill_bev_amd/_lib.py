@@ -177,6 +177,7 @@ _SIGNATURES = {
     "dbev_act8_weight_gradient_workspace_bytes": [_ll, _i, _i],
     "dbev_act8_weight_gradient": [_p, _i, _p, _p, _i, _ll, _i, _i, _p, _p, _p, _sz, _p],
     "dbev_gn_act_workspace_bytes": [_i, _ll, _i, _i],
+    "dbev_gn_act_form": [_i, _i, _ll, _i, _i, _i, _i],
     "dbev_gn_act_poll_limit": [_i],
     "dbev_gn_act_forward": [_p, _i, _i, _ll, _i, _i, _p, _p, _f, _i, _p, _p, _p, _i, _p, _p, _p, _sz, _p],
     "dbev_gn_act_backward": [_p, _i, _p, _i, _p, _p, _i, _ll, _i, _i, _p, _p, _p, _p, _i, _p, _p, _p, _p, _sz, _p],
@@ -213,7 +214,7 @@ _RESTYPES = {"dbev_target_arch": ctypes.c_char_p,
              "dbev_dcnv2_col2im_workspace_bytes": ctypes.c_size_t,
              "dbev_abs_mean_maps_nhwc_workspace_bytes": ctypes.c_size_t,
              "dbev_fgd_masked_mse_nhwc_workspace_bytes": ctypes.c_size_t}
-_NO_CHECK = set(_RESTYPES) | {"dbev_adapt_mse_map_slices", "dbev_conv1x1_stats_rows", "dbev_wino_conv3x3_stats_rows", "dbev_wino_conv3x3_forward_kernel", "dbev_gemm1x1_stats_rows", "dbev_gemm_bf16x6_stats_rows", "dbev_gn_act_poll_limit"}
+_NO_CHECK = set(_RESTYPES) | {"dbev_adapt_mse_map_slices", "dbev_conv1x1_stats_rows", "dbev_wino_conv3x3_stats_rows", "dbev_wino_conv3x3_forward_kernel", "dbev_gemm1x1_stats_rows", "dbev_gemm_bf16x6_stats_rows", "dbev_gn_act_poll_limit", "dbev_gn_act_form"}
 
 
 class DbevHipError(RuntimeError):

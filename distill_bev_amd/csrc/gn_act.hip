@@ -452,6 +452,12 @@ extern "C" size_t dbev_gn_act_workspace_bytes(int N, long long S, int C, int G) 
   return gn_ws(N, S, C, G);
 }
 
+extern "C" int dbev_gn_act_form(int dtype, int N, long long S, int C, int G, int fmt, int backward) {
+  if (!gn_ok(dtype, N, S, C, G) || !(fmt == DBEV_ACT8_NONE || a8_fmt_ok(fmt)) || N == 0 || S == 0) return -1;
+  if (!backward && gn_small_takes(dtype, N, S, C, G)) return 1;
+  return gn_one_takes(dtype, N, S, C, fmt, backward != 0) ? 2 : 0;
+}
+
 extern "C" int dbev_gn_act_forward(const void* x, int dtype, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps,
                                    int act, void* y, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales, void* workspace,
                                    size_t workspace_bytes, dbevStream_t stream) {

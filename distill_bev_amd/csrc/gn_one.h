@@ -5,6 +5,9 @@
 #include <stdint.h>
 
 __attribute__((visibility("hidden"))) size_t gn_one_bytes(int N, long long S, int C, int G);
+// would the one-launch form of small images / the one-pass form take 16-byte aligned tensors of this size?
+__attribute__((visibility("hidden"))) bool gn_small_takes(int dtype, int N, long long S, int C, int G);
+__attribute__((visibility("hidden"))) bool gn_one_takes(int dtype, int N, long long S, int C, int fmt, bool backward);
 __attribute__((visibility("hidden"))) bool gn_one_forward(const void* x, int dtype, int vec, int N, long long S, int C, int G, const float* gamma,
                                                           const float* beta, float eps, int act, void* y, float* mean, float* rstd, int fmt,
                                                           uint8_t* codes, uint8_t* scales, void* ws, hipStream_t st);

@@ -766,6 +766,21 @@ bool gn_small_plan(int dtype, int N, long long S, int C, int G, int vec, GnArgs*
   return a8_tile(unit, wide).ncol == 1 && S <= static_cast<long long>(a8_tile(unit, wide).RP) * GN_RF;
 }
 
+static int gn_one_vec(int dtype, int C) {
+  const int wide = dtype == DBEV_DT_F32 ? 4 : 8;
+  return C % wide == 0 ? wide : 0;
+}
+bool gn_small_takes(int dtype, int N, long long S, int C, int G) {
+  GnArgs a;
+  int W;
+  return gn_small_plan(dtype, N, S, C, G, gn_one_vec(dtype, C), &a, &W) && static_cast<long long>(N) * ((C + W - 1) / W) * a.t.threads < (1LL << 32);
+}
+bool gn_one_takes(int dtype, int N, long long S, int C, int fmt, bool backward) {
+  GnArgs a;
+  int T;
+  return !(backward && dtype != DBEV_DT_F32) && gn_one_plan(dtype, N, S, C, gn_one_vec(dtype, C), backward ? gn_rb(fmt) : GN_RF, &a, &T);
+}
+
 bool gn_small_forward(const void* x, int dtype, int vec, int N, long long S, int C, int G, const float* gamma, const float* beta, float eps, int act,
                       void* y, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales, hipStream_t st) {
   GnOneArgs o;

@@ -983,6 +983,9 @@ int dbev_act8_weight_gradient(const void* gy, int dtype, const uint8_t* codes, c
  *   Fixed summation order.  Workspace: dbev_gn_act_workspace_bytes (0: unsupported sizes), asked with the call's device current.
  * ---------------------------------------------------------------------------------- */
 size_t dbev_gn_act_workspace_bytes(int N, long long S, int C, int G);
+/* The form that 16-byte aligned tensors of a size take on the current device: 0 two launches, 1 one launch of small images (forward), 2 one
+ * pass over the data; -1 unsupported. */
+int dbev_gn_act_form(int dtype, int N, long long S, int C, int G, int fmt, int backward);
 /* Large batches are done in one pass over the data, where workgroups wait -- a bounded number of looks -- for their image's sums and a further
  * launch finishes what did not get them in time.  Sets that number (process-wide; < 0: leaves it) and returns the one before; 0 sends every
  * tile that is not the last of its image the long way (for tests).  The results are the same bits. */

@@ -17,6 +17,9 @@ struct GnArgs {
   int lack;                                                   // pixels missing from that tile
   A8Tile t;
 };
+// Entries of a chunk's row of per-group numbers: a group that crosses a border of column ranges has one in each.  Entry g + cc for group g in
+// range cc: neighbouring ranges share at most their border's group, so that no two are the same
+__host__ __device__ __forceinline__ int gn_row(const GnArgs& a) { return a.G + a.t.ncol - 1; }
 __host__ __device__ __forceinline__ long long gn_tile(const GnArgs& a) { return static_cast<long long>(a.t.RP) * GN_U; }
 // pixels of a chunk
 __device__ __forceinline__ int gn_rows(const GnArgs& a, int chunk) {

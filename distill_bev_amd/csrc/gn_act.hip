@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void gn_stats(const T* __restrict__ x, GnArgs 
       m2 += fmaf(rows * d, d, sh[w + c]);
     }
     m2 = gn_lane_sum(m2, lanes);
-    if (sub == 0) part[((static_cast<size_t>(p.n) * a.nchunk + p.chunk) * a.t.ncol + p.cc) * a.G + g] = make_float2(m, m2);
+    if (sub == 0) part[(static_cast<size_t>(p.n) * a.nchunk + p.chunk) * gn_row(a) + g + p.cc] = make_float2(m, m2);
   }
 }
 
@@ -133,7 +133,7 @@ __device__ __forceinline__ float* gn_gather(float* sh, const GnArgs& a, const Gn
   float* out = sh + 4 * blockDim.x;
   const int ng = p.g1 - p.g0, w = a.t.CH * V;
   const int wide = min(ng, static_cast<int>(blockDim.x)), ph = threadIdx.x / wide, np = blockDim.x / wide;
-  const float2* image = part + static_cast<size_t>(p.n) * a.nchunk * a.t.ncol * a.G;
+  const float2* image = part + static_cast<size_t>(p.n) * a.nchunk * gn_row(a);
   const double D = static_cast<double>(a.S) * a.cpg;
   for (int first = 0; first < ng; first += wide) {
     const int gi = first + threadIdx.x - ph * wide, g = p.g0 + gi;
@@ -144,7 +144,7 @@ __device__ __forceinline__ float* gn_gather(float* sh, const GnArgs& a, const Gn
         const int width = a.t.ncol > 1 ? min((cc + 1) * w, (g + 1) * a.cpg) - max(cc * w, g * a.cpg) : a.cpg;
 #pragma unroll 8
         for (int k = ph; k < a.nchunk; k += np) {
-          const float2 e = image[(static_cast<size_t>(k) * a.t.ncol + cc) * a.G + g];
+          const float2 e = image[static_cast<size_t>(k) * gn_row(a) + g + cc];
           if (STATS) {
             const double cnt = static_cast<double>(gn_rows(a, k)) * width, m = e.x;
             s0 += cnt * m;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce(const T* __restrict__ gy, c
     }
     A = gn_lane_sum(A, lanes);
     B = gn_lane_sum(B, lanes);
-    if (sub == 0) pg[((static_cast<size_t>(p.n) * a.nchunk + p.chunk) * a.t.ncol + p.cc) * a.G + g] = make_float2(A, B);
+    if (sub == 0) pg[(static_cast<size_t>(p.n) * a.nchunk + p.chunk) * gn_row(a) + g + p.cc] = make_float2(A, B);
   }
 }
 
@@ -432,16 +432,16 @@ bool gn_ok(int dtype, int N, long long S, int C, int G) {
 // a launch holds fewer than 2^32 threads
 bool gn_grid_ok(int N, const GnArgs& a) { return static_cast<long long>(N) * a.nchunk * a.t.ncol * a.t.threads < (1LL << 32) - (1LL << 26); }
 
-// chunk rows for whatever vector width a call ends up with: N * nchunk <= GN_BLOCKS / ncol + N
+// the chunk rows of whatever element type and vector width a call ends up with (the backward's: C sums, then the groups')
 size_t gn_ws(int N, long long S, int C, int G) {
   size_t m = gn_one_bytes(N, S, C, G);
-  for (int v : {1, 2, 4, 8}) {
-    if (C % v != 0) continue;
-    const A8Tile t = a8_tile(C, v);
-    const size_t rows = static_cast<size_t>(GN_BLOCKS / t.ncol) + static_cast<size_t>(N) + 1;
-    const size_t b = rows * (static_cast<size_t>(C) + static_cast<size_t>(t.ncol) * G) * sizeof(float2);
-    m = b > m ? b : m;
-  }
+  for (int esize : {2, 4})
+    for (int v = 16 / esize; v >= 1; v /= 2) {
+      if (C % v != 0) continue;
+      const GnArgs a = gn_args(N, S, C, G, v, esize);
+      const size_t b = static_cast<size_t>(N) * a.nchunk * (static_cast<size_t>(C) + gn_row(a)) * sizeof(float2);
+      m = b > m ? b : m;
+    }
   return m;
 }
 

@@ -44,3 +44,12 @@ def test_the_sizes_of_the_tests_take_the_forms_that_they_are_meant_for():
         assert _form(torch.float32, N, S, C, G) == 1 and _form(torch.float32, N, S, C, G, None, True) == 0
     assert _form(torch.float32, 2, 513, 32, 4) == 0 and _form(torch.float32, 2, 512, 32, 4) == 1
     assert _form(torch.float32, 2, 12, 33, 4) == -1 and _form(torch.float32, 0, 12, 32, 4) == -1
+
+
+@pytest.mark.parametrize("fmt", [None, "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,S,H,C,G", [(1, 40, 4, 3000, 3000), (2, 33, 3, 2058, 343), (1, 70, 7, 1030, 10), (2, 21, 3, 4104, 27), (1, 12, 3, 65536, 65536)])
+def test_groups_across_column_ranges(N, S, H, C, G, dtype, fmt):
+    """rows of several workgroups' channels: groups of one channel, groups that lie in two ranges, a group in many"""
+    assert _form(dtype, N, S, C, G, fmt, True) == 0
+    _check(N, S, H, C, G, dtype, fmt)

@@ -302,3 +302,14 @@ def test_modules_with_hooks_and_stacks_with_a_forward_of_their_own_are_not_folde
             GN.fuse_gn_act_modules(m, "int8")
             A.use_act8(m)
             assert torch.allclose(m(x), ref, atol=1e-6) and len(seen) == 2 and torch.allclose(seen[0], seen[1], atol=1e-6)
+
+
+def test_group_norm_workspace_follows_the_call():
+    """a chunk's row is 8 bytes a channel and 8 a group (and a border of column ranges); sizes for the widest to the narrowest access.  It was
+    4096 rows of every group in every range: 9.4 MB for a map of 180 KB, ten gigabytes for a group a channel"""
+    from distill_bev_amd import _lib as L
+    size = L.lib().dbev_gn_act_workspace_bytes
+    for N, S, C, G in ((6, 176, 256, 32), (6, 375, 256, 32), (1, 1024, 16384, 16384), (64, 16, 4096, 4096), (64, 16, 65536, 65536), (2, 600, 80, 16)):
+        assert 0 < size(N, S, C, G) <= 4 * N * S * C, (N, S, C, G)
+    for N, S, C, G in ((40000, 1, 256, 32), (3, 2, 33, 3)):                # one row an image at least: 16 bytes a channel and group
+        assert 0 < size(N, S, C, G) <= 8 * N * (C + G + -(-C // 256))

@@ -25,6 +25,7 @@ transform to the stock operators (device tensors are counted in the fallback led
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch._prims_common import suggest_memory_format
 from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
@@ -443,6 +444,15 @@ def conv1x1_stats(conv, x, kernel):
     return _Conv1x1_8.apply(x, conv.weight, None, conv.act8_format, True, kernel)
 
 
+def conv1x1_module(conv, x):
+    """the forward of a 1x1 convolution module that `keeps` x: conv1x1 in the layout that F.conv2d would give (contiguous unless the map or the
+    filter is channels-last)"""
+    y = conv1x1(x, conv.weight, conv.bias, conv.act8_format)
+    if x.is_contiguous(memory_format=torch.channels_last) or suggest_memory_format(conv.weight) == torch.channels_last:
+        return y
+    return y.contiguous()
+
+
 def keeps(conv, x):
     """does this call of a 1x1 convolution module keep x as an 8-bit checkpoint?  For code that runs a module's product without its forward
     (nets.Bottleneck, colsum.conv_bn_cancelled_bias)"""
@@ -495,8 +505,8 @@ class Act8Conv2d(Bf6Conv2d):
     act8_format = "int8"
 
     def forward(self, x):
-        if _recording(self.weight) and _plain_1x1(self) and x.dim() == 4 and x.numel() and _module_ready(x, self.weight, self.bias):
-            return conv1x1(x, self.weight, self.bias, self.act8_format)
+        if keeps(self, x):
+            return conv1x1_module(self, x)
         return super().forward(x)
 
     def extra_repr(self):

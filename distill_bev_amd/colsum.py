@@ -86,7 +86,7 @@ class BiasSumConv2d(nn.Conv2d):
         if self.act8_format is not None:
             from . import act8
             if act8.keeps(self, x):
-                return act8.conv1x1(x, self.weight, self.bias, self.act8_format)
+                return act8.conv1x1_module(self, x)
         if (self.bias is not None and self.padding_mode == "zeros" and torch.is_tensor(x) and x.is_cuda
                 and x.dtype == torch.float32 and _nhwc(x) and x.numel() > 0 and not isinstance(self.padding, str)):
             from . import gemm_bf6 as G                       # a 1x1 layer the bf16x6 GEMM takes: its kernels + this module's bias handling

@@ -195,3 +195,25 @@ def test_gelu_of_every_fp16_value_is_the_neighbour_only_where_fp32_cannot_tell()
     sure = tie > err
     assert float(sure.double().mean()) > 1 - 1 / 300
     assert torch.equal(A.activation(x.to(DEV), "gelu").cpu()[sure], y.half()[sure])
+
+
+def test_convolution_modules_give_the_layout_of_the_stock_ones():
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd.colsum import BiasSumConv2d, use_bias_sum_convs
+    for bias, cls in ((True, A.Act8Conv2d), (False, A.Act8Conv2d), (True, BiasSumConv2d)):
+        for wfmt in (torch.contiguous_format, torch.channels_last):
+            for xfmt in (torch.contiguous_format, torch.channels_last):
+                torch.manual_seed(4)
+                stock, mod = nn.Conv2d(16, 24, 1, bias=bias).to(DEV), nn.Conv2d(16, 24, 1, bias=bias).to(DEV)
+                mod.load_state_dict(stock.state_dict())
+                for m in (stock, mod):
+                    m.weight.data = m.weight.data.contiguous(memory_format=wfmt)
+                if cls is BiasSumConv2d:
+                    assert use_bias_sum_convs(mod) == 1
+                A.use_act8(mod)
+                assert type(mod) is cls and mod.act8_format == "int8"
+                x = torch.randn(2, 16, 5, 6, device=DEV).contiguous(memory_format=xfmt).requires_grad_(True)
+                y, ref = mod(x), stock(x)
+                assert torch.allclose(y, ref, atol=1e-5) and y.stride() == ref.stride(), (cls, wfmt, xfmt, y.stride(), ref.stride())
+                a, b = torch.autograd.grad(y.sum(), (x,))[0], torch.autograd.grad(ref.sum(), (x,))[0]
+                assert torch.allclose(a, b, atol=1e-5)

@@ -531,8 +531,9 @@ class Act8Activation(nn.Module):
 
 
 def hooked(m):
-    """has somebody registered hooks on this module?  They would not run if the module were left out, or see other values if it did more"""
-    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+    """has somebody registered hooks on this module, or given it a forward of its own?  They would not run if the module were left out, or see
+    other values if it did more"""
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or "forward" in m.__dict__)
 
 
 def act_name(m):
@@ -551,8 +552,8 @@ def act_name(m):
 def use_act8(model, fmt="int8"):
     """Let the plain Linear and 1x1 / stride-1 convolution modules of `model` (bf16x6 ones included) keep their input as an 8-bit checkpoint,
     and the activations whose input nothing else keeps: every SiLU / GELU, and a ReLU right behind one of those layers in an nn.Sequential
-    (elsewhere a ReLU's output is kept by the layer behind it anyway; one that carries hooks stays as it is).  nn.MultiheadAttention reads its projections' weights itself and
-    stays as it is.  Returns how many modules changed class.  Idempotent for one format.
+    (elsewhere a ReLU's output is kept by the layer behind it anyway; one that carries hooks stays as it is).  nn.MultiheadAttention reads
+    its projections' weights itself and stays as it is.  Returns how many modules changed class.  Idempotent for one format.
     The biased 1x1 layers of a model that has been through train_step.accelerate_modules (BiasSumConv2d) stay what they are and are given the
     format; two kernels that take such a layer as a whole keep its input their own way: the depth head's and the adaptation loss's."""
     from .colsum import BiasSumConv2d

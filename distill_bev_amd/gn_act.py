@@ -244,9 +244,9 @@ def fuse_gn_act_modules(model, checkpoint=None):
     """Rewire the nn.GroupNorm modules of nn.Sequential stacks and ConvModules onto the kernels, together with the ReLU / SiLU / GELU right
     behind them (replaced by nn.Identity; keys unchanged); other GroupNorm modules become GroupNormAct without an activation (the residual
     blocks of nets.py put theirs in by `norm_act`).
-    A norm that several places share, or that carries hooks, keeps the activations behind it as modules, and so do one with hooks of its own and
-    stacks whose forward is not the class's.  `checkpoint`: the format in which all norms of the model
-    keep their input; None leaves that to each norm (a GroupNormAct's own `act8_format`; plain norms keep x).  Returns how many norms changed.  Idempotent."""
+    A norm that several places share, or that carries hooks, keeps the activation behind it as a module; so does an activation with hooks, and a
+    stack whose forward is not its class's.  `checkpoint`: the format in which all norms of the model keep their input; None leaves that to
+    each norm (a GroupNormAct's own `act8_format`; plain norms keep x).  Returns how many norms changed.  Idempotent."""
     from .registry import ConvModule
     from .wino import ConvNormSequential
     if checkpoint is not None:
@@ -265,6 +265,8 @@ def fuse_gn_act_modules(model, checkpoint=None):
         return places[id(norm)] == 1 and not A.hooked(norm)
 
     for mod in list(model.modules()):
+        if "forward" in mod.__dict__:
+            continue
         if type(mod).forward in (nn.Sequential.forward, ConvNormSequential.forward):
             kids = list(mod._modules.items())
             for (_, a), (kb, b) in zip(kids, kids[1:]):

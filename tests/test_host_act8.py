@@ -313,3 +313,19 @@ def test_group_norm_workspace_follows_the_call():
         assert 0 < size(N, S, C, G) <= 4 * N * S * C, (N, S, C, G)
     for N, S, C, G in ((40000, 1, 256, 32), (3, 2, 33, 3)):                # one row an image at least: 16 bytes a channel and group
         assert 0 < size(N, S, C, G) <= 8 * N * (C + G + -(-C // 256))
+
+
+def test_forwards_given_to_instances_are_not_folded_away():
+    """as libraries that wrap modules do: module.forward = wrapper(module.forward)"""
+    from distill_bev_amd import act8 as A
+    from distill_bev_amd import gn_act as GN
+    x = torch.randn(2, 8, 4, 5)
+    for at in (None, 0, 1):
+        m = nn.Sequential(nn.GroupNorm(2, 8), nn.SiLU())
+        ref = m(x)
+        seen, target = [], m if at is None else m[at]
+        inner = target.forward
+        target.forward = lambda t: seen.append(1) or inner(t)
+        GN.fuse_gn_act_modules(m)
+        A.use_act8(m)
+        assert torch.allclose(m(x), ref, atol=1e-6) and len(seen) == 1

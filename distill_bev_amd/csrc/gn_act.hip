@@ -432,16 +432,16 @@ bool gn_ok(int dtype, int N, long long S, int C, int G) {
 // a launch holds fewer than 2^32 threads
 bool gn_grid_ok(int N, const GnArgs& a) { return static_cast<long long>(N) * a.nchunk * a.t.ncol * a.t.threads < (1LL << 32) - (1LL << 26); }
 
-// the chunk rows of whatever element type and vector width a call ends up with (the backward's: C sums, then the groups')
+// the chunk rows of whatever element type and vector width a call ends up with (the backward's: C sums, then the groups'); fp32 has at least as
+// many chunks as the 16-bit types
 size_t gn_ws(int N, long long S, int C, int G) {
   size_t m = gn_one_bytes(N, S, C, G);
-  for (int esize : {2, 4})
-    for (int v = 16 / esize; v >= 1; v /= 2) {
-      if (C % v != 0) continue;
-      const GnArgs a = gn_args(N, S, C, G, v, esize);
-      const size_t b = static_cast<size_t>(N) * a.nchunk * (static_cast<size_t>(C) + gn_row(a)) * sizeof(float2);
-      m = b > m ? b : m;
-    }
+  for (int v : {1, 2, 4, 8}) {
+    if (C % v != 0) break;
+    const GnArgs a = gn_args(N, S, C, G, v, sizeof(float));
+    const size_t b = static_cast<size_t>(N) * a.nchunk * (static_cast<size_t>(C) + gn_row(a)) * sizeof(float2);
+    m = b > m ? b : m;
+  }
   return m;
 }
 

@@ -14,7 +14,8 @@ costs the rounding of the values that the GRADIENTS see (the forward pass itself
 
 Formats: with a = max |x| of a block of 32 channels and one power of two 2^k per block,
     "int8"   k = floor(log2 a) - 6: whole numbers -127..127; |x - x^| <= 2^(k-1) (2^k where clamped), i.e. a / 128 (a / 64)
-    "e4m3"   k = floor(log2 a) - 8 or -7: floats with four significant bits; |x - x^| <= |x| / 16 down to a / 2^14
+    "e4m3"   k = floor(log2 a) - 8 or -7: floats with four significant bits; |x - x^| <= |x| / 16 down to a / 2^14; the topmost values of a
+             type, above 63488 in fp16 and 248 * 2^120 in fp32 and bf16, round up to an infinity of it
 int8 is the finer one for values that fill their block's range, e4m3 for blocks with outliers.  A block that holds an infinity or a NaN
 restores as NaN.  ReLU's derivative is taken at x^, where a positive value below half of the smallest code is zero.
 

@@ -4,7 +4,9 @@
 // Checkpoint format: rows x C values, 32 neighbouring channels of a row (fewer in a row's last block) share one power of two 2^k, kept
 // as the byte k + 127; a value is one byte, either a signed whole number (int8, -127..127) or an e4m3 float, times 2^k.
 //   int8   k = floor(log2 amax) - 6: codes 64..127 at the top of the block, |x - x^| <= 2^(k-1) (2^k where the code is clamped to 127)
-//   e4m3   k = floor(log2 amax) - 8, one more when amax > 448 * 2^k: nothing saturates, |x - x^| <= 2^-4 |x| down to 2^(k-6)
+//   e4m3   k = floor(log2 amax) - 8, one more when amax > 448 * 2^k: no code saturates, |x - x^| <= 2^-4 |x| down to 2^(k-6).  Rounding up to
+//          256 * 2^k can leave the type: fp16 values above 63488 restore as 2^16, an infinity in fp16, fp32's and bf16's above 248 * 2^120 as
+//          2^128, an infinity.  (int8 rounds down to 127 * 2^k there)
 // Multiplying by 2^-k is exact, so the one rounding (to nearest, ties to even) is the code itself and every correct implementation
 // gives the same bytes; the restored value has at most 8 significant bits, i.e. it IS a bf16 number -- the weight gradient feeds it to
 // the bf16 matrix cores unsplit.  A block that holds an infinity or a NaN gets the byte 255 and restores as NaN throughout: an overflow

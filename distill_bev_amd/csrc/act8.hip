@@ -5,8 +5,8 @@
 //   a8_act_fwd   y = act(x), and x's checkpoint            reads n * es, writes n * es + 1.03 n: the checkpoint costs no pass of its own
 //   a8_act_bwd   dx = dy * act'(x^)                        reads n * es + 1.03 n, writes n * es
 // All four are bound by HBM traffic: 5.5 to 7.3 TB/s of the bytes above on 70 to 280 million values, where a copy reaches 5.1 to 5.4 (270000 x 512
-// fp32, us: pack 107, unpack 96, SiLU forward 183, backward 186; GELU 185 / 203), but for GELU in 16-bit types, which VALU work holds
-// (69633 x 1024 bf16: SiLU 65 / 66, GELU 65 / 78; 540000 x 512: 226 / 222, 240 / 264).
+// fp32, us: pack 107, unpack 96, SiLU forward 183, backward 185; GELU 184 / 202), but for GELU in 16-bit types, which VALU work holds
+// (69633 x 1024 bf16: SiLU 65 / 67, GELU 66 / 79; 540000 x 512: 236 / 222, 242 / 262).
 // A lane holds 16 bytes of a row (4, 2 or 1 elements where the row length, the stride or an address is off), the 32 channels of a block are
 // 4 (16-bit types) or 8 (fp32) neighbouring lanes and their maximum is taken with DPP moves; a thread keeps its column and handles A8_U
 // rows, all loads first.  Dense rows of a multiple of 32 channels are walked as rows of 32: every access of a wave is then one contiguous

@@ -16,9 +16,11 @@
 // shares, partial sums [share][Co][Ci] are added in a fixed order by a8_wsum: bit-reproducible, no atomics.
 //
 // Measured, fp32 gy (bf16 gy), both launches, int8: 40000 rows, 256 -> 512: 49 us (35); 33792, 1024 -> 256: 68 us (45); 540672, 64 -> 256: 137 us
-// (76, 4.3 TB/s); the fp32 library product alone takes 470 us on the first.  What bounds the first: its 92 MB come at 4.7 TB/s while the chunks
-// run (0.95 us each; their matrix instructions are 0.64 us of that at 2.4 GHz, busy 40 % of the launch), then 32 MB of partial sums go out
-// and come back: 43 + 6.5 us.  Two workgroups a CU (64 MB of partial sums): 43 + 12 us; tiles of 128 x 128: 61 us; two teams of waves on
+// (76, 4.3 TB/s); the fp32 library product alone takes 470 us on the first: 42 + 6.5 us.  Its 20 chunks a share take 0.95 us each (0.64 of
+// that matrix instructions at 2.4 GHz), 19 of the 42 us; the rest has not been taken apart: the launch's ramp, three cold fetches before the
+// first chunk, and 128 KB a workgroup of partial sums in 4-byte stores, 33 MB that go out and come back.  16-bit gradients have a third or two
+// thirds of the matrix work and half the bytes, but the same plan and so the same partial sums, more than their inputs: 35 us in bf16, where
+// 51 MB of input take 10.  Two workgroups a CU (64 MB of partial sums): 43 + 12 us; tiles of 128 x 128: 61 us; two teams of waves on
 // one tile, or the whole chunk ordered as one block: 44 us; four bytes a row of a lane's codes written with a swizzle by 16 channels: 330
 // cycles of LDS conflicts a chunk, by 8: none.
 #include "act8.h"

@@ -15,7 +15,7 @@
 // Bound by HBM: 3 n es forward and 5 n es backward (n es = bytes of x; with a checkpoint the two reads of x in the backward are 1.03
 // bytes a value).  All sums have a fixed order: run-to-run bit-identical, no atomics.
 // Measured, fp32, SiLU: 1 x 128 x 1024 x 1024 forward 290 us (1.6 GB in three passes: 5.6 TB/s, part of the second read comes from the
-// memory-side cache), backward 446; 8 x 128 x 128 x 128, int8 kept: 28 + 28 and 24 + 27 us, half of it cache; 6 x 256 x 15 x 25 backward: 7 + 7
+// memory-side cache), backward 446; 8 x 128 x 128 x 128, int8 kept: 22 + 28 and 24 + 27 us, half of it cache; 6 x 256 x 15 x 25 backward: 7 + 7
 // us, launch and merge latency.
 #include "gn_act.h"
 #include "gn_one.h"

@@ -7,11 +7,11 @@
 // registers.  The image's last tiles collect, four groups a workgroup: all T pairs of a group in fp64 in a fixed order, and publish the totals.
 //
 // Measured at 48 x 256 x 64 x 176 (forward / backward, us; in brackets the two launches a direction of gn_act.hip):
-//   fp32                 no activation 227 / 394 (300 / 481)   SiLU 224 / 450 (299 / 484)   GELU 234 / 471 (308 / 488)
-//   fp32, int8 kept      no activation 240 / 304 (327 / 334)   SiLU 246 / 317 (328 / 342)   GELU 266 / 333 (331 / 347)
-//   bf16 (forward only)  no activation 134 (166)   SiLU 143 (163)   GELU 158 (179); int8 kept 152 (187)   156 (190)   172 (201)
-// i.e. the forward moves its floor of 2 n es (+ 1.03 n) bytes at 4.7 to 5.2 TB/s in fp32 where a copy reaches 5.3, the backward at 3.8 to 4.2;
-// GELU in bf16 (3.6) and the backward are held by VALU work (some 30 instructions an element) that a workgroup's phases overlap with the
+//   fp32                 no activation 229 / 388 (300 / 481)   SiLU 228 / 451 (299 / 484)   GELU 236 / 471 (308 / 488)
+//   fp32, int8 kept      no activation 241 / 301 (327 / 334)   SiLU 249 / 314 (328 / 342)   GELU 262 / 333 (331 / 347)
+//   bf16 (forward only)  no activation 142 (166)   SiLU 145 (163)   GELU 160 (179); int8 kept 154 (187)   162 (190)   179 (201)
+// i.e. the forward moves its floor of 2 n es (+ 1.03 n) bytes at 4.7 to 5.1 TB/s in fp32 where a copy reaches 5.3, the backward at 3.5 to 4.3;
+// GELU in bf16 (3.5) and the backward are held by VALU work (some 30 instructions an element) that a workgroup's phases overlap with the
 // transfers only in part.
 //
 // These tensors are as large as the memory-side cache or larger: they are read and written past it (nontemporal).  With an operator that
@@ -660,7 +660,7 @@ int gn_one_cus() {
 
 // One pass where it is the faster way: rows wide enough to fill a workgroup, an image of 2 to 512 tiles and at most half of what the device
 // holds (four a CU), so that another image's transfer covers one's wait, and 2048 tiles or more in all: below, the two extra launches eat
-// the gain (8 x 128 x 128 x 128 fp32, 1024 tiles: forward 41 us against 57 of GPU time but two launches more for the host, backward 63
+// the gain (8 x 128 x 128 x 128 fp32, 1024 tiles: forward 41 us against 50 of GPU time but two launches more for the host, backward 63
 // against 56).
 bool gn_one_plan(int dtype, int N, long long S, int C, int vec, int R, GnArgs* a, int* T) {
   const int wide = dtype == DBEV_DT_F32 ? 4 : 8;

@@ -946,6 +946,7 @@ int dbev_gemm1x1_backward_weight(const float* x_nhwc, const float* grad_y_nhwc, 
  *   With a = max |x| of a block: DBEV_ACT8_INT8 k = floor(log2 a) - 6, code = clamp(rne(x / 2^k), -127, 127) in two's complement;
  *   DBEV_ACT8_E4M3 k = floor(log2 a) - 8, one more if a > 448 * 2^k, code = the e4m3 float nearest to x / 2^k (ties to even); k >= -127,
  *   scale byte k + 127.  A block with an infinity or a NaN has scale byte 255 and restores as NaN.
+ *   (e4m3 rounds the topmost 3 % of a type's range up to 2^16 (fp16) or 2^128, which is an infinity in that type.)
  *   dbev_act8_pack                  x -> codes, scales
  *   dbev_act8_unpack                out[rows, C] (dense, `dtype`) = the values the codes stand for, rounded to `dtype`
  *   dbev_act8_activation_forward    y[rows, C] (dense) = act(x), and x's checkpoint in the same pass (fmt DBEV_ACT8_NONE: y only, codes and

@@ -178,10 +178,10 @@ def _ready(x, gn):
         why = f"dtype {x.dtype}"
     elif torch.is_autocast_enabled("cuda"):
         why = "autocast"
-    elif not _fits(x.shape[0], x.shape[1], x.numel() // (x.shape[0] * x.shape[1])):
-        why = f"size {tuple(x.shape)}"
     elif A.transformed():
         why = "traced or transformed"
+    elif not _fits(x.shape[0], x.shape[1], x.numel() // (x.shape[0] * x.shape[1])):
+        why = f"size {tuple(x.shape)}"
     if why:
         L.note_fallback("gn_act", why)
     return why is None

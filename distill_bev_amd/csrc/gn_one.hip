@@ -314,13 +314,17 @@ __device__ __forceinline__ void gn_one_stats(typename GnRaw<T, V>::type* raw, co
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = fmaf(-static_cast<float>(p.nv), ref[i], s[i]);
+  if (p.on && p.rp == 0) {                                    // for the group's mean below, without another load
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (p.col * V + i == gr[i] * a.cpg) out[2 * gr[i] + 1] = ref[i];
+  }
   gn_one_fold<V, 1>(sh, a, p, s, s);
   for (int g = threadIdx.x / lanes; g < a.G; g += blockDim.x / lanes) {
-    const float r = static_cast<float>(x0[g * a.cpg]);
     float m = 0.f;
     for (int c = sub; c < a.cpg; c += lanes) m += sh[g * a.cpg + c];
     m = gn_lane_sum(m, lanes);
-    if (sub == 0) out[2 * g] = r + m / (static_cast<float>(rows) * static_cast<float>(a.cpg));
+    if (sub == 0) out[2 * g] = out[2 * g + 1] + m / (static_cast<float>(rows) * static_cast<float>(a.cpg));
   }
   __syncthreads();
   float mu[V];

@@ -751,8 +751,8 @@ size_t gn_one_bytes(int N, long long S, int C, int G) {
 // Small images: W channels (whole groups, whole blocks of 32, or all of them), at most GN_RF rows a thread (fp32, 32 channels: 512 pixels); wider
 // while every thread still has a row of its own, and, with several rows a thread, while two workgroups a CU remain (5000 x 256 x 4 x 4, fp32 /
 // bf16: 109 / 112 us with 64 channels a workgroup, 37 / 62 with all; 500 x 256 x 8 x 8 27 / 43 -> 14 / 17).  Against the two launches, without an
-// activation, us a call: fp32 6 x 256 x 8 x 22 13 (16), 48 x 512 x 22 x 22 18 (34), 200 x 256 x 16 x 32 35 (60), 1000 x 256 x 4 x 4 14 (17), 5000 x 256 x 4 x 4
-// 37 (58), 40000 images of one pixel 195 (272); bf16 13 (16), 19 (27), 37 (48), 15 (22), 62 (84), 399 (460)
+// activation, us a call: fp32 6 x 256 x 8 x 22 13 (16), 48 x 512 x 22 x 22 18 (34), 200 x 256 x 16 x 32 35 (60), 1000 x 256 x 4 x 4 13 (17), 5000 x 256 x 4 x 4
+// 38 (58), 40000 images of one pixel 227 (287); bf16 13 (16), 19 (27), 22 (48), 15 (22), 60 (84), 424 (481)
 bool gn_small_plan(int dtype, int N, long long S, int C, int G, int vec, GnArgs* a, int* W) {
   const int wide = dtype == DBEV_DT_F32 ? 4 : 8, cpg = C / G;
   if (vec != wide || S > 256 * GN_RF) return false;
